@@ -115,7 +115,7 @@ def _plan_parts(n_seqs, max_rows, page):
     start = HEADER
     seq = start + _round4(n_seqs + 1)
     step = _round4(max_rows)
-    return start, seq, seq + step, seq + 2 * step, seq + 3 * step, seq + 3 * step + max_rows // page + 2 * n_seqs
+    return start, seq, seq + step, seq + 2 * step, seq + 3 * step, seq + 3 * step + 4 * (max_rows // page + 2 * n_seqs)
 
 
 def _codes(gen, fmt, shape):
@@ -270,10 +270,11 @@ def _plain_step(s, new):
     for o, v in ((o_seq, seq), (o_pos, pos), (o_slot, slot)):
         s.plan[o:o + _round4(s.max_rows)] = -1
         s.plan[o:o + s.max_rows] = torch.where(live, v, -1).to(torch.int32)
-    n_jobs = end - o_job
-    jobs = torch.full((n_jobs + 1,), -1, dtype=torch.int32, device="cuda")
-    jobs.scatter_(0, torch.where(leads, torch.cumsum(leads.long(), 0) - 1, n_jobs), torch.where(leads, row, -1).to(torch.int32))
-    s.plan[o_job:end] = jobs[:n_jobs]
+    n_jobs = (end - o_job) // 4
+    jobs = torch.full((n_jobs + 1, 4), -1, dtype=torch.int32, device="cuda")
+    record = torch.stack([row, torch.minimum(page - pos % page, ends[seq] - row), slot, pos], 1)
+    jobs[torch.where(leads, torch.cumsum(leads.long(), 0) - 1, n_jobs)] = torch.where(leads[:, None], record, -1).to(torch.int32)
+    s.plan[o_job:end] = jobs[:n_jobs].reshape(-1)
     s.plan[1], s.plan[2], s.plan[3] = total, leads.sum(), s.free[0]
     s.lens[:] = after
 
@@ -449,8 +450,8 @@ def work(case):
     if kind == "tables":
         n, rows = case["seqs"], case["seqs"] * (case["new"] if case["new"] == 1 else case["new"] / 2)
         turned = n * (case["new"] + case["back"]) / 2 / page
-        # lengths twice, counts twice, the table entries and stack words of the pages that move, three words a row, a job a page
-        return dict(bytes=4 * (5 * n + 4 * turned + 3 * rows + rows / page + n), flops=0)
+        # lengths twice, counts twice, the table entries and stack words of the pages that move, three words a row, four a touched page
+        return dict(bytes=4 * (5 * n + 4 * turned + 3 * rows + 4 * (rows / page + n)), flops=0)
     n_kv, hd = case["n_kv"], case["hd"]
     size = 4 if case["act"] == "f32" else 2
     if kind == "attention":
