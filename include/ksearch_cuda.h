@@ -34,7 +34,8 @@ typedef struct ks_ctx ks_ctx;
 typedef struct ks_buf ks_buf;
 
 /* crates/ksearch_ir/src/lib.rs:17-74 (DType and packed byte sizes) */
-typedef enum { KS_F32 = 0, KS_F16 = 1, KS_Q4K = 2, KS_Q6K = 3, KS_Q40 = 4, KS_Q5K = 5 } ks_dtype;  /* Q5K: dequant, row gather and load-time requantisation only */
+typedef enum { KS_F32 = 0, KS_F16 = 1, KS_Q4K = 2, KS_Q6K = 3, KS_Q40 = 4, KS_Q5K = 5,  /* Q5K: dequant, row gather and load-time requantisation only */
+               KS_I8 = 6, KS_E4M3 = 7 } ks_dtype;                                           /* codes of a paged cache only */
 
 typedef enum {
   KS_OK = 0,
@@ -211,6 +212,77 @@ int ks_sdpa_decode(ks_ctx* ctx, size_t n_slots, size_t n_q, size_t n_kv, size_t 
                    const ks_buf* V, size_t kv_byte_off, size_t slot_stride_bytes, const ks_buf* meta,
                    ks_buf* tmp, ks_buf* out, int n_splits);
 
+/* ---- a paged KV cache in 8 bits ---------------------------------------------------------------------------------------
+ * No counterpart in the reference, whose KvPool (KV:24-230) gives every slot a contiguous Q4_0 cache.  Here sequences hold
+ * pages of `page` positions out of one pool, handed out on the GPU, and a value is one byte times a scale that a page
+ * keeps for each KV head.  Everything below enqueues on the context's stream and can be captured into a graph; lengths,
+ * tables and plans live on the device, so one captured step serves every length.
+ *
+ * Index errors in device data (a table entry outside the pool, a slot outside the cache, a row the RoPE table does not
+ * reach, more rows of a sequence than rows_most) touch nothing out of range: the rows concerned are left out and the next
+ * ks_synchronize returns KS_ERR_INVALID. */
+#define KS_PAGES_MAX_SEQS 1024
+#define KS_PAGES_PLAN_HEADER 8
+typedef struct {
+  size_t n_seqs;      /* sequences, 1..KS_PAGES_MAX_SEQS */
+  size_t max_blocks;  /* pages a sequence may hold */
+  size_t n_pages;     /* pages of the pool */
+  size_t page;        /* positions of a page: 16, 32, 64 or 128; n_pages * page and max_blocks * page below 2^31 */
+  size_t max_rows;    /* new rows of one step, all sequences together: 1..2^20 */
+  ks_buf* lens;       /* int32 [n_seqs]: positions a sequence holds */
+  ks_buf* tables;     /* int32 [n_seqs, max_blocks]: its pages, -1 behind them */
+  ks_buf* free_pages; /* int32 [1 + n_pages]: how many pages are free, then the stack of their ids (the last is handed out first) */
+  ks_buf* plan;       /* int32 [ks_pages_plan_ints()]: what the last step put where */
+} ks_page_tables;
+typedef struct {
+  size_t n_pages, page, n_kv, hd;  /* hd: 64, 128 or 256 */
+  ks_dtype dtype;                  /* KS_I8: codes -127..127; KS_E4M3: 1.4.3 floats up to 448 (the NaN patterns read as 448) */
+  ks_buf *k, *v;                   /* codes [n_pages, n_kv, page, hd], on 16 bytes */
+  ks_buf *k_scale, *v_scale;       /* f32 [n_pages, n_kv]; value = code * scale; taken as at least 2^-100 and at most 2^100 */
+} ks_q8_cache;
+/* A plan: int32 words.  Header: [0] status (below), [1] rows, [2] touched pages (jobs), [3] pages free after the step, [4..7] zero;
+ * then, each part from a multiple of 4 words on: row_start [n_seqs + 1] (rows of sequence i: row_start[i] .. row_start[i + 1] - 1),
+ * row_seq, row_pos, row_slot [max_rows] (sequence, position and cache slot page_id * page + position % page of a row; -1 behind
+ * the last), jobs [max_rows / page + 2 n_seqs][4] (for each touched page: its first row, how many rows of the step lie in it, the first
+ * row's slot and position; -1 behind the last).  The plan starts on 16 bytes. */
+enum { KS_PLAN_ROW_START = 0, KS_PLAN_ROW_SEQ = 1, KS_PLAN_ROW_POS = 2, KS_PLAN_ROW_SLOT = 3, KS_PLAN_JOBS = 4, KS_PLAN_END = 5 };
+size_t ks_pages_plan_offset(size_t n_seqs, size_t max_rows, size_t page, int part);  /* first word of a part; 0 for arguments out of range */
+size_t ks_pages_plan_ints(size_t n_seqs, size_t max_rows, size_t page);              /* words of a plan (= offset of KS_PLAN_END) */
+/* Empties everything: no sequence holds a position, every page is free (0 is handed out first), the plan has no rows. */
+int ks_pages_reset(ks_ctx* ctx, const ks_page_tables* t);
+/* n_new int32 [n_seqs] rows more for each sequence (0: none): pages for them, tables, lengths and the plan.  New pages go to the
+ * sequences in order, a sequence's blocks in order.  All or nothing: with a status other than 0 lengths, tables and stack stay
+ * and the plan has no rows, so that what is enqueued behind it does nothing.  Status 1: not enough free pages, 2: a sequence
+ * would outgrow its table, 3: more rows than max_rows, 4: a count below 0 or a length outside the table (the highest that holds). */
+enum { KS_PLAN_OK = 0, KS_PLAN_NO_PAGES = 1, KS_PLAN_TABLE_FULL = 2, KS_PLAN_TOO_MANY_ROWS = 3, KS_PLAN_BAD_LENGTH = 4 };
+int ks_pages_step(ks_ctx* ctx, const ks_page_tables* t, const ks_buf* n_new);
+/* keep int32 [n_seqs]: sequence i ends at keep[i] positions if it holds more (0: it is released; below 0: left as it is); the
+ * pages behind go back on the stack, the last page first, so that the step that took them can be taken back exactly. */
+int ks_pages_trim(ks_ctx* ctx, const ks_page_tables* t, const ks_buf* keep);
+/* Rows k, v [max_rows, n_kv, hd] in `act`, kv_ld elements apart (a multiple of 8, at least n_kv * hd; offsets multiples of 8), into
+ * the slots of the plan; rows behind the plan's last are not read.  A page's scale is the least power of two that makes its largest
+ * finite value fit the codes (at least 2^-100); it starts anew with position 0 of the page and never shrinks until then: where new
+ * rows need a larger one, the codes of the page's earlier rows are rounded again.  Codes are rounded to nearest, ties to even;
+ * infinities become the largest code, NaN becomes 0. */
+int ks_kv_append_q8(ks_ctx* ctx, const ks_q8_cache* c, const ks_page_tables* t, ks_dtype act, const ks_buf* k, size_t k_off,
+                    const ks_buf* v, size_t v_off, size_t kv_ld);
+/* ks_rmsnorm_per_head_qkv_q40 over such a cache: q per-head RMS * qw and RoPE -> q_out [max_rows, n_q, hd], k RMS * kw and RoPE, v RMS,
+ * both appended as ks_kv_append_q8 does.  Row r turns by row row_pos[r] of rope, f32 [*, hd] = cos[hd / 2] || sin[hd / 2]. */
+int ks_rmsnorm_per_head_qkv_q8(ks_ctx* ctx, const ks_q8_cache* c, const ks_page_tables* t, size_t n_q, float eps, ks_dtype act, const ks_buf* q,
+                               const ks_buf* qw, const ks_buf* rope, const ks_buf* k, const ks_buf* kw, const ks_buf* v, ks_buf* q_out);
+/* Cached rows as numbers: k, v [n_rows, n_kv, hd] in `act` (f16: rounded to nearest) of slots int32 [n_rows] from element slot_off on,
+ * for instance a plan's row_slot; rows of slot -1 are left as they are. */
+int ks_kv_read_q8(ks_ctx* ctx, const ks_q8_cache* c, size_t n_rows, const ks_buf* slots, size_t slot_off, ks_dtype act, ks_buf* k, ks_buf* v);
+/* Attention of a plan's rows over the cache.  q, out: [max_rows, n_q, hd], which must not overlap; n_q a multiple of n_kv, at most 64
+ * query heads a KV head.  Row r of a sequence of `len` positions and `rows` rows is position p = len - rows + r and sees positions
+ * max(0, p - window + 1) .. p (window 0: all up to p), so the lengths are those AFTER the step; a row that sees none gets zeros.  Scores are
+ * scale * (q . k).  Only row_start, the lengths and the tables are read: a host may write its own.  rows_most: no sequence has
+ * more rows (0: nothing is done); ctx_most: the longest context to expect (a hint for how the work is split).  Rows behind the last
+ * sequence are left as they are.  tmp: ks_sdpa_paged_tmp_floats() f32, not shared with work that may overlap. */
+size_t ks_sdpa_paged_tmp_floats(const ks_ctx* ctx, const ks_q8_cache* c, const ks_page_tables* t, size_t n_q, size_t rows_most);
+int ks_sdpa_paged_q8(ks_ctx* ctx, const ks_q8_cache* c, const ks_page_tables* t, size_t n_q, size_t rows_most, size_t ctx_most, size_t window,
+                     float scale, ks_dtype act, const ks_buf* q, ks_buf* tmp, ks_buf* out);
+
 /* ---- small ops ------------------------------------------------------------ */
 /* K:1181 quantize_q40: n values (n % 32 == 0) -> Q4_0 at dst + dst_byte_off. */
 int ks_quantize_q40(ks_ctx* ctx, size_t n, ks_dtype act, const ks_buf* src, size_t src_off, ks_buf* dst,
@@ -355,6 +427,9 @@ int ks_debug_sdpa_chunk(ks_ctx* ctx, size_t n_q, size_t n_kv, size_t hd, size_t 
 /* Test hook, no GPU needed: do n prompt rows behind `base` positions (seen through a window, if > 0) share their context?  *span = tiles of
  * 64 positions that the launch which decodes them covers, if they do. */
 int ks_debug_prompt_pass(int n_q, int n_kv, int hd, int max_seq, int window, int n, int base, unsigned* span);
+/* Test hook, no GPU needed: a context without a device.  Calls of the paged cache check their arguments on it and are refused with
+ * KS_ERR_UNSUPPORTED ("no device") where they would launch; buffers can be wrapped, nothing else works.  Ends with ks_ctx_destroy. */
+ks_ctx* ks_debug_ctx_checks_only(void);
 /* Test hook, no GPU needed: decoded tiles a model of these sizes takes memory for where free_bytes are left, spare of which it may not
  * touch; 0: none, its prompts go row by row. */
 size_t ks_debug_image_tiles(int n_kv, int hd, int max_seq, int n_slots, size_t free_bytes, size_t spare);

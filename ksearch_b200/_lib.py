@@ -13,7 +13,7 @@ PKG = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(PKG, "libksearch_cuda.so")
 HEADER = os.path.join(os.path.dirname(PKG), "include", "ksearch_cuda.h")
 
-F32, F16, Q4K, Q6K, Q40, Q5K = 0, 1, 2, 3, 4, 5
+F32, F16, Q4K, Q6K, Q40, Q5K, I8, E4M3 = 0, 1, 2, 3, 4, 5, 6, 7
 OK, ERR_INVALID, ERR_CUDA, ERR_OOM, ERR_UNSUPPORTED, ERR_STATE, ERR_TIMEOUT = 0, -1, -2, -3, -4, -5, -6
 
 _sz, _i, _f, _vp, _u64 = C.c_size_t, C.c_int, C.c_float, C.c_void_p, C.c_uint64
@@ -78,6 +78,16 @@ SIGNATURES = {
     "ks_softcap_argmax": (_i, [_vp, _sz, _f, _i, _vp, _vp, _sz]),
     "ks_softcap_argmax_noalloc": (_i, [_i, _vp, _sz, _f, _vp, _vp]),
     "ks_gelu_mul": (_i, [_vp, _sz, _i, _vp, _vp, _vp]),
+    "ks_pages_plan_offset": (_sz, [_sz, _sz, _sz, _i]),
+    "ks_pages_plan_ints": (_sz, [_sz, _sz, _sz]),
+    "ks_pages_reset": (_i, [_vp, _vp]),
+    "ks_pages_step": (_i, [_vp, _vp, _vp]),
+    "ks_pages_trim": (_i, [_vp, _vp, _vp]),
+    "ks_kv_append_q8": (_i, [_vp, _vp, _vp, _i, _vp, _sz, _vp, _sz, _sz]),
+    "ks_rmsnorm_per_head_qkv_q8": (_i, [_vp, _vp, _vp, _sz, _f, _i, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "ks_kv_read_q8": (_i, [_vp, _vp, _sz, _vp, _sz, _i, _vp, _vp]),
+    "ks_sdpa_paged_tmp_floats": (_sz, [_vp, _vp, _vp, _sz, _sz]),
+    "ks_sdpa_paged_q8": (_i, [_vp, _vp, _vp, _sz, _sz, _sz, _sz, _f, _i, _vp, _vp, _vp]),
     "ks_model_create": (_vp, [_vp, _vp]),
     "ks_model_destroy": (None, [_vp]),
     "ks_model_warm_plans": (_i, [_vp, _i]),
@@ -126,6 +136,7 @@ SIGNATURES = {
     "ks_model_debug_graphs": (_i, [_vp]),
     "ks_debug_sdpa_chunk": (_i, [_vp, _sz, _sz, _sz, _sz, _f, _i, _vp, _vp, _sz, _vp, _vp, _vp, _vp, _vp, _i]),
     "ks_debug_prompt_pass": (_i, [_i, _i, _i, _i, _i, _i, _i, _vp]),
+    "ks_debug_ctx_checks_only": (_vp, []),
     "ks_debug_image_tiles": (_sz, [_i, _i, _i, _i, _sz, _sz]),
     "ks_debug_decode_ring": (_i, [_i, _i, _i, _i, _i, _i, _i, _sz, _i, _vp, _vp, _i]),
     "ks_comm_unique_id": (_i, [_vp]),
@@ -148,6 +159,18 @@ SIGNATURES = {
 class Plan(C.Structure):
     """ks_plan of include/ksearch_cuda.h"""
     _fields_ = [("variant", _i), ("nr", _i), ("nwarps", _i), ("ctas_per_sm", _i), ("ms", _f)]
+
+
+class PageTablesStruct(C.Structure):
+    """ks_page_tables of include/ksearch_cuda.h"""
+    _fields_ = [("n_seqs", _sz), ("max_blocks", _sz), ("n_pages", _sz), ("page", _sz), ("max_rows", _sz),
+                ("lens", _vp), ("tables", _vp), ("free_pages", _vp), ("plan", _vp)]
+
+
+class Q8CacheStruct(C.Structure):
+    """ks_q8_cache of include/ksearch_cuda.h"""
+    _fields_ = [("n_pages", _sz), ("page", _sz), ("n_kv", _sz), ("hd", _sz), ("dtype", _i),
+                ("k", _vp), ("v", _vp), ("k_scale", _vp), ("v_scale", _vp)]
 
 
 _lib = None

@@ -67,7 +67,7 @@ ks_ctx* ks_ctx_create(int device, uint64_t flags) {
     delete c;
     return nullptr;
   }
-  if (cudaMalloc(&c->ws, 16384) != cudaSuccess || cudaMemset(c->ws, 0, 16384) != cudaSuccess || cudaMalloc(&c->gemm_ws, KS_FEW_WS) != cudaSuccess) {
+  if (cudaMalloc(&c->ws, KS_WS_BYTES) != cudaSuccess || cudaMemset(c->ws, 0, KS_WS_BYTES) != cudaSuccess || cudaMalloc(&c->gemm_ws, KS_FEW_WS) != cudaSuccess) {
     g_create_err = "workspace allocation failed";
     cudaFree(c->ws);
     cudaStreamDestroy(c->stream);
@@ -78,8 +78,18 @@ ks_ctx* ks_ctx_create(int device, uint64_t flags) {
   return c;
 }
 
+ks_ctx* ks_debug_ctx_checks_only(void) {
+  ks_ctx* c = new ks_ctx();
+  c->device = -1;
+  return c;
+}
+
 void ks_ctx_destroy(ks_ctx* c) {
   if (!c) return;
+  if (c->device < 0) {
+    delete c;
+    return;
+  }
   cudaSetDevice(c->device);
   cudaStreamSynchronize(c->stream);
   for (cudaEvent_t ev : c->inflight) cudaEventDestroy(ev);
@@ -222,12 +232,17 @@ int ks_synchronize(ks_ctx* c) {
   for (cudaEvent_t ev : c->inflight) cudaEventDestroy(ev);
   c->inflight.clear();
   // a kernel whose bounded wait gave up leaves a mark instead of hanging
-  unsigned flag = 0;
-  KS_CUDA(c, cudaMemcpy(&flag, (unsigned*)c->ws + KS_WS_ERR_WORD, sizeof flag, cudaMemcpyDeviceToHost));
+  unsigned words[KS_WS_INDEX_WORD - KS_WS_ERR_WORD + 1] = {0};
+  KS_CUDA(c, cudaMemcpy(words, (unsigned*)c->ws + KS_WS_ERR_WORD, sizeof words, cudaMemcpyDeviceToHost));
+  const unsigned flag = words[0], index = words[KS_WS_INDEX_WORD - KS_WS_ERR_WORD];
+  if (index) cudaMemset((unsigned*)c->ws + KS_WS_INDEX_WORD, 0, sizeof index);
   if (flag) {
     cudaMemset((unsigned*)c->ws + KS_WS_ERR_WORD, 0, sizeof flag);
     return ks_fail(c, KS_ERR_TIMEOUT, "a device-side wait gave up (status word 0x%x)", flag);
   }
+  if (index)
+    return ks_fail(c, KS_ERR_INVALID, "paged cache: an index on the device is out of range:%s%s%s%s%s", index & KS_BAD_PAGE ? " page id" : "", index & KS_BAD_SLOT ? " slot" : "",
+                   index & KS_BAD_POSITION ? " position behind the RoPE table" : "", index & KS_BAD_ROWS ? " rows of a sequence" : "", index & KS_BAD_STACK ? " free stack" : "");
   return KS_OK;
 }
 

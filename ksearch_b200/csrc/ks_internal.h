@@ -78,6 +78,19 @@ static inline size_t ks_nbytes(ks_dtype d, size_t n) {
   return n / ks_block_elems(d) * ks_block_bytes(d);
 }
 
+// The context's device for as long as it lives: callers may have another one current.
+struct ks_on_device {
+  int was = -1;
+  explicit ks_on_device(const ks_ctx* ctx) {
+    if (cudaGetDevice(&was) != cudaSuccess) was = -1;
+    if (was != ctx->device) cudaSetDevice(ctx->device);
+    else was = -1;
+  }
+  ~ks_on_device() {
+    if (was >= 0) cudaSetDevice(was);
+  }
+};
+
 // Range check of (buffer, byte offset, byte extent).
 static inline bool ks_fits(const ks_buf* b, size_t off, size_t extent) {
   return b && b->dptr && off <= b->bytes && extent <= b->bytes - off;
@@ -135,6 +148,11 @@ int ks_launch_matvec_q4k_fx(ks_ctx* ctx, const ks_mv_seg* segs, int n_seg, ks_mv
 // Device error word raised by a kernel whose bounded wait gave up (index into ctx->ws, in words).
 #define KS_WS_ERR_WORD 4000
 #define KS_WS_FENCE_WORD 4001  // cleared behind the load-time quantiser and otherwise unused
+#define KS_WS_INDEX_WORD 4002  // an index in device data was out of range: KS_BAD_*; ks_synchronize reports and clears it
+enum { KS_BAD_PAGE = 1u, KS_BAD_SLOT = 2u, KS_BAD_POSITION = 4u, KS_BAD_ROWS = 8u, KS_BAD_STACK = 16u };
+#define KS_WS_COUNT_WORD 4096  // from here on: arrival counters of launches whose last block finishes the work; zero between launches
+#define KS_WS_COUNT_MOST 4096u
+#define KS_WS_BYTES ((KS_WS_COUNT_WORD + KS_WS_COUNT_MOST) * 4u)
 
 int ks_launch_rmsnorm(ks_ctx* ctx, size_t n, size_t rows, float eps, ks_dtype act, const void* x, const void* w,
                       const void* res, int has_scale, float scale, void* y);

@@ -1,0 +1,389 @@
+// Rows into and out of a paged 8-bit cache: append as they are, append behind the per-head norms and RoPE, read back.
+//
+// A block of the append takes the new rows of one page for one KV head, K or V.  With a = max |x| of its finite values it sets
+//   s = 2^e, the least e with a <= qmax 2^e   (qmax 127 or 448, e in -100 .. 100),   s = max(s, scale of the page) unless the page starts here,
+// writes rne(x / s), and rounds the page's earlier codes again by (old scale) / s where s grew.  Scales are powers of two so that the
+// division is exact: codes depend on nothing but the values, whatever the order of the operations around them, and however often a
+// scale doubles the error that re-rounding adds stays below one step in all (1/2 + 1/4 + ...); with a / qmax as the scale every new maximum
+// would add half a step.  The price is up to one bit of the int8 codes (none of e4m3's mantissa).
+#include <cuda_fp16.h>
+
+#include "ks_q8.h"
+#include "ks_q8.cuh"
+
+namespace {
+
+constexpr int kRowsPerWarp = 8;  // rows of a page a warp keeps in registers between their maximum and their codes
+
+struct AppendArgs {
+  uint8_t *kc, *vc;      // codes [n_pages, n_kv, page, hd]
+  float *ks, *vs;        // scales [n_pages, n_kv]
+  const int* plan;
+  ks_plan_layout at;
+  unsigned max_rows, page_log, n_kv, n_jobs;
+  unsigned n_slots;      // n_pages * page
+  const void *k, *v;
+  size_t kv_ld;
+  unsigned* bad;
+  // behind the norms
+  const void *q, *qw, *kw;
+  void* q_out;
+  const float* rope;
+  unsigned n_q, rope_rows;
+  float eps;
+};
+
+template <int V, typename T>
+__device__ __forceinline__ void load_act(const T* p, float (&x)[V]) {
+  if constexpr (sizeof(T) == 4) {
+    if constexpr (V == 4) {
+      const float4 a = *reinterpret_cast<const float4*>(p);
+      x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
+    } else if constexpr (V == 2) {
+      const float2 a = *reinterpret_cast<const float2*>(p);
+      x[0] = a.x; x[1] = a.y;
+    } else {
+      x[0] = *p;
+    }
+  } else {
+    if constexpr (V == 4) {
+      const uint2 a = *reinterpret_cast<const uint2*>(p);
+      const float2 u = __half22float2(q8_h2(a.x)), w = __half22float2(q8_h2(a.y));
+      x[0] = u.x; x[1] = u.y; x[2] = w.x; x[3] = w.y;
+    } else if constexpr (V == 2) {
+      const float2 u = __half22float2(*reinterpret_cast<const __half2*>(p));
+      x[0] = u.x; x[1] = u.y;
+    } else {
+      x[0] = __half2float(*p);
+    }
+  }
+}
+template <int V, typename T>
+__device__ __forceinline__ void store_act(T* p, const float (&x)[V]) {
+  if constexpr (sizeof(T) == 4) {
+    if constexpr (V == 4) *reinterpret_cast<float4*>(p) = make_float4(x[0], x[1], x[2], x[3]);
+    else if constexpr (V == 2) *reinterpret_cast<float2*>(p) = make_float2(x[0], x[1]);
+    else *p = x[0];
+  } else {
+    if constexpr (V == 4) {
+      uint2 a;
+      a.x = q8_u32(__floats2half2_rn(x[0], x[1]));
+      a.y = q8_u32(__floats2half2_rn(x[2], x[3]));
+      *reinterpret_cast<uint2*>(p) = a;
+    } else if constexpr (V == 2) {
+      *reinterpret_cast<__half2*>(p) = __floats2half2_rn(x[0], x[1]);
+    } else {
+      *p = __float2half_rn(x[0]);
+    }
+  }
+}
+template <int V, bool FP8>
+__device__ __forceinline__ void store_codes(uint8_t* p, const float (&x)[V], float inv) {
+  if constexpr (V == 4) {
+    *reinterpret_cast<uint32_t*>(p) = q8_encode2<FP8>(x[0] * inv, x[1] * inv) | q8_encode2<FP8>(x[2] * inv, x[3] * inv) << 16;
+  } else if constexpr (V == 2) {
+    *reinterpret_cast<unsigned short*>(p) = (unsigned short)q8_encode2<FP8>(x[0] * inv, x[1] * inv);
+  } else {
+    *p = (uint8_t)q8_encode2<FP8>(x[0] * inv, 0.0f);
+  }
+}
+
+// One head of one row behind its norm and RoPE (w == nullptr: the norm alone, as V has it).  A lane holds dims V lane.. of both halves, so
+// RoPE partners sit in one lane.
+template <int HD, int V, typename T>
+__device__ __forceinline__ void norm_rope(float (&x)[2][V], float eps, const T* w, const float* cs) {
+  float ss = 0.0f;
+#pragma unroll
+  for (int e = 0; e < V; e++) ss = fmaf(x[0][e], x[0][e], fmaf(x[1][e], x[1][e], ss));
+  ss = q8_warp_sum(ss);
+  const float inv = 1.0f / sqrtf(ss / (float)HD + eps);
+  if (w == nullptr) {
+#pragma unroll
+    for (int e = 0; e < V; e++) {
+      x[0][e] *= inv;
+      x[1][e] *= inv;
+    }
+    return;
+  }
+  float w0[V], w1[V], c[V], s[V];
+  load_act<V, T>(w, w0);
+  load_act<V, T>(w + HD / 2, w1);
+  load_act<V, float>(cs, c);
+  load_act<V, float>(cs + HD / 2, s);
+#pragma unroll
+  for (int e = 0; e < V; e++) {
+    const float a = __fmul_rn(__fmul_rn(x[0][e], inv), w0[e]), b = __fmul_rn(__fmul_rn(x[1][e], inv), w1[e]);
+    x[0][e] = __fsub_rn(__fmul_rn(a, c[e]), __fmul_rn(b, s[e]));
+    x[1][e] = __fadd_rn(__fmul_rn(a, s[e]), __fmul_rn(b, c[e]));
+  }
+}
+
+// Grid: (touched pages x n_kv x 2) blocks of page / 8 warps, K and V of a head next to each other; NORM: behind them the blocks of the
+// query heads, four (row, head) pairs a warp.
+template <int HD, typename T, bool FP8, bool NORM>
+__global__ void __launch_bounds__(512) append_q8_kernel(const AppendArgs a) {
+  constexpr int V = HD / 64;
+  __shared__ float red[16];
+  ks_pdl_entry();
+  const unsigned lane = threadIdx.x & 31u, warp = threadIdx.x >> 5, nwarp = blockDim.x >> 5;
+  const unsigned page = 1u << a.page_log, per_job = 2u * a.n_kv;
+  if (NORM && blockIdx.x >= a.n_jobs * per_job) {
+    const unsigned rows = min((unsigned)max(a.plan[1], 0), a.max_rows), items = rows * a.n_q;
+    const unsigned it0 = ((blockIdx.x - a.n_jobs * per_job) * nwarp + warp) * 4u;
+    float x[4][2][V];
+    int pos[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const unsigned it = it0 + i;
+      if (it >= items) continue;
+      const T* src = (const T*)a.q + (size_t)it * HD + lane * V;
+      load_act<V, T>(src, x[i][0]);
+      load_act<V, T>(src + HD / 2, x[i][1]);
+      pos[i] = a.plan[a.at.row_pos + it / a.n_q];
+    }
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const unsigned it = it0 + i;
+      if (it >= items) continue;
+      if ((unsigned)pos[i] >= a.rope_rows) {
+        if (lane == 0) atomicOr(a.bad, KS_BAD_POSITION);
+        continue;
+      }
+      norm_rope<HD, V, T>(x[i], a.eps, (const T*)a.qw + lane * V, a.rope + (size_t)pos[i] * HD + lane * V);
+      T* dst = (T*)a.q_out + (size_t)it * HD + lane * V;
+      store_act<V, T>(dst, x[i][0]);
+      store_act<V, T>(dst + HD / 2, x[i][1]);
+    }
+    return;
+  }
+  const unsigned j = blockIdx.x / per_job, head = blockIdx.x % per_job >> 1;
+  const bool vals = blockIdx.x & 1u;
+  const int4 job = reinterpret_cast<const int4*>(a.plan + a.at.jobs)[j];
+  if (job.x < 0) return;
+  const unsigned row0 = (unsigned)job.x, rows = (unsigned)job.y, slot = (unsigned)job.z, off = slot & (page - 1u);
+  if (job.z < 0 || slot >= a.n_slots || rows > page - off || row0 >= a.max_rows || rows > a.max_rows - row0) {
+    if (threadIdx.x == 0) atomicOr(a.bad, KS_BAD_SLOT);
+    return;
+  }
+  if (NORM && !vals && ((unsigned)job.w >= a.rope_rows || rows > a.rope_rows - (unsigned)job.w)) {
+    if (threadIdx.x == 0) atomicOr(a.bad, KS_BAD_POSITION);
+    return;
+  }
+  const size_t block = (size_t)(slot >> a.page_log) * a.n_kv + head;
+  float* scale_at = (vals ? a.vs : a.ks) + block;
+  const float held = off ? q8_scale(*scale_at) : 0.0f;
+  const T* src = (const T*)(vals ? a.v : a.k) + (size_t)row0 * a.kv_ld + (size_t)head * HD + lane * V;
+  float x[kRowsPerWarp][2][V], amax = 0.0f;
+#pragma unroll
+  for (int i = 0; i < kRowsPerWarp; i++) {
+    const unsigned r = warp + (unsigned)i * nwarp;
+    if (r >= rows) continue;
+    load_act<V, T>(src + (size_t)r * a.kv_ld, x[i][0]);
+    load_act<V, T>(src + (size_t)r * a.kv_ld + HD / 2, x[i][1]);
+  }
+#pragma unroll
+  for (int i = 0; i < kRowsPerWarp; i++) {
+    const unsigned r = warp + (unsigned)i * nwarp;
+    if (r >= rows) continue;
+    if constexpr (NORM) norm_rope<HD, V, T>(x[i], a.eps, vals ? (const T*)nullptr : (const T*)a.kw + lane * V, a.rope + (size_t)((unsigned)job.w + r) * HD + lane * V);
+#pragma unroll
+    for (int e = 0; e < 2 * V; e++) {
+      float& y = x[i][e / V][e % V];
+      const float m = fabsf(y);
+      if (m < INFINITY) amax = fmaxf(amax, m);
+      if (y != y) y = 0.0f;
+    }
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+  if (lane == 0) red[warp] = amax;
+  __syncthreads();
+  for (unsigned w = 0; w < nwarp; w++) amax = fmaxf(amax, red[w]);
+  const float s = fmaxf(q8_scale_for<FP8>(amax), q8_power_above(held)), inv = 1.0f / s;  // (powers of two: exact)
+  uint8_t* codes = (vals ? a.vc : a.kc) + (block << a.page_log) * HD;
+  if (off && s != held) {  // the page's earlier rows under the larger scale
+    const float turn = held * inv;
+    for (unsigned i = threadIdx.x; i < off * (HD / 4u); i += blockDim.x) {
+      uint32_t* at = reinterpret_cast<uint32_t*>(codes) + i;
+      const uint32_t w = *at;
+      const float2 lo = q8_decode2f<FP8>(w), hi = q8_decode2f<FP8>(w >> 16);
+      *at = q8_encode2<FP8>(lo.x * turn, lo.y * turn) | q8_encode2<FP8>(hi.x * turn, hi.y * turn) << 16;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < kRowsPerWarp; i++) {
+    const unsigned r = warp + (unsigned)i * nwarp;
+    if (r >= rows) continue;
+    uint8_t* dst = codes + (size_t)(off + r) * HD + lane * V;
+    store_codes<V, FP8>(dst, x[i][0], inv);
+    store_codes<V, FP8>(dst + HD / 2, x[i][1], inv);
+  }
+  if (threadIdx.x == 0 && s != held) *scale_at = s;
+}
+
+// Eight codes a thread; K and V in blockIdx.y.
+template <typename T, bool FP8>
+__global__ void __launch_bounds__(256) read_q8_kernel(const uint8_t* kc, const uint8_t* vc, const float* ks, const float* vs, unsigned hd_log, unsigned n_kv, unsigned page_log,
+                                                      unsigned n_slots, unsigned n_rows, const int* slots, T* k, T* v, unsigned* bad) {
+  ks_pdl_entry();
+  const uint8_t* codes = blockIdx.y ? vc : kc;
+  const float* scales = blockIdx.y ? vs : ks;
+  T* out = blockIdx.y ? v : k;
+  const unsigned chunk_log = hd_log - 3u, per_row = n_kv << chunk_log;
+  const size_t n = (size_t)n_rows * per_row, step = (size_t)gridDim.x * blockDim.x;
+  for (size_t i = (size_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += step) {
+    const unsigned row = (unsigned)(i / per_row), rest = (unsigned)(i - (size_t)row * per_row), head = rest >> chunk_log, c = rest & ((1u << chunk_log) - 1u);
+    const int slot = slots[row];
+    if (slot == -1) continue;
+    if ((unsigned)slot >= n_slots) {
+      atomicOr(bad, KS_BAD_SLOT);
+      continue;
+    }
+    const size_t block = (size_t)((unsigned)slot >> page_log) * n_kv + head;
+    const float s = q8_scale(scales[block]);
+    const uint2 w = *reinterpret_cast<const uint2*>(codes + ((((block << page_log) + ((unsigned)slot & ((1u << page_log) - 1u))) << hd_log) + 8u * c));
+    const float2 f0 = q8_decode2f<FP8>(w.x), f1 = q8_decode2f<FP8>(w.x >> 16), f2 = q8_decode2f<FP8>(w.y), f3 = q8_decode2f<FP8>(w.y >> 16);
+    const float lo[4] = {f0.x * s, f0.y * s, f1.x * s, f1.y * s}, hi[4] = {f2.x * s, f2.y * s, f3.x * s, f3.y * s};
+    store_act<4, T>(out + i * 8, lo);
+    store_act<4, T>(out + i * 8 + 4, hi);
+  }
+}
+
+AppendArgs append_args(ks_ctx* ctx, const ks_q8_cache* c, const ks_page_tables* t) {
+  AppendArgs a{};
+  a.kc = (uint8_t*)c->k->dptr;
+  a.vc = (uint8_t*)c->v->dptr;
+  a.ks = (float*)c->k_scale->dptr;
+  a.vs = (float*)c->v_scale->dptr;
+  a.plan = (const int*)t->plan->dptr;
+  a.at = ks_plan_parts(t->n_seqs, t->max_rows, t->page);
+  a.max_rows = (unsigned)t->max_rows;
+  a.page_log = (unsigned)__builtin_ctzll(c->page);
+  a.n_kv = (unsigned)c->n_kv;
+  a.n_jobs = a.at.n_jobs < a.max_rows ? a.at.n_jobs : a.max_rows;  // (a touched page has a row)
+  a.n_slots = (unsigned)(c->n_pages * c->page);
+  a.bad = (unsigned*)ctx->ws + KS_WS_INDEX_WORD;
+  return a;
+}
+
+template <bool NORM>
+int launch_append(ks_ctx* ctx, const ks_q8_cache* c, ks_dtype act, const AppendArgs& a, const char* who) {
+  const unsigned warps = (unsigned)c->page / kRowsPerWarp;
+  size_t blocks = (size_t)a.n_jobs * 2 * a.n_kv;
+  if (NORM) blocks += ((size_t)a.max_rows * a.n_q + 4 * warps - 1) / (4 * warps);
+  KS_REQUIRE(ctx, blocks < (1u << 31), "%s: too many rows and heads for one launch", who);
+  KS_REQUIRE_DEVICE(ctx, who);
+  ks_on_device on(ctx);
+#define KS_AP(HD_, T_, F_) KS_LAUNCH(ctx, (append_q8_kernel<HD_, T_, F_, NORM>), (unsigned)blocks, warps * 32, 0, a)
+#define KS_AP_T(HD_, F_) do { if (act == KS_F32) KS_AP(HD_, float, F_); else KS_AP(HD_, __half, F_); } while (0)
+#define KS_AP_F(HD_) do { if (c->dtype == KS_E4M3) KS_AP_T(HD_, true); else KS_AP_T(HD_, false); } while (0)
+  if (c->hd == 256) KS_AP_F(256);
+  else if (c->hd == 128) KS_AP_F(128);
+  else KS_AP_F(64);
+#undef KS_AP_F
+#undef KS_AP_T
+#undef KS_AP
+  return ks_after_launch(ctx, who);
+}
+
+}  // namespace
+
+int ks_check_cache(ks_ctx* ctx, const char* who, const ks_q8_cache* c, const ks_page_tables* t) {
+  KS_REQUIRE(ctx, c, "%s: null cache", who);
+  if (c->dtype != KS_I8 && c->dtype != KS_E4M3) return ks_fail(ctx, KS_ERR_UNSUPPORTED, "%s: cache dtype %d not supported (I8, E4M3)", who, (int)c->dtype);
+  if (c->hd != 64 && c->hd != 128 && c->hd != 256) return ks_fail(ctx, KS_ERR_UNSUPPORTED, "%s: head_dim %zu not supported (64, 128, 256)", who, c->hd);
+  KS_REQUIRE(ctx, ks_page_ok(c->page), "%s: pages of %zu positions not supported (16, 32, 64, 128)", who, c->page);
+  KS_REQUIRE(ctx, c->n_kv >= 1 && c->n_kv <= 1024, "%s: n_kv=%zu outside 1..1024", who, c->n_kv);
+  KS_REQUIRE(ctx, c->n_pages >= 1 && c->n_pages <= 0x7FFFFFFFu / c->page, "%s: %zu pages: at least one, and below 2^31 positions", who, c->n_pages);
+  if (t) KS_REQUIRE(ctx, t->n_pages == c->n_pages && t->page == c->page, "%s: the tables hand out %zu pages of %zu positions, the cache has %zu of %zu", who, t->n_pages, t->page, c->n_pages, c->page);
+  const size_t blocks = c->n_pages * c->n_kv;
+  KS_REQUIRE(ctx, ks_fits(c->k, 0, blocks * c->page * c->hd) && ks_fits(c->v, 0, blocks * c->page * c->hd), "%s: cache buffer too small for %zu pages", who, c->n_pages);
+  KS_REQUIRE(ctx, ks_fits(c->k_scale, 0, blocks * 4) && ks_fits(c->v_scale, 0, blocks * 4), "%s: scale buffer too small for %zu pages", who, c->n_pages);
+  KS_REQUIRE(ctx, ks_aligned(c->k, 16) && ks_aligned(c->v, 16) && ks_aligned(c->k_scale, 4) && ks_aligned(c->v_scale, 4), "%s: codes must start on 16 bytes, scales on 4", who);
+  return KS_OK;
+}
+
+extern "C" {
+
+int ks_kv_append_q8(ks_ctx* ctx, const ks_q8_cache* c, const ks_page_tables* t, ks_dtype act, const ks_buf* k, size_t k_off, const ks_buf* v, size_t v_off, size_t kv_ld) {
+  if (!ctx) return KS_ERR_INVALID;
+  int rc = ks_check_tables(ctx, "kv_append_q8", t);
+  if (!rc) rc = ks_check_cache(ctx, "kv_append_q8", c, t);
+  if (rc) return rc;
+  KS_REQUIRE(ctx, ks_is_act(act), "kv_append_q8: activation dtype must be F32 or F16");
+  const size_t ab = ks_act_bytes(act), width = c->n_kv * c->hd;
+  KS_REQUIRE(ctx, kv_ld >= width && kv_ld % 8 == 0 && kv_ld < (size_t(1) << 32) && k_off % 8 == 0 && v_off % 8 == 0, "kv_append_q8: rows %zu apart at offsets %zu, %zu: multiples of 8, rows at least n_kv * hd = %zu apart",
+             kv_ld, k_off, v_off, width);
+  const size_t need = ((t->max_rows - 1) * kv_ld + width) * ab;
+  KS_REQUIRE(ctx, k_off < (size_t(1) << 48) && v_off < (size_t(1) << 48) && ks_fits(k, k_off * ab, need) && ks_fits(v, v_off * ab, need), "kv_append_q8: k/v buffer too small for %zu rows", t->max_rows);
+  KS_REQUIRE(ctx, ks_aligned(k, 16) && ks_aligned(v, 16), "kv_append_q8: k and v must start on 16 bytes");
+  AppendArgs a = append_args(ctx, c, t);
+  a.k = (const uint8_t*)k->dptr + k_off * ab;
+  a.v = (const uint8_t*)v->dptr + v_off * ab;
+  a.kv_ld = kv_ld;
+  return launch_append<false>(ctx, c, act, a, "kv_append_q8");
+}
+
+int ks_rmsnorm_per_head_qkv_q8(ks_ctx* ctx, const ks_q8_cache* c, const ks_page_tables* t, size_t n_q, float eps, ks_dtype act, const ks_buf* q, const ks_buf* qw, const ks_buf* rope,
+                               const ks_buf* k, const ks_buf* kw, const ks_buf* v, ks_buf* q_out) {
+  if (!ctx) return KS_ERR_INVALID;
+  static const char who[] = "rmsnorm_per_head_qkv_q8";
+  int rc = ks_check_tables(ctx, who, t);
+  if (!rc) rc = ks_check_cache(ctx, who, c, t);
+  if (rc) return rc;
+  KS_REQUIRE(ctx, ks_is_act(act), "%s: activation dtype must be F32 or F16", who);
+  KS_REQUIRE(ctx, n_q >= 1 && n_q <= 65536 && n_q * t->max_rows < (1u << 30), "%s: bad query head count %zu", who, n_q);
+  const size_t ab = ks_act_bytes(act), q_bytes = t->max_rows * n_q * c->hd * ab, kv_bytes = t->max_rows * c->n_kv * c->hd * ab;
+  KS_REQUIRE(ctx, ks_fits(q, 0, q_bytes) && ks_fits(q_out, 0, q_bytes), "%s: q buffer too small for %zu rows", who, t->max_rows);
+  KS_REQUIRE(ctx, ks_fits(k, 0, kv_bytes) && ks_fits(v, 0, kv_bytes), "%s: k/v buffer too small for %zu rows", who, t->max_rows);
+  KS_REQUIRE(ctx, ks_fits(qw, 0, c->hd * ab) && ks_fits(kw, 0, c->hd * ab), "%s: norm weight too small", who);
+  KS_REQUIRE(ctx, ks_fits(rope, 0, c->hd * 4), "%s: rope table too small", who);
+  KS_REQUIRE(ctx, ks_aligned(q, 16) && ks_aligned(q_out, 16) && ks_aligned(k, 16) && ks_aligned(v, 16) && ks_aligned(qw, 16) && ks_aligned(kw, 16) && ks_aligned(rope, 16),
+             "%s: operands must start on 16 bytes", who);
+  AppendArgs a = append_args(ctx, c, t);
+  a.k = k->dptr;
+  a.v = v->dptr;
+  a.kv_ld = c->n_kv * c->hd;
+  a.q = q->dptr;
+  a.qw = qw->dptr;
+  a.kw = kw->dptr;
+  a.q_out = q_out->dptr;
+  a.rope = (const float*)rope->dptr;
+  const size_t rope_rows = rope->bytes / (c->hd * 4);
+  a.rope_rows = (unsigned)(rope_rows < 0x7FFFFFFFu ? rope_rows : 0x7FFFFFFFu);
+  a.n_q = (unsigned)n_q;
+  a.eps = eps;
+  return launch_append<true>(ctx, c, act, a, who);
+}
+
+int ks_kv_read_q8(ks_ctx* ctx, const ks_q8_cache* c, size_t n_rows, const ks_buf* slots, size_t slot_off, ks_dtype act, ks_buf* k, ks_buf* v) {
+  if (!ctx) return KS_ERR_INVALID;
+  int rc = ks_check_cache(ctx, "kv_read_q8", c, nullptr);
+  if (rc) return rc;
+  KS_REQUIRE(ctx, ks_is_act(act), "kv_read_q8: activation dtype must be F32 or F16");
+  KS_REQUIRE(ctx, n_rows >= 1 && n_rows < (1u << 31), "kv_read_q8: n_rows=%zu outside 1..2^31 - 1", n_rows);
+  KS_REQUIRE(ctx, slot_off < (size_t(1) << 48) && ks_fits(slots, slot_off * 4, n_rows * 4) && ks_aligned(slots, 4), "kv_read_q8: slots buffer too small for %zu rows, or not on 4 bytes", n_rows);
+  const size_t bytes = n_rows * c->n_kv * c->hd * ks_act_bytes(act);
+  KS_REQUIRE(ctx, ks_fits(k, 0, bytes) && ks_fits(v, 0, bytes) && ks_aligned(k, 16) && ks_aligned(v, 16), "kv_read_q8: k/v buffer too small for %zu rows, or not on 16 bytes", n_rows);
+  KS_REQUIRE_DEVICE(ctx, "kv_read_q8");
+  ks_on_device on(ctx);
+  const size_t items = n_rows * c->n_kv * c->hd / 8;
+  const size_t most = (size_t)ctx->sm_count * 8, blocks = (items + 255) / 256;
+  const dim3 grid((unsigned)(blocks < most ? blocks : most), 2);
+  const int* at = (const int*)slots->dptr + slot_off;
+  const unsigned hd_log = (unsigned)__builtin_ctzll(c->hd), page_log = (unsigned)__builtin_ctzll(c->page);
+  unsigned* bad = (unsigned*)ctx->ws + KS_WS_INDEX_WORD;
+#define KS_RD(T_, F_) KS_LAUNCH(ctx, (read_q8_kernel<T_, F_>), grid, 256, 0, (const uint8_t*)c->k->dptr, (const uint8_t*)c->v->dptr, (const float*)c->k_scale->dptr, \
+                                (const float*)c->v_scale->dptr, hd_log, (unsigned)c->n_kv, page_log, (unsigned)(c->n_pages * c->page), (unsigned)n_rows, at, (T_*)k->dptr, (T_*)v->dptr, bad)
+  if (act == KS_F32) {
+    if (c->dtype == KS_E4M3) KS_RD(float, true);
+    else KS_RD(float, false);
+  } else {
+    if (c->dtype == KS_E4M3) KS_RD(__half, true);
+    else KS_RD(__half, false);
+  }
+#undef KS_RD
+  return ks_after_launch(ctx, "kv_read_q8");
+}
+
+}  // extern "C"

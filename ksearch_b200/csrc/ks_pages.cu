@@ -1,0 +1,281 @@
+// Pages of a paged cache handed out on the GPU: tables, lengths, the stack of free pages and the plan of a step's rows.
+//
+// A step is integer arithmetic on three exclusive sums over the sequences (rows, new pages, touched pages) and one record per row, so it
+// is bound by latency: one trip for lengths and counts, the sums, one trip for a row's page, the stores.  Every block makes the sums
+// for itself and takes a run of rows; nothing that a block reads is written by another, except lengths and the stack's count, which the
+// block that arrives last at a counter writes (all have read them by then).
+#include "ks_q8.h"
+
+namespace {
+
+struct TablesArgs {
+  unsigned n_seqs, max_blocks, n_pages, page_log, max_rows;
+  int *lens, *tables, *free_pages, *plan;
+  ks_plan_layout at;
+  unsigned *bad, *arrived;
+};
+
+// Exclusive sums of three counts over the block's threads (a multiple of 32, up to 1024); totals in tot.
+__device__ __forceinline__ void scan3(unsigned (&v)[3], unsigned (&tot)[3], unsigned (*red)[3]) {
+  const unsigned lane = threadIdx.x & 31u, warp = threadIdx.x >> 5, nwarp = blockDim.x >> 5;
+  unsigned inc[3];
+#pragma unroll
+  for (int k = 0; k < 3; k++) {
+    inc[k] = v[k];
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const unsigned up = __shfl_up_sync(0xffffffffu, inc[k], o);
+      if (lane >= (unsigned)o) inc[k] += up;
+    }
+    if (lane == 31u) red[warp][k] = inc[k];
+  }
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < 3; k++) {
+    unsigned before = 0, all = 0;
+    for (unsigned w = 0; w < nwarp; w++) {
+      const unsigned x = red[w][k];
+      before += w < warp ? x : 0u;
+      all += x;
+    }
+    v[k] = before + inc[k] - v[k];
+    tot[k] = all;
+  }
+}
+
+__global__ void __launch_bounds__(1024) pages_step_kernel(const TablesArgs a, const int* n_new) {
+  __shared__ unsigned red[32][3];
+  __shared__ unsigned first_row[KS_PAGES_MAX_SEQS], first_page[KS_PAGES_MAX_SEQS], first_job[KS_PAGES_MAX_SEQS];
+  __shared__ int len_of[KS_PAGES_MAX_SEQS];
+  __shared__ unsigned last;
+  ks_pdl_entry();
+  const unsigned tid = threadIdx.x, page = 1u << a.page_log, cap = a.max_blocks << a.page_log;
+  const int count = a.free_pages[0];
+  int len = 0, add = 0;
+  if (tid < a.n_seqs) {
+    len = a.lens[tid];
+    add = n_new[tid];
+  }
+  // the highest status that holds; counts out of range are nothing in the sums
+  int status = 0;
+  if (len < 0 || (unsigned)len > cap || add < 0) status = KS_PLAN_BAD_LENGTH;
+  else if ((unsigned)add > a.max_rows) status = KS_PLAN_TOO_MANY_ROWS;
+  else if ((unsigned)add > cap - (unsigned)len) status = KS_PLAN_TABLE_FULL;
+  if (status >= KS_PLAN_TOO_MANY_ROWS) add = 0;  // (a sequence that would outgrow its table still counts its rows)
+  if (status == KS_PLAN_BAD_LENGTH) len = 0;
+  const unsigned after = (unsigned)len + (unsigned)add, held = ((unsigned)len + page - 1u) >> a.page_log;
+  unsigned v[3] = {(unsigned)add, ((after + page - 1u) >> a.page_log) - held, add ? ((after - 1u) >> a.page_log) - ((unsigned)len >> a.page_log) + 1u : 0u}, tot[3];
+  scan3(v, tot, red);
+  if (tid < a.n_seqs) {
+    first_row[tid] = v[0];
+    first_page[tid] = v[1];
+    first_job[tid] = v[2];
+    len_of[tid] = len;
+  }
+  int worst = status;
+#pragma unroll
+  for (int s = KS_PLAN_BAD_LENGTH; s > 0; s--)
+    if (__syncthreads_or(status == s)) {
+      worst = s;
+      break;
+    }
+  if (worst < KS_PLAN_TOO_MANY_ROWS && tot[0] > a.max_rows) worst = KS_PLAN_TOO_MANY_ROWS;
+  if (worst == 0 && (count < 0 || (unsigned)count > a.n_pages || tot[1] > (unsigned)count)) worst = KS_PLAN_NO_PAGES;
+  const unsigned rows = worst ? 0u : tot[0], jobs = worst ? 0u : tot[2];
+  // lengths and count have been read by every thread of this block
+  if (gridDim.x > 1u) {
+    if (tid == 0) {
+      __threadfence();
+      last = atomicAdd(a.arrived, 1u) == gridDim.x - 1u;
+    }
+    __syncthreads();
+  } else {
+    if (tid == 0) last = 1u;
+    __syncthreads();
+  }
+  if (last) {
+    if (tid < a.n_seqs && !worst) a.lens[tid] = (int)after;
+    if (tid == 0) {
+      if (!worst) a.free_pages[0] = count - (int)tot[1];
+      if (gridDim.x > 1u) *a.arrived = 0u;
+    }
+  }
+  if (blockIdx.x == 0) {
+    if (tid < a.n_seqs) a.plan[a.at.row_start + tid] = worst ? 0 : (int)v[0];
+    if (tid < KS_PAGES_PLAN_HEADER) {
+      const int head[4] = {worst, (int)rows, (int)jobs, worst ? count : count - (int)tot[1]};
+      a.plan[tid] = tid < 4u ? head[tid] : 0;
+    }
+    if (tid == 0) a.plan[a.at.row_start + a.n_seqs] = (int)rows;
+  }
+  const unsigned step = gridDim.x * blockDim.x, words = (a.max_rows + 3u) & ~3u;
+  for (unsigned r = blockIdx.x * blockDim.x + tid; r < words; r += step) {
+    int seq = -1, pos = -1, slot = -1;
+    if (r < rows) {
+      unsigned lo = 0, hi = a.n_seqs;  // the last sequence that starts at r or before and has rows
+      while (hi - lo > 1u) {
+        const unsigned mid = (lo + hi) >> 1;
+        if (first_row[mid] <= r) lo = mid;
+        else hi = mid;
+      }
+      const unsigned l0 = (unsigned)len_of[lo], p = l0 + (r - first_row[lo]), b = p >> a.page_log, had = (l0 + page - 1u) >> a.page_log;
+      int id;
+      if (b >= had) {
+        id = a.free_pages[(unsigned)count - first_page[lo] - (b - had)];
+        if ((p & (page - 1u)) == 0u) a.tables[(size_t)lo * a.max_blocks + b] = id;
+      } else {
+        id = a.tables[(size_t)lo * a.max_blocks + b];
+      }
+      seq = (int)lo;
+      pos = (int)p;
+      if (id >= 0 && (unsigned)id < a.n_pages) slot = (int)(((unsigned)id << a.page_log) + (p & (page - 1u)));
+      else atomicOr(a.bad, KS_BAD_PAGE);
+      if (r == first_row[lo] || (p & (page - 1u)) == 0u) {
+        const unsigned end = lo + 1u < a.n_seqs ? first_row[lo + 1u] : rows;
+        reinterpret_cast<int4*>(a.plan + a.at.jobs)[first_job[lo] + (b - (l0 >> a.page_log))] = make_int4((int)r, (int)min(page - (p & (page - 1u)), end - r), slot, (int)p);
+      }
+    }
+    a.plan[a.at.row_seq + r] = seq;
+    a.plan[a.at.row_pos + r] = pos;
+    a.plan[a.at.row_slot + r] = slot;
+  }
+  for (unsigned j = jobs + blockIdx.x * blockDim.x + tid; j < a.at.n_jobs; j += step) reinterpret_cast<int4*>(a.plan + a.at.jobs)[j] = make_int4(-1, -1, -1, -1);
+}
+
+// One block: the sum over the sequences, then one page per thread and step.
+__global__ void __launch_bounds__(1024) pages_trim_kernel(const TablesArgs a, const int* keep) {
+  __shared__ unsigned red[32][3];
+  __shared__ unsigned first[KS_PAGES_MAX_SEQS], from[KS_PAGES_MAX_SEQS];
+  ks_pdl_entry();
+  const unsigned tid = threadIdx.x, page = 1u << a.page_log, cap = a.max_blocks << a.page_log;
+  const int count = a.free_pages[0];
+  int len = 0, to = -1;
+  if (tid < a.n_seqs) {
+    len = a.lens[tid];
+    to = keep[tid];
+  }
+  const bool fine = len >= 0 && (unsigned)len <= cap, cut = fine && to >= 0 && to < len;
+  if (!fine) atomicOr(a.bad, KS_BAD_ROWS);
+  const unsigned old = fine ? ((unsigned)len + page - 1u) >> a.page_log : 0u, kept = cut ? ((unsigned)to + page - 1u) >> a.page_log : old;
+  unsigned v[3] = {old - kept, 0u, 0u}, tot[3];
+  scan3(v, tot, red);
+  if (tid < a.n_seqs) {
+    first[tid] = v[0];
+    from[tid] = kept;
+  }
+  __syncthreads();
+  if (count < 0 || (unsigned)count > a.n_pages || tot[0] > a.n_pages - (unsigned)count) {  // more pages than there are: nothing moves
+    if (tid == 0) atomicOr(a.bad, KS_BAD_STACK);
+    return;
+  }
+  if (cut) a.lens[tid] = to;
+  for (unsigned k = tid; k < tot[0]; k += blockDim.x) {
+    unsigned lo = 0, hi = a.n_seqs;
+    while (hi - lo > 1u) {
+      const unsigned mid = (lo + hi) >> 1;
+      if (first[mid] <= k) lo = mid;
+      else hi = mid;
+    }
+    int* entry = a.tables + (size_t)lo * a.max_blocks + from[lo] + (k - first[lo]);
+    const int id = *entry;
+    if (id < 0 || (unsigned)id >= a.n_pages) atomicOr(a.bad, KS_BAD_PAGE);
+    a.free_pages[(unsigned)count + tot[0] - k] = id;
+    *entry = -1;
+  }
+  if (tid == 0) a.free_pages[0] = count + (int)tot[0];
+}
+
+__global__ void __launch_bounds__(256) pages_reset_kernel(const TablesArgs a, size_t n_plan) {
+  ks_pdl_entry();
+  const size_t step = (size_t)gridDim.x * blockDim.x, i0 = (size_t)blockIdx.x * blockDim.x + threadIdx.x;
+  for (size_t i = i0; i < a.n_seqs; i += step) a.lens[i] = 0;
+  for (size_t i = i0; i < (size_t)a.n_seqs * a.max_blocks; i += step) a.tables[i] = -1;
+  for (size_t i = i0; i <= a.n_pages; i += step) a.free_pages[i] = i ? (int)(a.n_pages - i) : (int)a.n_pages;
+  for (size_t i = i0; i < n_plan; i += step) a.plan[i] = i >= a.at.row_seq ? -1 : i == 3 ? (int)a.n_pages : 0;
+}
+
+TablesArgs args_of(ks_ctx* ctx, const ks_page_tables* t) {
+  TablesArgs a;
+  a.n_seqs = (unsigned)t->n_seqs;
+  a.max_blocks = (unsigned)t->max_blocks;
+  a.n_pages = (unsigned)t->n_pages;
+  a.page_log = (unsigned)__builtin_ctzll(t->page);
+  a.max_rows = (unsigned)t->max_rows;
+  a.lens = (int*)t->lens->dptr;
+  a.tables = (int*)t->tables->dptr;
+  a.free_pages = (int*)t->free_pages->dptr;
+  a.plan = (int*)t->plan->dptr;
+  a.at = ks_plan_parts(t->n_seqs, t->max_rows, t->page);
+  a.bad = (unsigned*)ctx->ws + KS_WS_INDEX_WORD;
+  a.arrived = (unsigned*)ctx->ws + KS_WS_COUNT_WORD;
+  return a;
+}
+unsigned round32(size_t n) { return (unsigned)((n + 31) & ~size_t(31)); }
+
+bool sizes_ok(size_t n_seqs, size_t max_rows, size_t page) {
+  return n_seqs >= 1 && n_seqs <= KS_PAGES_MAX_SEQS && max_rows >= 1 && max_rows <= (1u << 20) && ks_page_ok(page);
+}
+
+}  // namespace
+
+int ks_check_tables(ks_ctx* ctx, const char* who, const ks_page_tables* t) {
+  KS_REQUIRE(ctx, t, "%s: null page tables", who);
+  KS_REQUIRE(ctx, ks_page_ok(t->page), "%s: pages of %zu positions not supported (16, 32, 64, 128)", who, t->page);
+  KS_REQUIRE(ctx, t->n_seqs >= 1 && t->n_seqs <= KS_PAGES_MAX_SEQS, "%s: n_seqs=%zu outside 1..%d", who, t->n_seqs, KS_PAGES_MAX_SEQS);
+  KS_REQUIRE(ctx, t->max_rows >= 1 && t->max_rows <= (1u << 20), "%s: max_rows=%zu outside 1..2^20", who, t->max_rows);
+  const size_t most = 0x7FFFFFFFu / t->page;
+  KS_REQUIRE(ctx, t->n_pages >= 1 && t->n_pages <= most && t->max_blocks >= 1 && t->max_blocks <= most, "%s: %zu pages, %zu to a sequence: at least one, and below 2^31 positions", who,
+             t->n_pages, t->max_blocks);
+  KS_REQUIRE(ctx, ks_fits(t->lens, 0, t->n_seqs * 4) && ks_fits(t->tables, 0, t->n_seqs * t->max_blocks * 4), "%s: lens or tables buffer too small", who);
+  KS_REQUIRE(ctx, ks_fits(t->free_pages, 0, (1 + t->n_pages) * 4), "%s: free_pages buffer too small (1 + n_pages words)", who);
+  KS_REQUIRE(ctx, ks_fits(t->plan, 0, ks_pages_plan_ints(t->n_seqs, t->max_rows, t->page) * 4), "%s: plan buffer too small", who);
+  KS_REQUIRE(ctx, ks_aligned(t->lens, 4) && ks_aligned(t->tables, 4) && ks_aligned(t->free_pages, 4) && ks_aligned(t->plan, 16), "%s: tables must start on 4 bytes, the plan on 16", who);
+  return KS_OK;
+}
+
+extern "C" {
+
+size_t ks_pages_plan_offset(size_t n_seqs, size_t max_rows, size_t page, int part) {
+  if (!sizes_ok(n_seqs, max_rows, page)) return 0;
+  const ks_plan_layout l = ks_plan_parts(n_seqs, max_rows, page);
+  const size_t at[6] = {l.row_start, l.row_seq, l.row_pos, l.row_slot, l.jobs, (size_t)l.jobs + 4 * l.n_jobs};
+  return part >= KS_PLAN_ROW_START && part <= KS_PLAN_END ? at[part] : 0;
+}
+size_t ks_pages_plan_ints(size_t n_seqs, size_t max_rows, size_t page) { return ks_pages_plan_offset(n_seqs, max_rows, page, KS_PLAN_END); }
+
+int ks_pages_reset(ks_ctx* ctx, const ks_page_tables* t) {
+  if (!ctx) return KS_ERR_INVALID;
+  int rc = ks_check_tables(ctx, "pages_reset", t);
+  if (rc) return rc;
+  KS_REQUIRE_DEVICE(ctx, "pages_reset");
+  ks_on_device on(ctx);
+  KS_LAUNCH(ctx, pages_reset_kernel, (unsigned)ctx->sm_count, 256, 0, args_of(ctx, t), ks_pages_plan_ints(t->n_seqs, t->max_rows, t->page));
+  return ks_after_launch(ctx, "pages_reset");
+}
+
+int ks_pages_step(ks_ctx* ctx, const ks_page_tables* t, const ks_buf* n_new) {
+  if (!ctx) return KS_ERR_INVALID;
+  int rc = ks_check_tables(ctx, "pages_step", t);
+  if (rc) return rc;
+  KS_REQUIRE(ctx, ks_fits(n_new, 0, t->n_seqs * 4) && ks_aligned(n_new, 4), "pages_step: n_new buffer too small or not on 4 bytes");
+  KS_REQUIRE_DEVICE(ctx, "pages_step");
+  ks_on_device on(ctx);
+  const unsigned threads = t->n_seqs > 256 || t->max_rows > 2048 ? (t->n_seqs > 512 ? 1024 : 512) : t->n_seqs > 128 || t->max_rows > 256 ? 256 : 128;
+  const size_t blocks = (t->max_rows + 4 * threads - 1) / (4 * threads);
+  const unsigned most = 64u;
+  KS_LAUNCH(ctx, pages_step_kernel, (unsigned)(blocks < most ? blocks : most), threads, 0, args_of(ctx, t), (const int*)n_new->dptr);
+  return ks_after_launch(ctx, "pages_step");
+}
+
+int ks_pages_trim(ks_ctx* ctx, const ks_page_tables* t, const ks_buf* keep) {
+  if (!ctx) return KS_ERR_INVALID;
+  int rc = ks_check_tables(ctx, "pages_trim", t);
+  if (rc) return rc;
+  KS_REQUIRE(ctx, ks_fits(keep, 0, t->n_seqs * 4) && ks_aligned(keep, 4), "pages_trim: keep buffer too small or not on 4 bytes");
+  KS_REQUIRE_DEVICE(ctx, "pages_trim");
+  ks_on_device on(ctx);
+  KS_LAUNCH(ctx, pages_trim_kernel, 1, round32(t->n_seqs) < 128u ? 128u : round32(t->n_seqs), 0, args_of(ctx, t), (const int*)keep->dptr);
+  return ks_after_launch(ctx, "pages_trim");
+}
+
+}  // extern "C"

@@ -19,7 +19,7 @@ import ctypes as C
 import numpy as np
 
 from . import _lib
-from ._lib import F16, F32, Q4K, Q6K, Q40  # noqa: F401  (re-exported)
+from ._lib import E4M3, F16, F32, I8, Q4K, Q6K, Q40  # noqa: F401  (re-exported)
 
 ACT_NP = {F32: np.float32, F16: np.float16}
 
@@ -191,6 +191,50 @@ class CudaContext:
             self.h = None
 
 
+class PageTables:
+    """Lengths, page tables, the stack of free pages and the plan of up to ``n_seqs`` sequences (``ks_page_tables``).
+
+    Buffers that are not given are allocated, and everything is emptied then.  ``plan_part`` says where a part of the
+    plan starts; ``row_slot`` is the one that a read-back takes."""
+
+    ROW_START, ROW_SEQ, ROW_POS, ROW_SLOT, JOBS, END = range(6)
+    STATUS = ("ok", "not enough free pages", "a sequence would outgrow its table", "more rows than max_rows", "a bad count or length")
+
+    def __init__(self, ctx: CudaContext, n_seqs, max_blocks, n_pages, page, max_rows, lens=None, tables=None, free=None, plan=None):
+        self.ctx, self.n_seqs, self.max_blocks, self.n_pages, self.page, self.max_rows = ctx, n_seqs, max_blocks, n_pages, page, max_rows
+        lib = ctx.lib
+        given = (lens, tables, free, plan)
+        sizes = (n_seqs, n_seqs * max_blocks, 1 + n_pages, lib.ks_pages_plan_ints(n_seqs, max_rows, page))
+        self.lens, self.tables, self.free, self.plan = (b if b is not None else ctx.buffer_empty_bytes(4 * n) for b, n in zip(given, sizes))
+        self.struct = _lib.PageTablesStruct(n_seqs, max_blocks, n_pages, page, max_rows, self.lens.h, self.tables.h, self.free.h, self.plan.h)
+        self.ref = C.byref(self.struct)
+        self.row_slot = self.plan_part(self.ROW_SLOT)
+        if all(b is None for b in given):
+            ctx.check(lib.ks_pages_reset(ctx.h, self.ref))
+
+    def plan_part(self, part: int) -> int:
+        return self.ctx.lib.ks_pages_plan_offset(self.n_seqs, self.max_rows, self.page, part)
+
+    def read(self, buf: Buffer) -> np.ndarray:
+        return self.ctx.read_bytes(buf).view(np.int32)
+
+    def status(self) -> int:
+        """Status of the last step (waits for it)."""
+        return int(self.ctx.read_bytes(self.plan, 4).view(np.int32)[0])
+
+
+class Q8Cache:
+    """One layer's paged cache of codes and scales (``ks_q8_cache``); buffers that are not given are allocated."""
+
+    def __init__(self, ctx: CudaContext, n_pages, page, n_kv, hd, dtype=I8, k=None, v=None, k_scale=None, v_scale=None):
+        self.ctx, self.n_pages, self.page, self.n_kv, self.hd, self.dtype = ctx, n_pages, page, n_kv, hd, dtype
+        codes, scales = n_pages * n_kv * page * hd, 4 * n_pages * n_kv
+        self.k, self.v, self.k_scale, self.v_scale = (b if b is not None else ctx.buffer_empty_bytes(n)
+                                                      for b, n in ((k, codes), (v, codes), (k_scale, scales), (v_scale, scales)))
+        self.struct = _lib.Q8CacheStruct(n_pages, page, n_kv, hd, dtype, self.k.h, self.v.h, self.k_scale.h, self.v_scale.h)
+        self.ref = C.byref(self.struct)
+
+
 class Eng:
     """The op interface of the decode path (crates/ksearch_kernels/src/lib.rs)."""
 
@@ -325,6 +369,38 @@ class Eng:
             self.sdpa_mwg_kv(ctx, n_q, n_kv, hd, max_t, kv_dtype, q, k, v, meta, tmp, out, scale)
         else:
             self.sdpa_naive_kv(ctx, n_q, n_kv, hd, max_t, kv_dtype, q, k, v, meta, out, scale)
+
+    # ---- a paged cache in 8 bits (no counterpart in the reference; include/ksearch_cuda.h has the definitions) ----
+    def pages_reset(self, ctx, tables: PageTables):
+        """No sequence holds a position, every page is free."""
+        ctx.check(ctx.lib.ks_pages_reset(ctx.h, tables.ref))
+
+    def pages_step(self, ctx, tables: PageTables, n_new):
+        """Pages, lengths and the plan for ``n_new`` (int32 per sequence) more rows; ``tables.status()`` says whether there was room."""
+        ctx.check(ctx.lib.ks_pages_step(ctx.h, tables.ref, n_new.h))
+
+    def pages_trim(self, ctx, tables: PageTables, keep):
+        """Sequences end at ``keep`` (int32 each; 0 releases, below 0 leaves alone); pages behind go back."""
+        ctx.check(ctx.lib.ks_pages_trim(ctx.h, tables.ref, keep.h))
+
+    def kv_append_q8(self, ctx, cache: Q8Cache, tables: PageTables, k, v, k_off_elems=0, v_off_elems=0, kv_ld=0):
+        """The plan's rows of k and v [max_rows, n_kv, hd] (``kv_ld`` elements apart, 0: next to each other) into their pages."""
+        ctx.check(ctx.lib.ks_kv_append_q8(ctx.h, cache.ref, tables.ref, self.act, k.h, k_off_elems, v.h, v_off_elems, kv_ld or cache.n_kv * cache.hd))
+
+    def rmsnorm_per_head_qkv_q8(self, ctx, cache: Q8Cache, tables: PageTables, n_q, eps, q, qw, rope, k, kw, v, q_out):
+        """``rmsnorm_per_head_qkv_q40_batch`` over a paged 8-bit cache: every row at its own sequence and position."""
+        ctx.check(ctx.lib.ks_rmsnorm_per_head_qkv_q8(ctx.h, cache.ref, tables.ref, n_q, eps, self.act, q.h, qw.h, rope.h, k.h, kw.h, v.h, q_out.h))
+
+    def kv_read_q8(self, ctx, cache: Q8Cache, n_rows, slots, slot_off_elems, k, v):
+        """Cached rows as numbers, by slot (``tables.plan`` from ``tables.row_slot`` on: the rows of the last step)."""
+        ctx.check(ctx.lib.ks_kv_read_q8(ctx.h, cache.ref, n_rows, slots.h, slot_off_elems, self.act, k.h, v.h))
+
+    def sdpa_paged_tmp_floats(self, ctx, cache: Q8Cache, tables: PageTables, n_q, rows_most) -> int:
+        return ctx.lib.ks_sdpa_paged_tmp_floats(ctx.h, cache.ref, tables.ref, n_q, rows_most)
+
+    def sdpa_paged_q8(self, ctx, cache: Q8Cache, tables: PageTables, n_q, rows_most, ctx_most, q, tmp, out, scale=1.0, window=0):
+        """Attention of the plan's rows over the cache, causal, through a window if ``window`` > 0."""
+        ctx.check(ctx.lib.ks_sdpa_paged_q8(ctx.h, cache.ref, tables.ref, n_q, rows_most, ctx_most, window, scale, self.act, q.h, tmp.h, out.h))
 
     # ---- small ops --------------------------------------------------------
     def quantize_q40(self, ctx, n, src, dst, dst_byte_off):
