@@ -42,24 +42,36 @@ __device__ __forceinline__ bool seq_of(const SdpaArgs& a, unsigned i, Seq& s) { 
 }
 
 // ---- few rows: the context is what counts -------------------------------------------------------------------
-// A piece is 16 rows (row and query head of the group, counted together) of a sequence against one KV head; its units are tiles of
-// TILE positions.  All units of the launch lie in one line and every block takes a run of them of the same length, so that a block's
-// share does not depend on how lengths differ; pieces that lie in several blocks leave a record (m, l, O) per block for the merge.
+// A piece is 8 rows (row and query head of the group, counted together) of a sequence against one KV head; its units are tiles of TILE
+// positions, SUB for each warp of a block.  All units of the launch lie in one line and every block takes a run of them of the same length, so
+// that a block's share does not depend on how lengths differ; pieces that lie in several blocks leave a record (m, l, O) per block for
+// the merge.
+//
+// Inside a block the warps have nothing to do with one another until the piece ends: each brings its SUB positions into a ring of its own
+// and keeps its own maximum, sum and values.  Both products are transposed, so that the 16 rows of mma.sync m16n8k16 are positions (dims)
+// and its 8 columns the query rows:
+//   S^T = K q^T:  a lane reads 16 bytes of two positions' codes, which are the A operand of four steps over 64 dims if q has its dims in that order;
+//   O^T = V^T P^T:  the probabilities, out of S^T's accumulators, become B operands by movmatrix; a lane reads 16 dims of four positions, pairs
+//   the codes of neighbouring positions by byte permutes, and has its 16 dims of two query rows in the accumulators.
+// Codes become f16 exactly, f32 queries and probabilities are two f16 terms each (the small one first), and in f32 the values of every SUB
+// positions are added to registers: a chain of accumulating MMAs loses low bits at every step.  The maximum that probabilities refer to
+// moves only when a score exceeds it by 2^4.
 template <int HD_, typename T_>
 struct Split {
   static constexpr int HD = HD_, TERMS = sizeof(T_) == 4 ? 2 : 1;
-  static constexpr int TILE = HD == 256 ? 64 : 128, STAGES = 3, WARPS = 8, THREADS = WARPS * 32;
-  static constexpr int KH = HD == 256 ? 2 : 1, KR = HD / KH;   // warps share out positions, and the halves of a head of 256: KR dims each
-  static constexpr int DG = HD / 32, PG = WARPS / DG;          // of the values: 32 dims each, and 1, 2 or 4 shares of the positions
-  static constexpr int CH = HD / 16, ROWS = THREADS / CH, PASSES = TILE / ROWS;  // a thread copies 16 bytes of PASSES rows
-  static constexpr int SP = TILE + 8, COLS = TILE / 16, GROUPS = TILE / 16;
-  static constexpr unsigned stage_bytes = 2 * TILE * HD, scales = STAGES * stage_bytes, scores = scales + STAGES * GROUPS * 8, probs = scores + KH * 16 * SP * 4,
-                            alpha = probs + TERMS * 16 * SP * 2, sums = alpha + 64, red = alpha + 128, total = red + (PG - 1) * 16 * HD * 4;
-  static constexpr unsigned record = 16 * (HD + 2);            // floats: m[16], l[16], O[16][HD]
-  static_assert(WARPS / KH * 16 == TILE, "a warp makes the scores of 16 positions");
+  static constexpr int NP = HD == 64 ? 2 : 1, SUB = 16 * NP, STAGES = 3, WARPS = 8, THREADS = WARPS * 32, TILE = WARPS * SUB;
+  static constexpr int PER_SM = HD == 256 ? 1 : 2;
+  static constexpr int KK = HD / 64;                    // runs of 64 dims
+  static constexpr int W = HD == 64 ? 64 : 128, WN = HD / W, WW = W / 32;  // windows of dims a lane's read of the values lies in, words of such a read
+  static constexpr int CH = HD / 16, LR = 32 / CH, COPIES = SUB / LR;      // chunks of a row, rows a warp copies at once, such copies
+  static constexpr unsigned stage_bytes = 2 * SUB * HD, ring = STAGES * stage_bytes, scales = WARPS * ring, total = scales + WARPS * STAGES * NP * 8;
+  static constexpr unsigned OP = HD + 4;                // the warps' results on their way together: [warp][8][OP] in the rings' place
+  static constexpr unsigned record = 8 * (HD + 2);      // floats: m[8], l[8], O[8][HD]
+  static_assert(WARPS * 8 * OP * 4 <= WARPS * ring, "the results fit the rings");
 };
 constexpr float kNone = -1.0e30f;       // the maximum of nothing
-constexpr float kProbs = 16384.0f;      // probabilities carry 2^14: the second f16 term of one of 2^-16 is no denormal
+constexpr float kProbs = 1024.0f;       // probabilities carry 2^10, are 2^5 at most, and 2^-35 of the largest is the least that counts
+constexpr float kSlack = 4.0f;          // log2 of how far a score may exceed what probabilities refer to
 
 __device__ __forceinline__ uint32_t smem_at(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool there) {
@@ -100,17 +112,22 @@ __device__ __forceinline__ void widen_pairs(uint32_t a, uint32_t b, uint32_t (&p
   widen4<FP8>(x, p[0], p[1]);
   widen4<FP8>(y, p[2], p[3]);
 }
-__device__ __forceinline__ void put8(float* to, const float (&v)[8], float f) {
-  *reinterpret_cast<float4*>(to) = make_float4(v[0] * f, v[1] * f, v[2] * f, v[3] * f);
-  *reinterpret_cast<float4*>(to + 4) = make_float4(v[4] * f, v[5] * f, v[6] * f, v[7] * f);
+// An 8 x 8 matrix of f16, a row's pair of columns per lane, transposed.
+__device__ __forceinline__ uint32_t turn8x8(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
 }
-__device__ __forceinline__ void put8(__half* to, const float (&v)[8], float f) {
-  uint4 w;
-  w.x = q8_u32(__floats2half2_rn(v[0] * f, v[1] * f));
-  w.y = q8_u32(__floats2half2_rn(v[2] * f, v[3] * f));
-  w.z = q8_u32(__floats2half2_rn(v[4] * f, v[5] * f));
-  w.w = q8_u32(__floats2half2_rn(v[6] * f, v[7] * f));
-  *reinterpret_cast<uint4*>(to) = w;
+// What a row's values are multiplied by in the end; a row that saw nothing is zero, NaN stays.
+__device__ __forceinline__ float over(float l) { return l > 0.0f ? (1.0f / kProbs) / l : l == 0.0f ? 0.0f : l; }
+__device__ __forceinline__ void put_dims(float* to, const float* v, int n) {
+  if (n == 4) *reinterpret_cast<float4*>(to) = make_float4(v[0], v[1], v[2], v[3]);
+  else *reinterpret_cast<float2*>(to) = make_float2(v[0], v[1]);
+}
+__device__ __forceinline__ void put_dims(__half* to, const float* v, int n) {
+  const uint32_t x = q8_u32(__floats2half2_rn(v[0], v[1]));
+  if (n == 4) *reinterpret_cast<uint2*>(to) = make_uint2(x, q8_u32(__floats2half2_rn(v[2], v[3])));
+  else *reinterpret_cast<uint32_t*>(to) = x;
 }
 // A positive scale (inside q8_scale's range) as 2^e and a factor of 1 to 2.
 __device__ __forceinline__ void split_scale(float s, float& e, float& factor, float& down) {
@@ -122,21 +139,21 @@ __device__ __forceinline__ void split_scale(float s, float& e, float& factor, fl
 }
 
 template <int HD, typename T, bool FP8>
-__global__ void __launch_bounds__(256, 2) sdpa_q8_split_kernel(const SdpaArgs a) {
+__global__ void __launch_bounds__(Split<HD, T>::THREADS, Split<HD, T>::PER_SM) sdpa_q8_split_kernel(const SdpaArgs a) {
   using S = Split<HD, T>;
   extern __shared__ __align__(128) unsigned char smem[];
   __shared__ unsigned long long scan[S::WARPS], seq_first;
   __shared__ unsigned seq_at;
+  __shared__ float row_m[S::WARPS][8], row_l[S::WARPS][8];
   ks_pdl_entry();
   const unsigned tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5, g = lane >> 2, c = lane & 3u;
-  const uint32_t sb = smem_at(smem);
 
   // ---- the line of units: a thread counts for up to four neighbouring sequences
   auto units_of = [&](const Seq& s) -> unsigned long long {
     const unsigned m = (unsigned)s.rows * a.G;
     if (m > a.few) return 0ull;
     const int t0 = s.begin / S::TILE, t1 = (s.len + S::TILE - 1) / S::TILE;
-    return (unsigned long long)((m + 15u) / 16u) * a.n_kv * (unsigned)max(t1 - t0, 1);  // (a row that sees nothing still gets its zeros)
+    return (unsigned long long)((m + 7u) / 8u) * a.n_kv * (unsigned)max(t1 - t0, 1);  // (a row that sees nothing still gets its zeros)
   };
   const unsigned per = (a.n_seqs + S::THREADS - 1u) / S::THREADS;
   unsigned long long mine[KS_PAGES_MAX_SEQS / 256], sum = 0;
@@ -183,6 +200,11 @@ __global__ void __launch_bounds__(256, 2) sdpa_q8_split_kernel(const SdpaArgs a)
   if (blockIdx.x == 0 && tid == 0) a.first[a.n_seqs] = total;
   __syncthreads();
 
+  unsigned char* ring = smem + warp * S::ring;
+  const uint32_t ring_at = smem_at(ring), scales_at = smem_at(smem) + S::scales + warp * (S::STAGES * S::NP * 8);
+  const float* scales = reinterpret_cast<const float*>(smem + S::scales) + warp * (S::STAGES * S::NP * 2);
+  const float to_log2 = a.scale * 1.44269504088896340736f;
+
   // ---- piece after piece
   unsigned seq = seq_at, in_block = 0;
   unsigned long long u = u_begin, at = seq_first;
@@ -194,76 +216,78 @@ __global__ void __launch_bounds__(256, 2) sdpa_q8_split_kernel(const SdpaArgs a)
       have = seq_of(a, ++seq, s);
     }
     const int tile0 = s.begin / S::TILE, n_tiles = max((s.len + S::TILE - 1) / S::TILE - tile0, 1);
-    const unsigned m_rows = (unsigned)s.rows * a.G, m_tiles = (m_rows + 15u) / 16u;
+    const unsigned m_rows = (unsigned)s.rows * a.G, m_tiles = (m_rows + 7u) / 8u;
     const unsigned piece = (unsigned)((u - at) / (unsigned)n_tiles), t_first = (unsigned)((u - at) % (unsigned)n_tiles);
-    const unsigned kvh = piece / m_tiles, m0 = piece % m_tiles * 16u;
+    const unsigned kvh = piece / m_tiles, m0 = piece % m_tiles * 8u;
     const unsigned n = (unsigned)min((unsigned long long)((unsigned)n_tiles - t_first), u_end - u);  // tiles of this piece that are ours
-    const int t0 = tile0 + (int)t_first;
+    const int p_first = (tile0 + (int)t_first) * S::TILE + (int)warp * S::SUB;                       // this warp's positions of the first
+    const int* table = a.tables + (size_t)seq * a.max_blocks;
 
-    // copies of tile t of the piece into stage st: 16 bytes a thread and row, chunks swapped about so that the reads below meet no bank twice
-    auto send = [&](int t, unsigned st) {
-      const uint32_t to = sb + st * S::stage_bytes;
-      const unsigned ch = tid % S::CH;
+    // the page of 16 positions (a page has no fewer), -1 where no row sees any of them
+    auto page_of = [&](int p) -> int {
+      if (p + 15 < s.begin || p >= s.len) return -1;
+      const int id = table[(unsigned)p >> a.page_log];
+      if (id >= 0 && (unsigned)id < a.n_pages) return id;
+      if (lane == 0) atomicOr(a.bad, KS_BAD_PAGE);
+      return -1;
+    };
+    // copies of SUB positions into stage st: 16 bytes a lane, chunks swapped about so that the reads below meet no bank twice; positions that
+    // nobody sees become zeros
+    auto send = [&](int p0, const int (&id)[S::NP], unsigned st) {
+      const unsigned ch = lane % S::CH, r0 = lane / S::CH;
 #pragma unroll
-      for (int i = 0; i < S::PASSES; i++) {
-        const unsigned r = tid / S::CH + (unsigned)i * S::ROWS;
-        const int pos = t * S::TILE + (int)r;
-        bool there = pos >= s.begin && pos < s.len;
-        size_t from = 0;
-        if (there) {
-          const int id = a.tables[(size_t)seq * a.max_blocks + ((unsigned)pos >> a.page_log)];
-          there = id >= 0 && (unsigned)id < a.n_pages;
-          if (there) from = (((((size_t)id * a.n_kv + kvh) << a.page_log) + ((unsigned)pos & ((1u << a.page_log) - 1u))) * HD) + ch * 16u;
-          else if (ch == 0) atomicOr(a.bad, KS_BAD_PAGE);
+      for (int b = 0; b < S::NP; b++) {
+        const int p = p0 + 16 * b;
+        const size_t block = (size_t)(id[b] < 0 ? 0 : id[b]) * a.n_kv + kvh;
+        const size_t from = (((block << a.page_log) + ((unsigned)p & ((1u << a.page_log) - 1u)) + r0) * HD) + ch * 16u;
+        const uint32_t to = ring_at + st * S::stage_bytes + (unsigned)b * 16u * HD;
+#pragma unroll
+        for (int i = 0; i < S::COPIES / S::NP; i++) {
+          const unsigned r = r0 + (unsigned)(i * S::LR);
+          const bool there = id[b] >= 0 && p + (int)r >= s.begin && p + (int)r < s.len;
+          const unsigned kch = HD >= 128 ? ch ^ ((r & 1u) << 2) : ch, vch = HD >= 128 ? ch ^ ((r >> 1 & 3u) << 1) : ch ^ ((r >> 1 & 1u) << 1);
+          copy16(to + r * HD + kch * 16u, a.kc + from + (size_t)(i * S::LR) * HD, there);
+          copy16(to + S::SUB * HD + r * HD + vch * 16u, a.vc + from + (size_t)(i * S::LR) * HD, there);
         }
-        const unsigned kch = HD >= 128 ? ch ^ ((r & 1u) << 2) : ch, vch = HD >= 128 ? ch ^ ((r >> 1 & 3u) << 1) : ch ^ ((r >> 1 & 1u) << 1);
-        copy16(to + r * HD + kch * 16u, a.kc + from, there);
-        copy16(to + S::TILE * HD + r * HD + vch * 16u, a.vc + from, there);
+        if (lane < 2u) copy4(scales_at + ((st * S::NP + b) * 2u + lane) * 4u, (lane ? a.vs : a.ks) + block, id[b] >= 0);
       }
-      if (tid < 2 * S::GROUPS) {  // a scale for each 16 positions (a page has no fewer)
-        const unsigned gr = tid % S::GROUPS;
-        const int pos = t * S::TILE + 16 * (int)gr;
-        bool there = pos + 15 >= s.begin && pos < s.len;
-        size_t from = 0;
-        if (there) {
-          const int id = a.tables[(size_t)seq * a.max_blocks + ((unsigned)pos >> a.page_log)];
-          there = id >= 0 && (unsigned)id < a.n_pages;
-          if (there) from = (size_t)id * a.n_kv + kvh;
-        }
-        copy4(sb + S::scales + (st * 2 * S::GROUPS + tid) * 4u, (tid < S::GROUPS ? a.ks : a.vs) + from, there);
-      }
+    };
+    int id[S::NP];
+    auto pages = [&](unsigned i) {
+#pragma unroll
+      for (int b = 0; b < S::NP; b++) id[b] = i < n ? page_of(p_first + (int)i * S::TILE + 16 * b) : -1;
     };
 #pragma unroll
     for (int i = 0; i < S::STAGES - 1; i++) {
-      if ((unsigned)i < n) send(t0 + i, (unsigned)i);
+      pages((unsigned)i);
+      if ((unsigned)i < n) send(p_first + i * S::TILE, id, (unsigned)i);
       copies_sent();
     }
+    pages(S::STAGES - 1);
 
-    // ---- q: rows g and g + 8, dims 16 c .. 16 c + 15 of every 64: what the codes of a 16-byte read meet.  f32 rows are brought to 2^14 by a
-    // power of two (per half of a head) and split into two f16 terms
-    const unsigned kh = S::KH == 2 ? warp >> 2 : 0u, pw = S::KH == 2 ? warp & 3u : warp;
-    uint32_t qa[S::TERMS][S::KR / 64][4][4];
+    // ---- q: row g, dims 16 c .. 16 c + 15 of every 64: what the codes of a 16-byte read meet.  f32 rows are brought to 2^14 by a power of
+    // two and split into two f16 terms
+    uint32_t qb[S::TERMS][S::KK][4][2];
     float up[2] = {1.0f, 1.0f};
-#pragma unroll
-    for (int h = 0; h < 2; h++) {
-      const unsigned m = m0 + g + 8u * h;
+    {
+      const unsigned m = m0 + g;
       const bool in = m < m_rows;
-      const T* src = (const T*)a.q + ((size_t)(s.row0 + (int)(m / a.G)) * a.n_q + kvh * a.G + m % a.G) * HD + kh * S::KR + 16u * c;
+      const T* src = (const T*)a.q + ((size_t)(s.row0 + (int)(m / a.G)) * a.n_q + kvh * a.G + m % a.G) * HD + 16u * c;
       if constexpr (S::TERMS == 1) {
 #pragma unroll
-        for (int kk = 0; kk < S::KR / 64; kk++) {
+        for (int kk = 0; kk < S::KK; kk++) {
           const uint4 x = in ? *reinterpret_cast<const uint4*>(src + 64 * kk) : make_uint4(0, 0, 0, 0), y = in ? *reinterpret_cast<const uint4*>(src + 64 * kk + 8) : make_uint4(0, 0, 0, 0);
           const uint32_t w[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
 #pragma unroll
           for (int k = 0; k < 4; k++) {
-            qa[0][kk][k][h] = w[2 * k];
-            qa[0][kk][k][h + 2] = w[2 * k + 1];
+            qb[0][kk][k][0] = w[2 * k];
+            qb[0][kk][k][1] = w[2 * k + 1];
           }
         }
       } else {
-        float x[S::KR / 64][16], big = 0.0f;
+        float x[S::KK][16], big = 0.0f;
 #pragma unroll
-        for (int kk = 0; kk < S::KR / 64; kk++)
+        for (int kk = 0; kk < S::KK; kk++)
 #pragma unroll
           for (int e = 0; e < 16; e += 4) {
             const float4 v = in ? *reinterpret_cast<const float4*>((const float*)src + 64 * kk + e) : make_float4(0.f, 0.f, 0.f, 0.f);
@@ -273,213 +297,273 @@ __global__ void __launch_bounds__(256, 2) sdpa_q8_split_kernel(const SdpaArgs a)
         big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
         big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
         const int ex = big > 0.0f && big < 3.0e38f ? max((int)(__float_as_uint(big) >> 23) - 127 - 14, -100) : 0;
-        up[h] = __uint_as_float((uint32_t)(127 + ex) << 23);
-        const float down = __uint_as_float((uint32_t)(127 - ex) << 23);
+        const float mul = __uint_as_float((uint32_t)(127 + ex) << 23), down = __uint_as_float((uint32_t)(127 - ex) << 23);
+        up[0] = __shfl_sync(0xffffffffu, mul, 8u * c);
+        up[1] = __shfl_sync(0xffffffffu, mul, 8u * c + 4u);
 #pragma unroll
-        for (int kk = 0; kk < S::KR / 64; kk++)
+        for (int kk = 0; kk < S::KK; kk++)
 #pragma unroll
           for (int e = 0; e < 16; e += 2) {
             const float x0 = x[kk][e] * down, x1 = x[kk][e + 1] * down;
             const __half2 hi = __floats2half2_rn(x0, x1);
             const float2 f = __half22float2(hi);
-            const int k = e / 4, r = h + (e & 2);
-            qa[0][kk][k][r] = q8_u32(hi);
-            qa[S::TERMS - 1][kk][k][r] = q8_u32(__floats2half2_rn(x0 - f.x, x1 - f.y));
+            qb[0][kk][e / 4][(e & 2) / 2] = q8_u32(hi);
+            qb[S::TERMS - 1][kk][e / 4][(e & 2) / 2] = q8_u32(__floats2half2_rn(x0 - f.x, x1 - f.y));
           }
       }
     }
-    // ---- a row of scores: 16 threads, COLS neighbouring positions each
-    const unsigned row = tid >> 4, col = (tid & 15u) * S::COLS;
-    int lo = 0, hi = -1;  // positions lo .. hi are seen
-    if (m0 + row < m_rows) {
-      hi = s.len - s.rows + (int)((m0 + row) / a.G);
-      lo = a.window && hi >= (int)a.window ? hi - (int)a.window + 1 : 0;
+    // ---- this lane's scores: positions g (+ 8) of query rows 2 c and 2 c + 1, which see positions lo .. hi
+    int lo[2], hi[2], lo_all, hi_all;
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+      const unsigned m = min(m0 + 2u * c + h, m_rows - 1u);  // (columns behind the last row repeat it)
+      hi[h] = s.len - s.rows + (int)(m / a.G);
+      lo[h] = a.window && hi[h] >= (int)a.window ? hi[h] - (int)a.window + 1 : 0;
     }
-    float m = kNone, l = 0.0f, acc[4][4];
+    hi_all = s.len - s.rows + (int)(m0 / a.G);
+    {
+      const int last = s.len - s.rows + (int)(min(m0 + 7u, m_rows - 1u) / a.G);
+      lo_all = a.window && last >= (int)a.window ? last - (int)a.window + 1 : 0;
+    }
+    float m[2] = {kNone, kNone}, l[2] = {0.0f, 0.0f}, acc[S::WN][S::WW][2][4];
 #pragma unroll
-    for (int j = 0; j < 4; j++)
+    for (int w = 0; w < S::WN; w++)
 #pragma unroll
-      for (int e = 0; e < 4; e++) acc[j][e] = 0.0f;
-    const float to_log2 = a.scale * 1.44269504088896340736f;
-    const unsigned dg = warp % S::DG, pg = warp / S::DG;
+      for (int k = 0; k < S::WW; k++)
+#pragma unroll
+        for (int e = 0; e < 8; e++) acc[w][k][e / 4][e % 4] = 0.0f;
 
+    unsigned st = 0;
     for (unsigned i = 0; i < n; i++) {
-      const unsigned st = i % S::STAGES;
       copies_wait<S::STAGES - 2>();
-      __syncthreads();
-      if (i + S::STAGES - 1 < n) send(t0 + (int)(i + S::STAGES - 1), (i + S::STAGES - 1) % S::STAGES);
-      copies_sent();
-      // scores of 16 positions
+      __syncwarp();
+      const int p0 = p_first + (int)i * S::TILE;
       {
-        float d[2][4];
+        const unsigned to = st == 0 ? S::STAGES - 1 : st - 1u;
+        if (i + S::STAGES - 1 < n) send(p0 + (S::STAGES - 1) * S::TILE, id, to);
+        copies_sent();
+        pages(i + S::STAGES);
+      }
+      const unsigned char* at_k = ring + st * S::stage_bytes;
+      const unsigned char* at_v = at_k + S::SUB * HD;
+      // scores
+      float x[S::NP][4];
 #pragma unroll
-        for (int nt = 0; nt < 2; nt++)
+      for (int b = 0; b < S::NP; b++) {
+        float d[2 * S::TERMS][4];
 #pragma unroll
-          for (int e = 0; e < 4; e++) d[nt][e] = 0.0f;
+        for (int k = 0; k < 2 * S::TERMS; k++)
 #pragma unroll
-        for (int nt = 0; nt < 2; nt++) {
-          const unsigned p = pw * 16u + nt * 8u + g;
+          for (int e = 0; e < 4; e++) d[k][e] = 0.0f;
 #pragma unroll
-          for (int kk = 0; kk < S::KR / 64; kk++) {
-            const unsigned ch = kh * (S::KR / 16) + 4u * kk + c, kch = HD >= 128 ? ch ^ ((p & 1u) << 2) : ch;
-            const uint4 w = *reinterpret_cast<const uint4*>(smem + st * S::stage_bytes + p * HD + kch * 16u);
-            const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
+        for (int kk = 0; kk < S::KK; kk++) {
+          const unsigned ch = 4u * kk + c, r = 16u * b + g, kch = HD >= 128 ? ch ^ ((g & 1u) << 2) : ch;
+          const uint4 u0 = *reinterpret_cast<const uint4*>(at_k + r * HD + kch * 16u), u1 = *reinterpret_cast<const uint4*>(at_k + (r + 8u) * HD + kch * 16u);
+          const uint32_t w0[4] = {u0.x, u0.y, u0.z, u0.w}, w1[4] = {u1.x, u1.y, u1.z, u1.w};
 #pragma unroll
-            for (int k = 0; k < 4; k++) {
-              uint32_t b0, b1;
-              widen4<FP8>(ww[k], b0, b1);
-              if constexpr (S::TERMS == 2) mma16816(d[nt], qa[S::TERMS - 1][kk][k], b0, b1);
-              mma16816(d[nt], qa[0][kk][k], b0, b1);
+          for (int k = 0; k < 4; k++) {
+            uint32_t af[4];
+            widen4<FP8>(w0[k], af[0], af[2]);
+            widen4<FP8>(w1[k], af[1], af[3]);
+            if constexpr (S::TERMS == 2) mma16816(d[2 + (k & 1)], af, qb[S::TERMS - 1][kk][k][0], qb[S::TERMS - 1][kk][k][1]);
+            mma16816(d[k & 1], af, qb[0][kk][k][0], qb[0][kk][k][1]);
+          }
+        }
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          x[b][e] = d[0][e] + d[1][e];
+          if constexpr (S::TERMS == 2) x[b][e] += d[2][e] + d[2 * S::TERMS - 1][e];
+        }
+      }
+      // probabilities
+      float vf[S::NP], vd[S::NP], top[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+      for (int b = 0; b < S::NP; b++) {
+        const float2 sc = *reinterpret_cast<const float2*>(scales + (st * S::NP + b) * 2);
+        const float ks = q8_scale(sc.x) * to_log2;
+        float ve;
+        split_scale(q8_scale(sc.y), ve, vf[b], vd[b]);
+#pragma unroll
+        for (int e = 0; e < 4; e++) x[b][e] = fmaf(x[b][e], S::TERMS == 2 ? ks * up[e & 1] : ks, ve);
+      }
+      if (p0 < lo_all || p0 + S::SUB - 1 > hi_all) {
+#pragma unroll
+        for (int b = 0; b < S::NP; b++)
+#pragma unroll
+          for (int e = 0; e < 4; e++) {
+            const int p = p0 + 16 * b + (int)g + (e >> 1) * 8;
+            if (p < lo[e & 1] || p > hi[e & 1]) x[b][e] = -INFINITY;
+          }
+      }
+#pragma unroll
+      for (int b = 0; b < S::NP; b++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) top[e & 1] = fmaxf(top[e & 1], x[b][e]);
+      if (__any_sync(0xffffffffu, top[0] > m[0] + kSlack || top[1] > m[1] + kSlack)) {
+        float turn[2];
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+#pragma unroll
+          for (int o = 4; o < 32; o <<= 1) top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], o));
+          top[h] = fmaxf(top[h], m[h]);
+          turn[h] = exp2_fast(m[h] - top[h]);
+          m[h] = top[h];
+          l[h] *= turn[h];
+        }
+#pragma unroll
+        for (int w = 0; w < S::WN; w++)
+#pragma unroll
+          for (int k = 0; k < S::WW; k++)
+#pragma unroll
+            for (int e = 0; e < 8; e++) acc[w][k][e / 4][e % 4] *= turn[e & 1];
+      }
+      uint32_t pb[S::NP][S::TERMS][2];
+#pragma unroll
+      for (int b = 0; b < S::NP; b++) {
+        const float f = vf[b] * kProbs;
+        float sum[2];
+#pragma unroll
+        for (int e = 0; e < 4; e++) x[b][e] = exp2_fast(x[b][e] - m[e & 1]);
+        sum[0] = x[b][0] + x[b][2];
+        sum[1] = x[b][1] + x[b][3];
+        l[0] = fmaf(sum[0], vd[b], l[0]);
+        l[1] = fmaf(sum[1], vd[b], l[1]);
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+          const float y0 = x[b][2 * h] * f, y1 = x[b][2 * h + 1] * f;
+          const __half2 big = __floats2half2_rn(y0, y1);
+          pb[b][0][h] = turn8x8(q8_u32(big));
+          if constexpr (S::TERMS == 2) {
+            const float2 t = __half22float2(big);
+            pb[b][S::TERMS - 1][h] = turn8x8(q8_u32(__floats2half2_rn(y0 - t.x, y1 - t.y)));
+          }
+        }
+      }
+      // values
+#pragma unroll
+      for (int w = 0; w < S::WN; w++) {
+        uint32_t v[S::NP][4][S::WW];
+#pragma unroll
+        for (int b = 0; b < S::NP; b++)
+#pragma unroll
+          for (int e = 0; e < 4; e++) {
+            const unsigned r = 16u * b + 2u * c + (e & 1) + (e >> 1) * 8u, byte = w * S::W + g * (S::W / 8), ch = byte >> 4;
+            const unsigned vch = HD >= 128 ? ch ^ ((r >> 1 & 3u) << 1) : ch ^ ((r >> 1 & 1u) << 1);
+            const unsigned char* from = at_v + r * HD + vch * 16u + (byte & 15u);
+            if constexpr (S::WW == 4) {
+              const uint4 y = *reinterpret_cast<const uint4*>(from);
+              v[b][e][0] = y.x; v[b][e][1] = y.y; v[b][e][2] = y.z; v[b][e][3] = y.w;
+            } else {
+              const uint2 y = *reinterpret_cast<const uint2*>(from);
+              v[b][e][0] = y.x; v[b][e][1] = y.y;
+            }
+          }
+#pragma unroll
+        for (int k = 0; k < S::WW; k++) {
+          float d[2][4];
+#pragma unroll
+          for (int b = 0; b < S::NP; b++) {
+            uint32_t p01[4], p89[4];
+            widen_pairs<FP8>(v[b][0][k], v[b][1][k], p01);
+            widen_pairs<FP8>(v[b][2][k], v[b][3][k], p89);
+#pragma unroll
+            for (int t = 0; t < 2; t++) {
+              const uint32_t af[4] = {p01[2 * t], p01[2 * t + 1], p89[2 * t], p89[2 * t + 1]};
+              if constexpr (S::TERMS == 2) {
+                if (b == 0)
+#pragma unroll
+                  for (int e = 0; e < 4; e++) d[t][e] = 0.0f;
+                mma16816(d[t], af, pb[b][S::TERMS - 1][0], pb[b][S::TERMS - 1][1]);
+                mma16816(d[t], af, pb[b][0][0], pb[b][0][1]);
+              } else {
+                mma16816(acc[w][k][t], af, pb[b][0][0], pb[b][0][1]);
+              }
+            }
+          }
+          if constexpr (S::TERMS == 2)
+#pragma unroll
+            for (int e = 0; e < 8; e++) acc[w][k][e / 4][e % 4] += d[e / 4][e % 4];
+        }
+      }
+      st = st + 1u == S::STAGES ? 0u : st + 1u;
+      __syncwarp();  // the stage has been read
+    }
+    // ---- the warps' results together: to `out`, or a record if other blocks have a part of the piece
+    copies_wait<0>();
+#pragma unroll
+    for (int h = 0; h < 2; h++)
+#pragma unroll
+      for (int o = 4; o < 32; o <<= 1) l[h] += __shfl_xor_sync(0xffffffffu, l[h], o);
+    if (g == 0) {
+#pragma unroll
+      for (int h = 0; h < 2; h++) {
+        row_m[warp][2u * c + h] = m[h];
+        row_l[warp][2u * c + h] = l[h];
+      }
+    }
+    __syncthreads();  // every ring is free
+    float* mid = reinterpret_cast<float*>(smem);
+#pragma unroll
+    for (int w = 0; w < S::WN; w++)
+#pragma unroll
+      for (int k = 0; k < S::WW; k++)
+#pragma unroll
+        for (int h = 0; h < 2; h++)
+          *reinterpret_cast<float4*>(mid + (size_t)(warp * 8u + 2u * c + h) * S::OP + w * S::W + g * (S::W / 8) + 4 * k) =
+              make_float4(acc[w][k][0][h], acc[w][k][0][h + 2], acc[w][k][1][h], acc[w][k][1][h + 2]);
+    __syncthreads();
+    {
+      // a warp a row: the lanes share its dims
+      const unsigned r = warp, mm = m0 + r;
+      float top = kNone, sum = 0.0f, e[S::WARPS];
+#pragma unroll
+      for (int w = 0; w < S::WARPS; w++) top = fmaxf(top, row_m[w][r]);
+#pragma unroll
+      for (int w = 0; w < S::WARPS; w++) {
+        e[w] = exp2_fast(row_m[w][r] - top);
+        sum = fmaf(e[w], row_l[w][r], sum);
+      }
+      const bool whole = n == (unsigned)n_tiles;
+      float* rec = a.part + ((size_t)blockIdx.x * 2u + (in_block ? 1u : 0u)) * S::record;
+      if (!whole && lane == 0) {
+        rec[r] = top;
+        rec[8 + r] = sum;
+      }
+      const float f = whole ? over(sum) : 1.0f;
+      if (mm < m_rows) {
+        constexpr int D = HD / 32;
+        float v[D];
+#pragma unroll
+        for (int d = 0; d < D; d++) v[d] = 0.0f;
+#pragma unroll
+        for (int w = 0; w < S::WARPS; w++) {
+          const float* from = mid + (size_t)(w * 8u + r) * S::OP;
+          if constexpr (D == 2) {
+            const float2 y = *reinterpret_cast<const float2*>(from + 2u * lane);
+            v[0] = fmaf(y.x, e[w], v[0]);
+            v[1] = fmaf(y.y, e[w], v[1]);
+          } else {
+#pragma unroll
+            for (int d = 0; d < D; d += 4) {
+              const float4 y = *reinterpret_cast<const float4*>(from + 4u * lane + 32 * d);
+              v[d] = fmaf(y.x, e[w], v[d]);
+              v[d + 1] = fmaf(y.y, e[w], v[d + 1]);
+              v[d + 2] = fmaf(y.z, e[w], v[d + 2]);
+              v[d + 3] = fmaf(y.w, e[w], v[d + 3]);
             }
           }
         }
-        float* to = reinterpret_cast<float*>(smem + S::scores) + (size_t)kh * 16 * S::SP + pw * 16u + 2u * c;
+        T* to = (T*)a.out + ((size_t)(s.row0 + (int)(mm / a.G)) * a.n_q + kvh * a.G + mm % a.G) * HD;
 #pragma unroll
-        for (int nt = 0; nt < 2; nt++) {
-          *reinterpret_cast<float2*>(to + g * S::SP + nt * 8) = make_float2(d[nt][0] * up[0], d[nt][1] * up[0]);
-          *reinterpret_cast<float2*>(to + (g + 8u) * S::SP + nt * 8) = make_float2(d[nt][2] * up[1], d[nt][3] * up[1]);
-        }
-      }
-      __syncthreads();
-      {
-        const float* scales = reinterpret_cast<const float*>(smem + S::scales) + st * 2 * S::GROUPS + col / 16u;
-        const float ks = q8_scale(scales[0]) * to_log2;
-        float ve, vf, vd;
-        split_scale(q8_scale(scales[S::GROUPS]), ve, vf, vd);
-        const float* from = reinterpret_cast<const float*>(smem + S::scores) + row * S::SP + col;
-        float x[S::COLS], mx = m;
-        const int p0 = (t0 + (int)i) * S::TILE + (int)col;
+        for (int d = 0; d < D; d += D == 2 ? 2 : 4) {
+          const unsigned dim = (D == 2 ? 2u : 4u) * lane + 32u * d;
+          if (whole) {
 #pragma unroll
-        for (int k = 0; k < S::COLS; k += 4) {
-          float4 v = *reinterpret_cast<const float4*>(from + k);
-          if constexpr (S::KH == 2) {
-            const float4 w = *reinterpret_cast<const float4*>(from + 16 * S::SP + k);
-            v = make_float4(v.x + w.x, v.y + w.y, v.z + w.z, v.w + w.w);
+            for (int k = 0; k < (D == 2 ? 2 : 4); k++) v[d + k] *= f;
+            put_dims(to + dim, v + d, D == 2 ? 2 : 4);
+          } else {
+            put_dims(rec + 16 + r * HD + dim, v + d, D == 2 ? 2 : 4);
           }
-          x[k] = v.x; x[k + 1] = v.y; x[k + 2] = v.z; x[k + 3] = v.w;
-        }
-#pragma unroll
-        for (int k = 0; k < S::COLS; k++) {
-          x[k] = p0 + k >= lo && p0 + k <= hi ? fmaf(x[k], ks, ve) : -INFINITY;
-          mx = fmaxf(mx, x[k]);
-        }
-#pragma unroll
-        for (int o = 8; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-        const float turn = exp2_fast(m - mx);
-        m = mx;
-        float sum = 0.0f;
-#pragma unroll
-        for (int k = 0; k < S::COLS; k++) {
-          x[k] = exp2_fast(x[k] - mx);
-          sum += x[k];
-          x[k] *= vf * kProbs;
-        }
-        l = fmaf(l, turn, sum * vd);
-        __half* to = reinterpret_cast<__half*>(smem + S::probs) + row * S::SP + col;
-#pragma unroll
-        for (int k = 0; k < S::COLS; k += 2) {
-          const __half2 h = __floats2half2_rn(x[k], x[k + 1]);
-          *reinterpret_cast<__half2*>(to + k) = h;
-          if constexpr (S::TERMS == 2) {
-            const float2 f = __half22float2(h);
-            *reinterpret_cast<__half2*>(to + 16 * S::SP + k) = __floats2half2_rn(x[k] - f.x, x[k + 1] - f.y);
-          }
-        }
-        if ((tid & 15u) == 0) reinterpret_cast<float*>(smem + S::alpha)[row] = turn;
-      }
-      __syncthreads();
-      // values: 32 dims of the positions of this warp's share
-      {
-        float d[4][4];
-#pragma unroll
-        for (int j = 0; j < 4; j++)
-#pragma unroll
-          for (int e = 0; e < 4; e++) d[j][e] = 0.0f;
-        constexpr int KS = S::TILE / S::PG / 16;
-#pragma unroll
-        for (int k = 0; k < KS; k++) {
-          const unsigned base = pg * (S::TILE / S::PG) + 16u * k;
-          uint32_t p[S::TERMS][4];
-#pragma unroll
-          for (int t = 0; t < S::TERMS; t++) {
-            const uint32_t from = sb + S::probs + (t * 16 * S::SP + ((lane & 7u) + (lane >> 3 & 1u) * 8u) * S::SP + base + (lane >> 4) * 8u) * 2u;
-            asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(p[t][0]), "=r"(p[t][1]), "=r"(p[t][2]), "=r"(p[t][3]) : "r"(from) : "memory");
-          }
-          uint32_t w[4];
-#pragma unroll
-          for (int e = 0; e < 4; e++) {
-            const unsigned r = base + 2u * c + (e & 1) + (e >> 1) * 8u, byte = dg * 32u + 4u * g, ch = byte >> 4;
-            const unsigned vch = HD >= 128 ? ch ^ ((r >> 1 & 3u) << 1) : ch ^ ((r >> 1 & 1u) << 1);
-            w[e] = *reinterpret_cast<const uint32_t*>(smem + st * S::stage_bytes + S::TILE * HD + r * HD + vch * 16u + (byte & 15u));
-          }
-          uint32_t b0[4], b1[4];
-          widen_pairs<FP8>(w[0], w[1], b0);
-          widen_pairs<FP8>(w[2], w[3], b1);
-#pragma unroll
-          for (int j = 0; j < 4; j++) {
-            if constexpr (S::TERMS == 2) mma16816(d[j], p[S::TERMS - 1], b0[j], b1[j]);
-            mma16816(d[j], p[0], b0[j], b1[j]);
-          }
-        }
-        const float t0f = reinterpret_cast<const float*>(smem + S::alpha)[g], t1f = reinterpret_cast<const float*>(smem + S::alpha)[g + 8u];
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-          acc[j][0] = fmaf(acc[j][0], t0f, d[j][0]);
-          acc[j][1] = fmaf(acc[j][1], t0f, d[j][1]);
-          acc[j][2] = fmaf(acc[j][2], t1f, d[j][2]);
-          acc[j][3] = fmaf(acc[j][3], t1f, d[j][3]);
-        }
-      }
-    }
-    // ---- the piece's result: to `out`, or a record if other blocks have a part of it
-#pragma unroll
-    for (int o = 8; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
-    const bool whole = n == (unsigned)n_tiles;
-    float* rec = a.part + ((size_t)blockIdx.x * 2u + (in_block ? 1u : 0u)) * S::record;
-    if ((tid & 15u) == 0) {
-      if (whole) {
-        reinterpret_cast<float*>(smem + S::sums)[row] = l > 0.0f ? (1.0f / kProbs) / l : l == 0.0f ? 0.0f : l;  // (NaN stays)
-      } else {
-        rec[row] = m;
-        rec[16 + row] = l;
-      }
-    }
-    if constexpr (S::PG > 1) {
-      float* red = reinterpret_cast<float*>(smem + S::red);
-      if (pg > 0) {
-#pragma unroll
-        for (int h = 0; h < 2; h++) {
-          float* to = red + (size_t)(pg - 1u) * 16 * HD + (g + 8u * h) * HD + dg * 32u + 8u * c;
-          *reinterpret_cast<float4*>(to) = make_float4(acc[0][2 * h], acc[1][2 * h], acc[2][2 * h], acc[3][2 * h]);
-          *reinterpret_cast<float4*>(to + 4) = make_float4(acc[0][2 * h + 1], acc[1][2 * h + 1], acc[2][2 * h + 1], acc[3][2 * h + 1]);
-        }
-      }
-    }
-    __syncthreads();
-    if (pg == 0) {
-#pragma unroll
-      for (int h = 0; h < 2; h++) {
-        const unsigned r = g + 8u * h, mm = m0 + r;
-        float v[8];
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-          v[j] = acc[j][2 * h];
-          v[j + 4] = acc[j][2 * h + 1];
-        }
-        if constexpr (S::PG > 1)
-#pragma unroll
-          for (int k = 0; k < S::PG - 1; k++)
-#pragma unroll
-            for (int e = 0; e < 8; e++) v[e] += reinterpret_cast<const float*>(smem + S::red)[(size_t)k * 16 * HD + r * HD + dg * 32u + 8u * c + e];
-        if (mm >= m_rows) continue;
-        if (whole) {
-          const float f = reinterpret_cast<const float*>(smem + S::sums)[r];
-          T* to = (T*)a.out + ((size_t)(s.row0 + (int)(mm / a.G)) * a.n_q + kvh * a.G + mm % a.G) * HD + dg * 32u + 8u * c;
-          put8(to, v, f);
-        } else {
-          float* to = rec + 32 + r * HD + dg * 32u + 8u * c;
-          *reinterpret_cast<float4*>(to) = make_float4(v[0], v[1], v[2], v[3]);
-          *reinterpret_cast<float4*>(to + 4) = make_float4(v[4], v[5], v[6], v[7]);
         }
       }
     }
@@ -514,7 +598,7 @@ __global__ void __launch_bounds__(256) sdpa_q8_merge_kernel(const SdpaArgs a, un
     seq = found;
     piece = 0;
   } else {
-    const unsigned per = a.n_kv * ((a.few + 15u) / 16u);
+    const unsigned per = a.n_kv * ((a.few + 7u) / 8u);
     seq = blockIdx.x / per;
     piece = blockIdx.x % per;
   }
@@ -522,17 +606,17 @@ __global__ void __launch_bounds__(256) sdpa_q8_merge_kernel(const SdpaArgs a, un
   const unsigned long long units = a.first[seq + 1u] - at;
   Seq s;
   if (units == 0ull || !seq_of(a, seq, s)) return;
-  const unsigned m_rows = (unsigned)s.rows * a.G, m_tiles = (m_rows + 15u) / 16u;
+  const unsigned m_rows = (unsigned)s.rows * a.G, m_tiles = (m_rows + 7u) / 8u;
   const unsigned long long n_tiles = units / (m_tiles * a.n_kv);
   if (by_border) piece = (unsigned)((border - at) / n_tiles);
   else if (piece >= m_tiles * a.n_kv) return;
   const unsigned long long u0 = at + piece * n_tiles, u1 = u0 + n_tiles;
   const unsigned b0 = (unsigned)(((u0 + 1u) * blocks - 1u) / total), b1 = (unsigned)((u1 * blocks - 1u) / total);  // the blocks of its first and last unit
   if (b0 == b1 || (by_border && b0 != blockIdx.x)) return;  // whole; or another border's
-  const unsigned n = b1 - b0 + 1u, kvh = piece / m_tiles, m0 = piece % m_tiles * 16u;
+  const unsigned n = b1 - b0 + 1u, kvh = piece / m_tiles, m0 = piece % m_tiles * 8u;
   const unsigned slot0 = b0 * total / blocks >= u0 ? 0u : 1u;  // the first block's record is its second unless the piece starts with the block
   auto record = [&](unsigned k) { return a.part + ((size_t)(b0 + k) * 2u + (k ? 0u : slot0)) * S::record; };
-  for (unsigned r = blockIdx.y; r < 16u && m0 + r < m_rows; r += gridDim.y) {
+  for (unsigned r = blockIdx.y; r < 8u && m0 + r < m_rows; r += gridDim.y) {
     float mx = kNone;
     for (unsigned k = tid; k < n; k += 256u) mx = fmaxf(mx, record(k)[r]);
 #pragma unroll
@@ -544,20 +628,20 @@ __global__ void __launch_bounds__(256) sdpa_q8_merge_kernel(const SdpaArgs a, un
     for (unsigned k = tid; k < n; k += 256u) {
       const float e = exp2_fast(record(k)[r] - mx);
       fac[k] = e;
-      l = fmaf(e, record(k)[16 + r], l);
+      l = fmaf(e, record(k)[8 + r], l);
     }
     l = q8_warp_sum(l);
     if (lane == 0) l_s[warp] = l;
     __syncthreads();
     l = 0.0f;
     for (int w = 0; w < 8; w++) l += l_s[w];
-    const float f = l > 0.0f ? (1.0f / kProbs) / l : l == 0.0f ? 0.0f : l;
+    const float f = over(l);
     for (unsigned d0 = blockIdx.z * 64u; d0 < HD; d0 += gridDim.z * 64u) {
       const unsigned share = tid >> 4, d = (tid & 15u) * 4u;
       float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
       for (unsigned k = share; k < n; k += 16u) {
-        const float4 o = *reinterpret_cast<const float4*>(record(k) + 32 + r * HD + d0 + d);
+        const float4 o = *reinterpret_cast<const float4*>(record(k) + 16 + r * HD + d0 + d);
         const float e = fac[k];
         v.x = fmaf(o.x, e, v.x);
         v.y = fmaf(o.y, e, v.y);
@@ -577,8 +661,7 @@ __global__ void __launch_bounds__(256) sdpa_q8_merge_kernel(const SdpaArgs a, un
   }
 }
 
-constexpr unsigned kSplitPerSm = 2;  // blocks of the split kernel an SM holds (shared memory)
-unsigned split_blocks(const ks_ctx* ctx) { return (unsigned)ctx->sm_count * kSplitPerSm; }
+unsigned split_blocks(const ks_ctx* ctx, size_t hd) { return (unsigned)ctx->sm_count * (hd == 256 ? Split<256, float>::PER_SM : Split<128, float>::PER_SM); }  // as many as run at once
 size_t first_floats(const ks_page_tables* t) { return (2 * (t->n_seqs + 1) + 3) & ~size_t(3); }
 
 template <int HD, typename T, bool FP8>
@@ -593,9 +676,9 @@ int launch_split(ks_ctx* ctx, const SdpaArgs& a, unsigned blocks) {
   KS_LAUNCH(ctx, (sdpa_q8_split_kernel<HD, T, FP8>), blocks, S::THREADS, S::total, a);
   int rc = ks_after_launch(ctx, "sdpa_paged_q8");
   if (rc || blocks == 1) return rc;
-  const size_t pieces = (size_t)a.n_seqs * a.n_kv * ((a.few + 15u) / 16u);
+  const size_t pieces = (size_t)a.n_seqs * a.n_kv * ((a.few + 7u) / 8u);
   const bool by_border = pieces >= blocks;
-  const unsigned rows = a.few < 16u ? a.few : 16u;
+  const unsigned rows = a.few < 8u ? a.few : 8u;
   KS_LAUNCH(ctx, (sdpa_q8_merge_kernel<HD, T>), dim3(by_border ? blocks - 1u : (unsigned)pieces, by_border ? 1u : rows, by_border ? 1u : HD / 64u), 256, 0, a, blocks, by_border);
   return ks_after_launch(ctx, "sdpa_paged_q8 merge");
 }
@@ -606,7 +689,7 @@ extern "C" {
 
 size_t ks_sdpa_paged_tmp_floats(const ks_ctx* ctx, const ks_q8_cache* c, const ks_page_tables* t, size_t n_q, size_t rows_most) {
   if (!ctx || !c || !t || !c->n_kv || !rows_most || n_q < c->n_kv) return 0;
-  return first_floats(t) + (size_t)split_blocks(ctx) * 2 * 16 * (c->hd + 2);
+  return first_floats(t) + (size_t)split_blocks(ctx, c->hd) * 2 * 8 * (c->hd + 2);
 }
 
 int ks_sdpa_paged_q8(ks_ctx* ctx, const ks_q8_cache* c, const ks_page_tables* t, size_t n_q, size_t rows_most, size_t ctx_most, size_t window, float scale, ks_dtype act,
@@ -659,7 +742,7 @@ int ks_sdpa_paged_q8(ks_ctx* ctx, const ks_q8_cache* c, const ks_page_tables* t,
   a.G = (unsigned)G;
   a.window = (unsigned)window;
   a.scale = scale;
-  const unsigned blocks = split_blocks(ctx);
+  const unsigned blocks = split_blocks(ctx, c->hd);
 #define KS_AT(HD_, T_, F_) launch_split<HD_, T_, F_>(ctx, a, blocks)
 #define KS_AT_T(HD_, F_) (act == KS_F32 ? KS_AT(HD_, float, F_) : KS_AT(HD_, __half, F_))
 #define KS_AT_F(HD_) (c->dtype == KS_E4M3 ? KS_AT_T(HD_, true) : KS_AT_T(HD_, false))
