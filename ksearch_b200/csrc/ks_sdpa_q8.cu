@@ -2,44 +2,9 @@
 //
 // Row r of a sequence of `len` positions and `rows` rows sits at p = len - rows + r and sees positions max(0, p - window + 1) .. p:
 //   s_j = scale q . k_j,   out = sum_j exp(s_j - m) v_j / sum_j exp(s_j - m),   m = max_j s_j.
-#include "ks_q8.h"
-#include "ks_q8.cuh"
+#include "ks_sdpa_q8.cuh"
 
 namespace {
-
-struct SdpaArgs {
-  const uint8_t *kc, *vc;
-  const float *ks, *vs;
-  const int *lens, *tables, *row_start;
-  const void* q;
-  void* out;
-  float* part;               // records of split pieces
-  unsigned long long* first; // [n_seqs + 1]: units in front of each sequence
-  unsigned* bad;
-  unsigned n_seqs, max_blocks, n_pages, page_log, max_rows, rows_most, n_q, n_kv, G, window;
-  unsigned few;              // sequences of up to so many rows (times G) take the split kernel
-  unsigned least;            // units a block takes at least
-  float scale;
-};
-
-// ---- what a sequence has to do ------------------------------------------------------------------------------
-struct Seq {
-  int row0, rows, len, begin;  // first row of the call, rows, positions, first position that some row sees
-};
-__device__ __forceinline__ bool seq_of(const SdpaArgs& a, unsigned i, Seq& s) {  // false: nothing to do
-  const int r0 = a.row_start[i], r1 = a.row_start[i + 1u], len = a.lens[i];
-  s.row0 = r0;
-  s.rows = r1 - r0;
-  s.len = min(max(len, 0), (int)(a.max_blocks << a.page_log));
-  const int p0 = s.len - s.rows;
-  s.begin = a.window && p0 >= (int)a.window ? p0 - (int)a.window + 1 : 0;
-  if (s.rows <= 0) return false;
-  if (r0 < 0 || r1 > (int)a.max_rows || s.rows > (int)a.rows_most) {
-    if (blockIdx.x == 0) atomicOr(a.bad, KS_BAD_ROWS);
-    return false;
-  }
-  return true;
-}
 
 // ---- few rows: the context is what counts -------------------------------------------------------------------
 // A piece is 8 rows (row and query head of the group, counted together) of a sequence against one KV head; its units are tiles of TILE
@@ -69,10 +34,6 @@ struct Split {
   static constexpr unsigned record = 8 * (HD + 2);      // floats: m[8], l[8], O[8][HD]
   static_assert(WARPS * 8 * OP * 4 <= WARPS * ring, "the results fit the rings");
 };
-constexpr float kNone = -1.0e30f;       // the maximum of nothing
-constexpr float kProbs = 1024.0f;       // probabilities carry 2^10, are 2^5 at most, and 2^-35 of the largest is the least that counts
-constexpr float kSlack = 4.0f;          // log2 of how far a score may exceed what probabilities refer to
-
 __device__ __forceinline__ uint32_t smem_at(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool there) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
@@ -88,58 +49,14 @@ __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], 
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ float exp2_fast(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-// The four codes of a word as f16: 0, 1 and 2, 3.
-template <bool FP8>
-__device__ __forceinline__ void widen4(uint32_t w, uint32_t& lo, uint32_t& hi) {
-  if constexpr (FP8) {
-    lo = q8_u32(q8_decode2h<true>(w));
-    hi = q8_u32(q8_decode2h<true>(w >> 16));
-  } else {
-    w ^= 0x80808080u;
-    lo = q8_u32(__hsub2(q8_h2(__byte_perm(w, 0x64646464u, 0x4140)), __float2half2_rn(1152.0f)));
-    hi = q8_u32(__hsub2(q8_h2(__byte_perm(w, 0x64646464u, 0x4342)), __float2half2_rn(1152.0f)));
-  }
-}
-// Codes j = 0..3 of two rows' words as pairs (row a, row b).
-template <bool FP8>
-__device__ __forceinline__ void widen_pairs(uint32_t a, uint32_t b, uint32_t (&p)[4]) {
-  const uint32_t x = __byte_perm(a, b, 0x5140), y = __byte_perm(a, b, 0x7362);
-  widen4<FP8>(x, p[0], p[1]);
-  widen4<FP8>(y, p[2], p[3]);
-}
 // An 8 x 8 matrix of f16, a row's pair of columns per lane, transposed.
 __device__ __forceinline__ uint32_t turn8x8(uint32_t x) {
   uint32_t y;
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
   return y;
 }
-// What a row's values are multiplied by in the end; a row that saw nothing is zero, NaN stays.
-__device__ __forceinline__ float over(float l) { return l > 0.0f ? (1.0f / kProbs) / l : l == 0.0f ? 0.0f : l; }
-__device__ __forceinline__ void put_dims(float* to, const float* v, int n) {
-  if (n == 4) *reinterpret_cast<float4*>(to) = make_float4(v[0], v[1], v[2], v[3]);
-  else *reinterpret_cast<float2*>(to) = make_float2(v[0], v[1]);
-}
-__device__ __forceinline__ void put_dims(__half* to, const float* v, int n) {
-  const uint32_t x = q8_u32(__floats2half2_rn(v[0], v[1]));
-  if (n == 4) *reinterpret_cast<uint2*>(to) = make_uint2(x, q8_u32(__floats2half2_rn(v[2], v[3])));
-  else *reinterpret_cast<uint32_t*>(to) = x;
-}
-// A positive scale (inside q8_scale's range) as 2^e and a factor of 1 to 2.
-__device__ __forceinline__ void split_scale(float s, float& e, float& factor, float& down) {
-  const uint32_t b = __float_as_uint(s);
-  const int x = (int)(b >> 23) - 127;
-  e = (float)x;
-  factor = __uint_as_float((b & 0x7FFFFFu) | 0x3F800000u);
-  down = __uint_as_float((uint32_t)(127 - x) << 23);
-}
-
 template <int HD, typename T, bool FP8>
-__global__ void __launch_bounds__(Split<HD, T>::THREADS, Split<HD, T>::PER_SM) sdpa_q8_split_kernel(const SdpaArgs a) {
+__global__ void __launch_bounds__(Split<HD, T>::THREADS, Split<HD, T>::PER_SM) sdpa_q8_split_kernel(const ks_sdpa_q8_args a) {
   using S = Split<HD, T>;
   extern __shared__ __align__(128) unsigned char smem[];
   __shared__ unsigned long long scan[S::WARPS], seq_first;
@@ -223,14 +140,8 @@ __global__ void __launch_bounds__(Split<HD, T>::THREADS, Split<HD, T>::PER_SM) s
     const int p_first = (tile0 + (int)t_first) * S::TILE + (int)warp * S::SUB;                       // this warp's positions of the first
     const int* table = a.tables + (size_t)seq * a.max_blocks;
 
-    // the page of 16 positions (a page has no fewer), -1 where no row sees any of them
-    auto page_of = [&](int p) -> int {
-      if (p + 15 < s.begin || p >= s.len) return -1;
-      const int id = table[(unsigned)p >> a.page_log];
-      if (id >= 0 && (unsigned)id < a.n_pages) return id;
-      if (lane == 0) atomicOr(a.bad, KS_BAD_PAGE);
-      return -1;
-    };
+    // the page of 16 positions (a page has no fewer) as the table has it: read a step before it is looked at
+    auto page_of = [&](int p) -> int { return p + 15 < s.begin || p >= s.len ? -1 : table[(unsigned)p >> a.page_log]; };
     // copies of SUB positions into stage st: 16 bytes a lane, chunks swapped about so that the reads below meet no bank twice; positions that
     // nobody sees become zeros
     auto send = [&](int p0, const int (&id)[S::NP], unsigned st) {
@@ -238,18 +149,20 @@ __global__ void __launch_bounds__(Split<HD, T>::THREADS, Split<HD, T>::PER_SM) s
 #pragma unroll
       for (int b = 0; b < S::NP; b++) {
         const int p = p0 + 16 * b;
-        const size_t block = (size_t)(id[b] < 0 ? 0 : id[b]) * a.n_kv + kvh;
+        const bool page = (unsigned)id[b] < a.n_pages;
+        if (!page && p + 15 >= s.begin && p < s.len && lane == 0) atomicOr(a.bad, KS_BAD_PAGE);
+        const size_t block = (size_t)(page ? id[b] : 0) * a.n_kv + kvh;
         const size_t from = (((block << a.page_log) + ((unsigned)p & ((1u << a.page_log) - 1u)) + r0) * HD) + ch * 16u;
         const uint32_t to = ring_at + st * S::stage_bytes + (unsigned)b * 16u * HD;
 #pragma unroll
         for (int i = 0; i < S::COPIES / S::NP; i++) {
           const unsigned r = r0 + (unsigned)(i * S::LR);
-          const bool there = id[b] >= 0 && p + (int)r >= s.begin && p + (int)r < s.len;
+          const bool there = page && p + (int)r >= s.begin && p + (int)r < s.len;
           const unsigned kch = HD >= 128 ? ch ^ ((r & 1u) << 2) : ch, vch = HD >= 128 ? ch ^ ((r >> 1 & 3u) << 1) : ch ^ ((r >> 1 & 1u) << 1);
           copy16(to + r * HD + kch * 16u, a.kc + from + (size_t)(i * S::LR) * HD, there);
           copy16(to + S::SUB * HD + r * HD + vch * 16u, a.vc + from + (size_t)(i * S::LR) * HD, there);
         }
-        if (lane < 2u) copy4(scales_at + ((st * S::NP + b) * 2u + lane) * 4u, (lane ? a.vs : a.ks) + block, id[b] >= 0);
+        if (lane < 2u) copy4(scales_at + ((st * S::NP + b) * 2u + lane) * 4u, (lane ? a.vs : a.ks) + block, page);
       }
     };
     int id[S::NP];
@@ -578,7 +491,7 @@ __global__ void __launch_bounds__(Split<HD, T>::THREADS, Split<HD, T>::PER_SM) s
 // pieces than borders; rows; 64 dims).  Of a block's 256 threads 16 share 64 dims, and there are 16 shares of the records.
 constexpr unsigned kMergeMost = 1024;  // blocks of the split kernel
 template <int HD, typename T>
-__global__ void __launch_bounds__(256) sdpa_q8_merge_kernel(const SdpaArgs a, unsigned split_blocks, bool by_border) {
+__global__ void __launch_bounds__(256) sdpa_q8_merge_kernel(const ks_sdpa_q8_args a, unsigned split_blocks, bool by_border) {
   using S = Split<HD, T>;
   __shared__ float fac[kMergeMost], red[16][64 + 4], mx_s[8], l_s[8];
   __shared__ unsigned found;
@@ -665,7 +578,7 @@ unsigned split_blocks(const ks_ctx* ctx, size_t hd) { return (unsigned)ctx->sm_c
 size_t first_floats(const ks_page_tables* t) { return (2 * (t->n_seqs + 1) + 3) & ~size_t(3); }
 
 template <int HD, typename T, bool FP8>
-int launch_split(ks_ctx* ctx, const SdpaArgs& a, unsigned blocks) {
+int launch_split(ks_ctx* ctx, const ks_sdpa_q8_args& a, unsigned blocks) {
   using S = Split<HD, T>;
   static bool set[16] = {false};
   if (!set[ctx->device & 15]) {
@@ -683,13 +596,16 @@ int launch_split(ks_ctx* ctx, const SdpaArgs& a, unsigned blocks) {
   return ks_after_launch(ctx, "sdpa_paged_q8 merge");
 }
 
+size_t split_floats(const ks_ctx* ctx, const ks_q8_cache* c, const ks_page_tables* t) { return (first_floats(t) + (size_t)split_blocks(ctx, c->hd) * 2 * 8 * (c->hd + 2) + 3) & ~size_t(3); }
+
 }  // namespace
 
 extern "C" {
 
 size_t ks_sdpa_paged_tmp_floats(const ks_ctx* ctx, const ks_q8_cache* c, const ks_page_tables* t, size_t n_q, size_t rows_most) {
   if (!ctx || !c || !t || !c->n_kv || !rows_most || n_q < c->n_kv) return 0;
-  return first_floats(t) + (size_t)split_blocks(ctx, c->hd) * 2 * 8 * (c->hd + 2);
+  const size_t G = n_q / c->n_kv;
+  return split_floats(ctx, c, t) + (rows_most * G > KS_Q8_FEW ? ks_sdpa_q8_wide_floats(ctx, t->n_seqs, t->max_rows, c->n_kv, G, c->hd) : 0);
 }
 
 int ks_sdpa_paged_q8(ks_ctx* ctx, const ks_q8_cache* c, const ks_page_tables* t, size_t n_q, size_t rows_most, size_t ctx_most, size_t window, float scale, ks_dtype act,
@@ -713,10 +629,9 @@ int ks_sdpa_paged_q8(ks_ctx* ctx, const ks_q8_cache* c, const ks_page_tables* t,
   KS_REQUIRE(ctx, qa + bytes <= oa || oa + bytes <= qa, "%s: q and out overlap", who);
   KS_REQUIRE(ctx, ks_fits(tmp, 0, ks_sdpa_paged_tmp_floats(ctx, c, t, n_q, rows_most) * 4) && ks_aligned(tmp, 16), "%s: tmp buffer too small, or not on 16 bytes", who);
   if (rows_most == 0) return KS_OK;
-  (void)ctx_most;
   KS_REQUIRE_DEVICE(ctx, who);
   ks_on_device on(ctx);
-  SdpaArgs a{};
+  ks_sdpa_q8_args a{};
   a.kc = (const uint8_t*)c->k->dptr;
   a.vc = (const uint8_t*)c->v->dptr;
   a.ks = (const float*)c->k_scale->dptr;
@@ -728,7 +643,7 @@ int ks_sdpa_paged_q8(ks_ctx* ctx, const ks_q8_cache* c, const ks_page_tables* t,
   a.out = out->dptr;
   a.first = (unsigned long long*)tmp->dptr;
   a.part = (float*)tmp->dptr + first_floats(t);
-  a.few = (unsigned)(rows_most * G);
+  a.few = rows_most * G > KS_Q8_FEW ? KS_Q8_FEW : (unsigned)(rows_most * G);
   a.least = 1;
   a.bad = (unsigned*)ctx->ws + KS_WS_INDEX_WORD;
   a.n_seqs = (unsigned)t->n_seqs;
@@ -746,10 +661,12 @@ int ks_sdpa_paged_q8(ks_ctx* ctx, const ks_q8_cache* c, const ks_page_tables* t,
 #define KS_AT(HD_, T_, F_) launch_split<HD_, T_, F_>(ctx, a, blocks)
 #define KS_AT_T(HD_, F_) (act == KS_F32 ? KS_AT(HD_, float, F_) : KS_AT(HD_, __half, F_))
 #define KS_AT_F(HD_) (c->dtype == KS_E4M3 ? KS_AT_T(HD_, true) : KS_AT_T(HD_, false))
-  return c->hd == 256 ? KS_AT_F(256) : c->hd == 128 ? KS_AT_F(128) : KS_AT_F(64);
+  rc = c->hd == 256 ? KS_AT_F(256) : c->hd == 128 ? KS_AT_F(128) : KS_AT_F(64);
 #undef KS_AT_F
 #undef KS_AT_T
 #undef KS_AT
+  if (rc || rows_most * G <= KS_Q8_FEW) return rc;
+  return ks_launch_sdpa_q8_wide(ctx, a, c->hd, act, c->dtype == KS_E4M3, (float*)tmp->dptr + split_floats(ctx, c, t), ctx_most);
 }
 
 }  // extern "C"
