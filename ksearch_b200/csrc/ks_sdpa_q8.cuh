@@ -46,7 +46,7 @@ __device__ __forceinline__ bool seq_of(const ks_sdpa_q8_args& a, unsigned i, Seq
 }
 
 constexpr float kNone = -1.0e30f;       // the maximum of nothing
-constexpr float kProbs = 1024.0f;       // probabilities carry 2^10, are 2^5 at most, and 2^-35 of the largest is the least that counts
+constexpr float kProbs = 1024.0f, kProbsLog2 = 10.0f;       // probabilities carry 2^10, are 2^5 at most, and 2^-35 of the largest is the least that counts
 constexpr float kSlack = 4.0f;          // log2 of how far a score may exceed what probabilities refer to
 
 __device__ __forceinline__ float exp2_fast(float x) {
