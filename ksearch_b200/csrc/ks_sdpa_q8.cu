@@ -59,7 +59,7 @@ template <int HD, typename T, bool FP8>
 __global__ void __launch_bounds__(Split<HD, T>::THREADS, Split<HD, T>::PER_SM) sdpa_q8_split_kernel(const ks_sdpa_q8_args a) {
   using S = Split<HD, T>;
   extern __shared__ __align__(128) unsigned char smem[];
-  __shared__ unsigned long long scan[S::WARPS], seq_first;
+  __shared__ unsigned long long scan[S::WARPS], seq_first, line[2];
   __shared__ unsigned seq_at;
   __shared__ float row_m[S::WARPS][8], row_l[S::WARPS][8];
   ks_pdl_entry();
@@ -95,18 +95,20 @@ __global__ void __launch_bounds__(Split<HD, T>::THREADS, Split<HD, T>::PER_SM) s
     before += w < warp ? scan[w] : 0ull;
     total += scan[w];
   }
-  if (total == 0ull) {
-    if (blockIdx.x == 0 && tid == 0) a.first[a.n_seqs] = 0ull;
+  const unsigned long long blocks = min((unsigned long long)gridDim.x, (total + a.least - 1u) / a.least);
+  if (blockIdx.x >= blocks) {
+    if (tid == 0) a.merges[2u * blockIdx.x] = make_int4(0, 0, 0, 0);
     return;
   }
-  const unsigned long long blocks = min((unsigned long long)gridDim.x, (total + a.least - 1u) / a.least);
-  if (blockIdx.x >= blocks) return;
+  if (tid == 0) {
+    line[0] = total;
+    line[1] = blocks;
+  }
   const unsigned long long u_begin = blockIdx.x * total / blocks, u_end = (blockIdx.x + 1u) * total / blocks;
 #pragma unroll
   for (unsigned k = 0; k < KS_PAGES_MAX_SEQS / 256; k++) {
     const unsigned i = tid * per + k;
     if (k < per && i < a.n_seqs) {
-      if (blockIdx.x == 0) a.first[i] = before;
       if (u_begin >= before && u_begin - before < mine[k]) {
         seq_at = i;
         seq_first = before;
@@ -114,7 +116,6 @@ __global__ void __launch_bounds__(Split<HD, T>::THREADS, Split<HD, T>::PER_SM) s
       before += mine[k];
     }
   }
-  if (blockIdx.x == 0 && tid == 0) a.first[a.n_seqs] = total;
   __syncthreads();
 
   unsigned char* ring = smem + warp * S::ring;
@@ -480,6 +481,14 @@ __global__ void __launch_bounds__(Split<HD, T>::THREADS, Split<HD, T>::PER_SM) s
         }
       }
     }
+    // what the merge has to do for this block: the piece that began in an earlier one and ends here, if there is one
+    if (in_block == 0 && tid == 0) {
+      const bool ends = t_first > 0 && t_first + n == (unsigned)n_tiles;
+      const unsigned long long u0 = u - t_first, total = line[0], blocks = line[1];
+      const unsigned b0 = (unsigned)(((u0 + 1u) * blocks - 1u) / total);
+      a.merges[2u * blockIdx.x] = make_int4((int)b0, ends ? (int)(blockIdx.x - b0 + 1u) : 0, b0 * total / blocks >= u0 ? 0 : 1, (int)m0);
+      a.merges[2u * blockIdx.x + 1u] = make_int4(s.row0, (int)kvh, (int)m_rows, 0);
+    }
     u += n;
     in_block++;
     __syncthreads();  // everything in shared memory is free again
@@ -487,95 +496,70 @@ __global__ void __launch_bounds__(Split<HD, T>::THREADS, Split<HD, T>::PER_SM) s
 }
 
 // ---- the records of pieces that lie in several blocks ----------------------------------------------------------
-// out = sum_b e_b O_b / sum_b e_b l_b, e_b = exp2(m_b - max m), in the order of the blocks.  Grid: (pieces, or block borders where there are more
-// pieces than borders; rows; 64 dims).  Of a block's 256 threads 16 share 64 dims, and there are 16 shares of the records.
-constexpr unsigned kMergeMost = 1024;  // blocks of the split kernel
+// out = sum_b e_b O_b / sum_b e_b l_b, e_b = exp2(m_b - max m), in the order of the blocks.  A block for each of the split kernel's, for the piece that
+// ends there; its warps are 8 rows x 4 shares of the records.
 template <int HD, typename T>
-__global__ void __launch_bounds__(256) sdpa_q8_merge_kernel(const ks_sdpa_q8_args a, unsigned split_blocks, bool by_border) {
+__global__ void __launch_bounds__(1024) sdpa_q8_merge_kernel(const ks_sdpa_q8_args a) {
   using S = Split<HD, T>;
-  __shared__ float fac[kMergeMost], red[16][64 + 4], mx_s[8], l_s[8];
-  __shared__ unsigned found;
+  constexpr int D = HD / 32, V = D == 2 ? 2 : 4;
+  __shared__ float red[3][8][HD];
   ks_pdl_entry();
-  const unsigned tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5;
-  const unsigned long long total = a.first[a.n_seqs];
-  if (total == 0ull) return;
-  const unsigned long long blocks = min((unsigned long long)split_blocks, (total + a.least - 1u) / a.least);
-  unsigned seq, piece;
-  unsigned long long at, border = 0;
-  if (by_border) {
-    if (blockIdx.x + 1u >= blocks) return;
-    border = (blockIdx.x + 1u) * total / blocks;  // first unit of block blockIdx.x + 1
-    for (unsigned i = tid; i < a.n_seqs; i += 256u)
-      if (a.first[i] <= border && border < a.first[i + 1u]) found = i;
-    __syncthreads();
-    seq = found;
-    piece = 0;
-  } else {
-    const unsigned per = a.n_kv * ((a.few + 7u) / 8u);
-    seq = blockIdx.x / per;
-    piece = blockIdx.x % per;
-  }
-  at = a.first[seq];
-  const unsigned long long units = a.first[seq + 1u] - at;
-  Seq s;
-  if (units == 0ull || !seq_of(a, seq, s)) return;
-  const unsigned m_rows = (unsigned)s.rows * a.G, m_tiles = (m_rows + 7u) / 8u;
-  const unsigned long long n_tiles = units / (m_tiles * a.n_kv);
-  if (by_border) piece = (unsigned)((border - at) / n_tiles);
-  else if (piece >= m_tiles * a.n_kv) return;
-  const unsigned long long u0 = at + piece * n_tiles, u1 = u0 + n_tiles;
-  const unsigned b0 = (unsigned)(((u0 + 1u) * blocks - 1u) / total), b1 = (unsigned)((u1 * blocks - 1u) / total);  // the blocks of its first and last unit
-  if (b0 == b1 || (by_border && b0 != blockIdx.x)) return;  // whole; or another border's
-  const unsigned n = b1 - b0 + 1u, kvh = piece / m_tiles, m0 = piece % m_tiles * 8u;
-  const unsigned slot0 = b0 * total / blocks >= u0 ? 0u : 1u;  // the first block's record is its second unless the piece starts with the block
-  auto record = [&](unsigned k) { return a.part + ((size_t)(b0 + k) * 2u + (k ? 0u : slot0)) * S::record; };
-  for (unsigned r = blockIdx.y; r < 8u && m0 + r < m_rows; r += gridDim.y) {
-    float mx = kNone;
-    for (unsigned k = tid; k < n; k += 256u) mx = fmaxf(mx, record(k)[r]);
+  const unsigned lane = threadIdx.x & 31u, warp = threadIdx.x >> 5, r = warp & 7u, share = warp >> 3;
+  const int4 job = a.merges[2u * blockIdx.x], where = a.merges[2u * blockIdx.x + 1u];
+  const unsigned n = (unsigned)job.y, m = (unsigned)job.w + r;
+  if (n == 0u) return;
+  const float* rec = a.part + (size_t)job.x * 2u * S::record;
+  auto record = [&](unsigned k) { return rec + (k ? k * 2u : (unsigned)job.z) * (size_t)S::record; };  // (the first block's record is its second one unless the piece starts with the block)
+  float top = kNone, l = 0.0f, v[D];
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-    if (lane == 0) mx_s[warp] = mx;
-    __syncthreads();
-    for (int w = 0; w < 8; w++) mx = fmaxf(mx, mx_s[w]);
-    float l = 0.0f;
-    for (unsigned k = tid; k < n; k += 256u) {
-      const float e = exp2_fast(record(k)[r] - mx);
-      fac[k] = e;
-      l = fmaf(e, record(k)[8 + r], l);
-    }
+  for (int d = 0; d < D; d++) v[d] = 0.0f;
+  const bool live = m < (unsigned)where.z;
+  if (live) {
+    for (unsigned k = lane; k < n; k += 32u) top = fmaxf(top, record(k)[r]);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    for (unsigned k = lane; k < n; k += 32u) l = fmaf(exp2_fast(record(k)[r] - top), record(k)[8 + r], l);
     l = q8_warp_sum(l);
-    if (lane == 0) l_s[warp] = l;
-    __syncthreads();
-    l = 0.0f;
-    for (int w = 0; w < 8; w++) l += l_s[w];
-    const float f = over(l);
-    for (unsigned d0 = blockIdx.z * 64u; d0 < HD; d0 += gridDim.z * 64u) {
-      const unsigned share = tid >> 4, d = (tid & 15u) * 4u;
-      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
-      for (unsigned k = share; k < n; k += 16u) {
-        const float4 o = *reinterpret_cast<const float4*>(record(k) + 16 + r * HD + d0 + d);
-        const float e = fac[k];
-        v.x = fmaf(o.x, e, v.x);
-        v.y = fmaf(o.y, e, v.y);
-        v.z = fmaf(o.z, e, v.z);
-        v.w = fmaf(o.w, e, v.w);
-      }
-      *reinterpret_cast<float4*>(&red[share][d]) = v;
-      __syncthreads();
-      if (tid < 64u) {
-        float x = 0.0f;
+    for (unsigned k = share; k < n; k += 4u) {
+      const float* x = record(k);
+      const float e = exp2_fast(x[r] - top);
 #pragma unroll
-        for (int k = 0; k < 16; k++) x += red[k][tid];
-        ((T*)a.out)[((size_t)(s.row0 + (int)((m0 + r) / a.G)) * a.n_q + kvh * a.G + (m0 + r) % a.G) * HD + d0 + tid] = (T)(x * f);
+      for (int d = 0; d < D; d += V) {
+        const float* from = x + 16 + r * HD + V * lane + 32 * d;
+        if constexpr (V == 4) {
+          const float4 y = *reinterpret_cast<const float4*>(from);
+          v[d] = fmaf(y.x, e, v[d]);
+          v[d + 1] = fmaf(y.y, e, v[d + 1]);
+          v[d + 2] = fmaf(y.z, e, v[d + 2]);
+          v[d + 3] = fmaf(y.w, e, v[d + 3]);
+        } else {
+          const float2 y = *reinterpret_cast<const float2*>(from);
+          v[d] = fmaf(y.x, e, v[d]);
+          v[d + 1] = fmaf(y.y, e, v[d + 1]);
+        }
       }
-      __syncthreads();
     }
+    if (share > 0)
+#pragma unroll
+      for (int d = 0; d < D; d += V) put_dims(&red[share - 1u][r][V * lane + 32 * d], v + d, V);
+  }
+  __syncthreads();
+  if (!live || share > 0) return;
+  const float f = over(l);
+  T* to = (T*)a.out + ((size_t)(where.x + (int)(m / a.G)) * a.n_q + (unsigned)where.y * a.G + m % a.G) * HD;
+#pragma unroll
+  for (int d = 0; d < D; d += V) {
+#pragma unroll
+    for (int k = 0; k < V; k++) {
+      const unsigned at = V * lane + 32 * d + k;
+      v[d + k] = (v[d + k] + red[0][r][at] + (red[1][r][at] + red[2][r][at])) * f;
+    }
+    put_dims(to + V * lane + 32 * d, v + d, V);
   }
 }
 
 unsigned split_blocks(const ks_ctx* ctx, size_t hd) { return (unsigned)ctx->sm_count * (hd == 256 ? Split<256, float>::PER_SM : Split<128, float>::PER_SM); }  // as many as run at once
-size_t first_floats(const ks_page_tables* t) { return (2 * (t->n_seqs + 1) + 3) & ~size_t(3); }
 
 template <int HD, typename T, bool FP8>
 int launch_split(ks_ctx* ctx, const ks_sdpa_q8_args& a, unsigned blocks) {
@@ -589,14 +573,11 @@ int launch_split(ks_ctx* ctx, const ks_sdpa_q8_args& a, unsigned blocks) {
   KS_LAUNCH(ctx, (sdpa_q8_split_kernel<HD, T, FP8>), blocks, S::THREADS, S::total, a);
   int rc = ks_after_launch(ctx, "sdpa_paged_q8");
   if (rc || blocks == 1) return rc;
-  const size_t pieces = (size_t)a.n_seqs * a.n_kv * ((a.few + 7u) / 8u);
-  const bool by_border = pieces >= blocks;
-  const unsigned rows = a.few < 8u ? a.few : 8u;
-  KS_LAUNCH(ctx, (sdpa_q8_merge_kernel<HD, T>), dim3(by_border ? blocks - 1u : (unsigned)pieces, by_border ? 1u : rows, by_border ? 1u : HD / 64u), 256, 0, a, blocks, by_border);
+  KS_LAUNCH(ctx, (sdpa_q8_merge_kernel<HD, T>), blocks, 1024, 0, a);
   return ks_after_launch(ctx, "sdpa_paged_q8 merge");
 }
 
-size_t split_floats(const ks_ctx* ctx, const ks_q8_cache* c, const ks_page_tables* t) { return (first_floats(t) + (size_t)split_blocks(ctx, c->hd) * 2 * 8 * (c->hd + 2) + 3) & ~size_t(3); }
+size_t split_floats(const ks_ctx* ctx, const ks_q8_cache* c) { return (size_t)split_blocks(ctx, c->hd) * (8 + 2 * 8 * (c->hd + 2)); }
 
 }  // namespace
 
@@ -605,7 +586,7 @@ extern "C" {
 size_t ks_sdpa_paged_tmp_floats(const ks_ctx* ctx, const ks_q8_cache* c, const ks_page_tables* t, size_t n_q, size_t rows_most) {
   if (!ctx || !c || !t || !c->n_kv || !rows_most || n_q < c->n_kv) return 0;
   const size_t G = n_q / c->n_kv;
-  return split_floats(ctx, c, t) + (rows_most * G > KS_Q8_FEW ? ks_sdpa_q8_wide_floats(ctx, t->n_seqs, t->max_rows, c->n_kv, G, c->hd) : 0);
+  return split_floats(ctx, c) + (rows_most * G > KS_Q8_FEW ? ks_sdpa_q8_wide_floats(ctx, t->n_seqs, t->max_rows, c->n_kv, G, c->hd) : 0);
 }
 
 int ks_sdpa_paged_q8(ks_ctx* ctx, const ks_q8_cache* c, const ks_page_tables* t, size_t n_q, size_t rows_most, size_t ctx_most, size_t window, float scale, ks_dtype act,
@@ -641,8 +622,8 @@ int ks_sdpa_paged_q8(ks_ctx* ctx, const ks_q8_cache* c, const ks_page_tables* t,
   a.row_start = (const int*)t->plan->dptr + ks_plan_parts(t->n_seqs, t->max_rows, t->page).row_start;
   a.q = q->dptr;
   a.out = out->dptr;
-  a.first = (unsigned long long*)tmp->dptr;
-  a.part = (float*)tmp->dptr + first_floats(t);
+  a.merges = (int4*)tmp->dptr;
+  a.part = (float*)tmp->dptr + 8 * (size_t)split_blocks(ctx, c->hd);
   a.few = rows_most * G > KS_Q8_FEW ? KS_Q8_FEW : (unsigned)(rows_most * G);
   a.least = 1;
   a.bad = (unsigned*)ctx->ws + KS_WS_INDEX_WORD;
@@ -666,7 +647,7 @@ int ks_sdpa_paged_q8(ks_ctx* ctx, const ks_q8_cache* c, const ks_page_tables* t,
 #undef KS_AT_T
 #undef KS_AT
   if (rc || rows_most * G <= KS_Q8_FEW) return rc;
-  return ks_launch_sdpa_q8_wide(ctx, a, c->hd, act, c->dtype == KS_E4M3, (float*)tmp->dptr + split_floats(ctx, c, t), ctx_most);
+  return ks_launch_sdpa_q8_wide(ctx, a, c->hd, act, c->dtype == KS_E4M3, (float*)tmp->dptr + split_floats(ctx, c), ctx_most);
 }
 
 }  // extern "C"

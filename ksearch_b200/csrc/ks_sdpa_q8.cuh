@@ -10,7 +10,7 @@ struct ks_sdpa_q8_args {
   const void* q;
   void* out;
   float* part;               // records of split pieces
-  unsigned long long* first; // [n_seqs + 1]: units in front of each sequence
+  int4* merges;              // [blocks][2]: first block, records, which of the first block's, first (row, head); row, KV head, (row, head)s of the sequence
   unsigned* bad;
   unsigned n_seqs, max_blocks, n_pages, page_log, max_rows, rows_most, n_q, n_kv, G, window;
   unsigned few;              // sequences of up to so many rows (times G) take the split kernel

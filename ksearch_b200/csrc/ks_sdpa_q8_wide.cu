@@ -88,6 +88,25 @@ __device__ __forceinline__ uint64_t mul2(uint64_t x, uint64_t y) {
   return r;
 }
 
+// Products issued by the elected lane of a warp that runs the code as one: predicates instead of a branch keep addresses and descriptors in
+// uniform registers (behind a branch every product took 90 to 130 clocks to issue).  A descriptor's low word is its address in 16 bytes
+// and the stride between chunks, its high word is the same for all: 128 bytes between groups of 8 rows.
+constexpr uint32_t kDescHigh = (128u >> 4) | 1u << 14;
+__device__ __forceinline__ uint32_t desc_low(uint32_t smem_addr, unsigned chunk) { return (smem_addr >> 4 & 0x3FFFu) | (chunk >> 4 & 0x3FFFu) << 16; }
+__device__ __forceinline__ void issue_ss(unsigned leader, uint32_t d, uint32_t a_low, uint32_t b_low, uint32_t idesc, unsigned add) {
+  asm volatile("{\n\t.reg .pred p, q;\n\t.reg .b64 a, b;\n\tsetp.ne.u32 p, %4, 0;\n\tsetp.ne.u32 q, %5, 0;\n\tmov.b64 a, {%1, %6};\n\tmov.b64 b, {%2, %6};\n\t"
+               "@q tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, p;\n\t}" ::"r"(d), "r"(a_low), "r"(b_low), "r"(idesc), "r"(add), "r"(leader), "r"(kDescHigh)
+               : "memory");
+}
+__device__ __forceinline__ void issue_ts(unsigned leader, uint32_t d, uint32_t a_tmem, uint32_t b_low, uint32_t idesc, unsigned add) {
+  asm volatile("{\n\t.reg .pred p, q;\n\t.reg .b64 b;\n\tsetp.ne.u32 p, %4, 0;\n\tsetp.ne.u32 q, %5, 0;\n\tmov.b64 b, {%2, %6};\n\t"
+               "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %3, p;\n\t}" ::"r"(d), "r"(a_tmem), "r"(b_low), "r"(idesc), "r"(add), "r"(leader), "r"(kDescHigh)
+               : "memory");
+}
+__device__ __forceinline__ void commit_if(unsigned leader, uint32_t bar) {
+  asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.u32 q, %1, 0;\n\t@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar), "r"(leader) : "memory");
+}
+
 struct ks_wide_args {
   ks_sdpa_q8_args a;
   unsigned n_splits, share;  // splits of the launch, tiles that one of them takes
@@ -535,52 +554,50 @@ __global__ void __launch_bounds__(Wide<HD, T>::THREADS, 1) sdpa_q8_wide_kernel(c
       const unsigned leader = elect_one(), tiles = __reduce_max_sync(0xffffffffu, n_tiles), qts = __reduce_max_sync(0xffffffffu, q_tiles);
       constexpr uint32_t idesc_s = (1u << 4) | ((W::TILE >> 3) << 17) | ((kRows >> 4) << 24), idesc_o = (1u << 4) | ((HD >> 3) << 17) | ((kRows >> 4) << 24);
       auto wait = [&](unsigned b, unsigned parity) { return __all_sync(0xffffffffu, mb_wait(bar(b), parity & 1u, kWait)); };
+      const uint32_t base = __reduce_max_sync(0xffffffffu, sb);
+      const uint32_t d_q = desc_low(base + W::q, kRows * 16u), d_k = desc_low(base + W::k, W::TILE * 16u), d_v = desc_low(base + W::v, HD * 16u);
       auto scores = [&](unsigned i, unsigned t) {
-        if (leader) {
-          const uint64_t d_q = tc_desc(sb + W::q + t * W::q_bytes, kRows * 16u, 128u), d_k = tc_desc(sb + W::k + i % W::NK * W::kv_bytes, W::TILE * 16u, 128u);
-          const uint32_t to = t * W::t_tile + W::t_s;
+        const uint32_t k = d_k + i % W::NK * (W::kv_bytes / 16u), q = d_q + t * (W::q_bytes / 16u), to = t * W::t_tile + W::t_s;
 #pragma unroll
-          for (unsigned ks = 0; ks < HD / 16u; ks++) tc_mma_f16(to, d_q + (uint64_t)(2u * ks * kRows), d_k + (uint64_t)(2u * ks * W::TILE), idesc_s, ks ? 1u : 0u);
-          if constexpr (W::TERMS == 2)
+        for (unsigned ks = 0; ks < HD / 16u; ks++) issue_ss(leader, to, q + 2u * ks * kRows, k + 2u * ks * W::TILE, idesc_s, ks ? 1u : 0u);
+        if constexpr (W::TERMS == 2)
 #pragma unroll
-            for (unsigned ks = 0; ks < HD / 16u; ks++) tc_mma_f16_ta(to, W::t_q + 8u * ks, d_k + (uint64_t)(2u * ks * W::TILE), idesc_s, 1u);
-          tc_commit(bar(B_S_FULL + t));
-          if (t + 1u == qts) tc_commit(bar(B_K_FREE + i % W::NK));
-        }
-        __syncwarp();
+          for (unsigned ks = 0; ks < HD / 16u; ks++) issue_ts(leader, to, W::t_q + 8u * ks, k + 2u * ks * W::TILE, idesc_s, 1u);
+        commit_if(leader, base + 8u * (B_S_FULL + t));
+        if (t + 1u == qts) commit_if(leader, base + 8u * (B_K_FREE + i % W::NK));
       };
       bool ok = wait(B_K_FULL, 0u);
       if (ok) {
         tc_fence_after();
-        for (unsigned t = 0; t < qts; t++) scores(0, t);
+#pragma unroll
+        for (unsigned t = 0; t < W::QT; t++)
+          if (t < qts) scores(0, t);
       }
       for (unsigned i = 0; ok && i < tiles; i++) {
-        for (unsigned t = 0; ok && t < qts; t++) {
+#pragma unroll
+        for (unsigned t = 0; t < W::QT; t++) {
+          if (!ok || t >= qts) continue;
           if (i + 1u < tiles) {
             ok = (t || wait(B_K_FULL + (i + 1u) % W::NK, (i + 1u) / W::NK)) && wait(B_S_FREE + t, i);
-            if (!ok) break;
+            if (!ok) continue;
             tc_fence_after();
             scores(i + 1u, t);
           }
           ok = (t || wait(B_V_FULL + i % W::NV, i / W::NV)) && wait(B_P_FULL + t, i);
-          if (!ok) break;
+          if (!ok) continue;
           tc_fence_after();
-          if (leader) {
-            const uint64_t d_v = tc_desc(sb + W::v + i % W::NV * W::kv_bytes, HD * 16u, 128u);
-            const uint32_t to = t * W::t_tile + W::t_o, p = t * W::t_tile + W::t_p;
-            if constexpr (W::TERMS == 2) {
+          const uint32_t v = d_v + i % W::NV * (W::kv_bytes / 16u), to = t * W::t_tile + W::t_o, p = t * W::t_tile + W::t_p;
+          if constexpr (W::TERMS == 2) {
 #pragma unroll
-              for (unsigned ks = 0; ks < W::TILE / 16u; ks++) tc_mma_f16_ta(to, W::t_p + W::TILE / 2 + 8u * ks, d_v + (uint64_t)(2u * ks * HD), idesc_o, ks ? 1u : 0u);
+            for (unsigned ks = 0; ks < W::TILE / 16u; ks++) issue_ts(leader, to, p + W::TILE / 2 + 8u * ks, v + 2u * ks * HD, idesc_o, ks ? 1u : 0u);
 #pragma unroll
-              for (unsigned ks = 0; ks < W::TILE / 16u; ks++) tc_mma_f16_ta(to, p + 8u * ks, d_v + (uint64_t)(2u * ks * HD), idesc_o, 1u);
-            } else {
+            for (unsigned ks = 0; ks < W::TILE / 16u; ks++) issue_ts(leader, to, p + 8u * ks, v + 2u * ks * HD, idesc_o, 1u);
+          } else {
 #pragma unroll
-              for (unsigned ks = 0; ks < W::TILE / 16u; ks++) tc_mma_f16_ta(to, p + 8u * ks, d_v + (uint64_t)(2u * ks * HD), idesc_o, i || ks ? 1u : 0u);
-            }
-            tc_commit(bar(B_PV_DONE + t));
-            if (t + 1u == qts) tc_commit(bar(B_V_FREE + i % W::NV));
+            for (unsigned ks = 0; ks < W::TILE / 16u; ks++) issue_ts(leader, to, p + 8u * ks, v + 2u * ks * HD, idesc_o, ks ? 1u : i);
           }
-          __syncwarp();
+          commit_if(leader, base + 8u * (B_PV_DONE + t));
+          if (t + 1u == qts) commit_if(leader, base + 8u * (B_V_FREE + i % W::NV));
         }
       }
       if (leader) {  // every product issued must finish before shared and tensor memory go away (bounded)
@@ -658,28 +675,32 @@ __global__ void __launch_bounds__(Wide<HD, T>::THREADS, 1) sdpa_q8_wide_kernel(c
 
 // Records of blocks whose tiles were split, in their order; a warp a row.
 template <int HD, typename T>
-__global__ void __launch_bounds__(256) sdpa_q8_wide_merge_kernel(const __grid_constant__ ks_wide_args wa) {
+__global__ void __launch_bounds__(1024) sdpa_q8_wide_merge_kernel(const __grid_constant__ ks_wide_args wa) {
   using W = Wide<HD, T>;
   ks_pdl_entry();
   const ks_sdpa_q8_args& a = wa.a;
-  const unsigned lane = threadIdx.x & 31u, r = blockIdx.y * 8u + (threadIdx.x >> 5);
+  const unsigned lane = threadIdx.x & 31u, r = blockIdx.y * 32u + (threadIdx.x >> 5);
   const int4 meta = wa.meta[blockIdx.x];
   const unsigned m = (unsigned)meta.y + r, n_splits = (unsigned)meta.w >> 16, kvh = (unsigned)meta.w & 0xFFFFu;
   if (m >= (unsigned)meta.z || n_splits <= 1u) return;
   const float* rec = wa.part + (size_t)blockIdx.x * wa.n_splits * W::record;
   float top = kNone, l = 0.0f, v[HD / 32];
-  for (unsigned k = 0; k < n_splits; k++) top = fmaxf(top, rec[k * (size_t)W::record + r]);
+  // a split's (m, l) per lane
+  const float mk = lane < n_splits ? rec[lane * (size_t)W::record + r] : kNone, lk = lane < n_splits ? rec[lane * (size_t)W::record + W::ROWS + r] : 0.0f;
+  top = mk;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  const float ek = lk == 0.0f ? 0.0f : exp2_fast(mk - top);  // (nothing seen: it may have left no values)
+  l = q8_warp_sum(ek * lk);
 #pragma unroll
   for (int d = 0; d < HD / 32; d++) v[d] = 0.0f;
   for (unsigned k = 0; k < n_splits; k++) {
-    const float* x = rec + k * (size_t)W::record;
-    const float lk = x[W::ROWS + r];
-    if (lk == 0.0f) continue;  // nothing seen: it may have left no values
-    const float e = exp2_fast(x[r] - top);
-    l = fmaf(e, lk, l);
+    const float e = __shfl_sync(0xffffffffu, ek, k);
+    if (e == 0.0f) continue;
+    const float* x = rec + k * (size_t)W::record + 2 * W::ROWS + (size_t)r * HD + 2u * lane;
 #pragma unroll
     for (int d = 0; d < HD / 32; d += 2) {
-      const float2 y = *reinterpret_cast<const float2*>(x + 2 * W::ROWS + (size_t)r * HD + 2u * lane + 32 * d);
+      const float2 y = *reinterpret_cast<const float2*>(x + 32 * d);
       v[d] = fmaf(e, y.x, v[d]);
       v[d + 1] = fmaf(e, y.y, v[d + 1]);
     }
@@ -698,16 +719,24 @@ size_t wide_tiles(size_t n_seqs, size_t max_rows, size_t G, size_t rows) {
   const size_t pairs = max_rows * G, seqs = pairs / (KS_Q8_FEW + 1);
   return pairs / rows + (seqs < n_seqs ? seqs : n_seqs);
 }
-// Splits of the longest context: runs of `share` tiles, so that the launch has about two blocks an SM and none has much more to do than another, but four
-// tiles each at least.  blocks x splits is 2 blocks an SM + blocks at most.
-constexpr unsigned kMostSplits = 32;
-unsigned wide_splits(const ks_ctx* ctx, size_t blocks, size_t tiles, unsigned* share) {
-  const size_t want = 2 * (size_t)ctx->sm_count;
+// Splits of the longest context: the number for which the launch should end first.  Blocks see three quarters of the longest context on the
+// average (causal rows), and the last blocks leave a quarter of their time to nobody; setting up is worth `set_up` tiles, with a record to leave
+// (and to merge) `set_up_split`.  blocks x splits is 4 blocks an SM at most.  Measured: 2047 rows of 8 heads (f32, 128 blocks of up to 32 tiles) 102, 89, 96, 106 us in
+// 1 .. 4 splits; 4096 behind 4096 (f16, 256 blocks of up to 128) 329 and 365 in 1 and 2; eight ragged pieces through a window of 512 (f32, 40 blocks of
+// up to 9) 55, 47 and 62.
+constexpr unsigned kMostSplits = 32;  // a lane of the merge each
+unsigned wide_splits(const ks_ctx* ctx, size_t blocks, size_t tiles, size_t set_up, size_t set_up_split, unsigned* share) {
   if (tiles < 1) tiles = 1;
-  size_t s = (blocks * tiles + want - 1) / want;
-  if (s < 4) s = 4;
-  if (s * kMostSplits < tiles) s = (tiles + kMostSplits - 1) / kMostSplits;
-  if (blocks >= want || s > tiles) s = tiles;
+  const size_t sms = (size_t)ctx->sm_count;
+  size_t best = 1, least = ~size_t(0);
+  for (size_t n = 1; n <= kMostSplits && n <= tiles && (n == 1 || blocks * n <= 4 * sms); n++) {
+    const size_t extra = n == 1 ? set_up : set_up_split, one = (tiles + n - 1) / n + extra, even = 3 * blocks * (tiles + n * extra) / 4 / sms + one / 4, time = one > even ? one : even;
+    if (time < least) {
+      least = time;
+      best = n;
+    }
+  }
+  const size_t s = (tiles + best - 1) / best;
   *share = (unsigned)(s < 0x7FFFFFFFu ? s : 0x7FFFFFFFu);
   return (unsigned)((tiles + s - 1) / s);
 }
@@ -726,14 +755,14 @@ int launch_wide(ks_ctx* ctx, const ks_sdpa_q8_args& a, float* tmp, size_t ctx_mo
   ks_wide_args wa;
   wa.a = a;
   const size_t window = a.window ? (size_t)a.window + W::ROWS / a.G + 1 : ctx_most;
-  wa.n_splits = wide_splits(ctx, blocks, ((window < ctx_most ? window : ctx_most) + W::TILE - 1) / W::TILE, &wa.share);
+  wa.n_splits = wide_splits(ctx, blocks, ((window < ctx_most ? window : ctx_most) + W::TILE - 1) / W::TILE, W::TERMS == 1 ? 4 : 2, W::TERMS == 1 ? 12 : 5, &wa.share);
   wa.meta = (int4*)tmp;
   wa.part = tmp + 4 * blocks;
   wa.err = (unsigned*)ctx->ws + KS_WS_ERR_WORD;
   KS_LAUNCH(ctx, (sdpa_q8_wide_kernel<HD, T, FP8>), dim3((unsigned)blocks, wa.n_splits), W::THREADS, W::total, wa);
   int rc = ks_after_launch(ctx, "sdpa_paged_q8 wide");
   if (rc || wa.n_splits == 1) return rc;
-  KS_LAUNCH(ctx, (sdpa_q8_wide_merge_kernel<HD, T>), dim3((unsigned)blocks, W::ROWS / 8), 256, 0, wa);
+  KS_LAUNCH(ctx, (sdpa_q8_wide_merge_kernel<HD, T>), dim3((unsigned)blocks, W::ROWS / 32), 1024, 0, wa);
   return ks_after_launch(ctx, "sdpa_paged_q8 wide merge");
 }
 
@@ -742,8 +771,8 @@ int launch_wide(ks_ctx* ctx, const ks_sdpa_q8_args& a, float* tmp, size_t ctx_mo
 size_t ks_sdpa_q8_wide_floats(const ks_ctx* ctx, size_t n_seqs, size_t max_rows, size_t n_kv, size_t G, size_t hd) {
   size_t most = 0;
   for (size_t rows = kRows; rows <= (hd == 256 ? 1 : 2) * kRows; rows += kRows) {  // either activation type
-    const size_t blocks = wide_tiles(n_seqs, max_rows, G, rows) * n_kv, want = 2 * (size_t)ctx->sm_count;
-    const size_t n = 4 * blocks + (blocks < want ? (want + blocks) * rows * (hd + 2) : 0);
+    const size_t blocks = wide_tiles(n_seqs, max_rows, G, rows) * n_kv, most_records = 4 * (size_t)ctx->sm_count;
+    const size_t n = 4 * blocks + (2 * blocks <= most_records ? most_records * rows * (hd + 2) : 0);
     if (n > most) most = n;
   }
   return most;
