@@ -19,9 +19,9 @@ constexpr int kRows = 128;
 constexpr unsigned kWait = 1u << 20;
 constexpr int kWork = 8;  // softmax warps
 
-// Barriers: codes of a ring's stage there (copies) and converted; scales of a tile there; K, V converted and multiplied; scores there and read; probabilities there;
-// values done; all products done.
-enum { B_RAW_FULL = 0, B_RAW_FREE = 4, B_SCALE = 8, B_K_FULL = 16, B_K_FREE = 18, B_V_FULL = 20, B_V_FREE = 22, B_S_FULL = 24, B_S_FREE = 26, B_P_FULL = 28, B_PV_DONE = 30, B_DONE = 32, B_COUNT = 33 };
+// Barriers: codes of a ring's stage there (copies) and converted, K and V; scales of a tile there; K, V converted and multiplied; scores there and read;
+// probabilities there; values done; all products done.
+enum { B_RAW_FULL = 0, B_RAW_FREE = 8, B_SCALE = 16, B_K_FULL = 24, B_K_FREE = 26, B_V_FULL = 28, B_V_FREE = 30, B_S_FULL = 32, B_S_FREE = 34, B_P_FULL = 36, B_PV_DONE = 38, B_DONE = 40, B_COUNT = 41 };
 
 template <int HD_, typename T_>
 struct Wide {
@@ -30,15 +30,16 @@ struct Wide {
   static constexpr int TILE = HD == 256 || QT == 2 ? 64 : 128, GROUPS = TILE / 16, COLS = TILE / (QT == 2 ? 1 : 2);
   static constexpr int NK = 2, NV = HD == 256 ? 1 : 2;                            // buffers of converted K and V
   static constexpr int RING = HD == 256 || (HD == 128 && TERMS == 2) ? 2 : 4;     // tiles of codes
-  // The loader is RING tiles ahead of the converters at most, those of V NV ahead of the softmax warps: a tile's scales are read before their place comes again
-  static constexpr int SCALES = 2 * RING;
-  static_assert(SCALES >= RING + NV, "scales");
+  // The loader of K is RING tiles ahead of its converters at most, those NK ahead of the products and the softmax warps one behind those: a tile's scales are
+  // read before their place comes again
+  static constexpr int SCALES = RING == 2 ? 6 : 8;
+  static_assert(SCALES >= RING + NK + 2 && SCALES <= 8, "scales");
   static constexpr int CONV_K = TERMS == 1 ? 4 : 2, CONV_V = CONV_K, WARPS = kWork + CONV_K + CONV_V + 4, THREADS = WARPS * 32;
   static constexpr int R_WORK = TERMS == 1 ? 128 : 208, R_CONV = TERMS == 1 ? 80 : 64, R_REST = TERMS == 1 ? 64 : 32;
   static_assert(kWork * 32 * R_WORK + (CONV_K + CONV_V) * 32 * R_CONV + 128 * R_REST <= THREADS * (65536 / THREADS / 8 * 8), "registers: the shares fit the launch");
   // shared memory: barriers, the tensor-memory address and the failure flag; per row: scale, maxima of its two threads; per 16 positions: the score's
   // factor, what is added to it, the probability's factor, the sum's
-  static constexpr unsigned slot = 272, row = 288, best = row + (TERMS == 2 ? kRows * 4 : 0), scale = best + 2 * kRows * 4, q = (scale + SCALES * GROUPS * 16 + 127) / 128 * 128;
+  static constexpr unsigned slot = 336, row = 352, best = row + (TERMS == 2 ? kRows * 4 : 0), scale = best + 2 * kRows * 4, q = (scale + SCALES * GROUPS * 16 + 127) / 128 * 128;
   static_assert(8 * B_COUNT <= slot && slot + 16 <= row, "the words fit in front of the operands");
   static constexpr unsigned q_bytes = kRows * HD * 2, kv_bytes = TILE * HD * 2, k = q + QT * q_bytes, v = k + NK * kv_bytes, raw = v + NV * kv_bytes, raw_bytes = 2 * TILE * HD,
                             total = raw + RING * raw_bytes;
@@ -210,7 +211,9 @@ __global__ void __launch_bounds__(Wide<HD, T>::THREADS, 1) sdpa_q8_wide_kernel(c
   if (tid == 0) {
     for (unsigned i = 0; i < W::RING; i++) {
       mb_init(bar(B_RAW_FULL + i), 1);
-      mb_init(bar(B_RAW_FREE + i), W::CONV_K + W::CONV_V);
+      mb_init(bar(B_RAW_FULL + 4u + i), 1);
+      mb_init(bar(B_RAW_FREE + i), W::CONV_K);
+      mb_init(bar(B_RAW_FREE + 4u + i), W::CONV_V);
     }
     for (unsigned i = 0; i < W::SCALES; i++) mb_init(bar(B_SCALE + i), 1);
     for (unsigned i = 0; i < 2u; i++) {
@@ -496,11 +499,11 @@ __global__ void __launch_bounds__(Wide<HD, T>::THREADS, 1) sdpa_q8_wide_kernel(c
     // ---- codes -> f16 core matrices, K and V by warps of their own
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(W::R_CONV));
     const bool keys = warp < kWork + W::CONV_K;
-    const unsigned cw = warp - kWork - (keys ? 0u : W::CONV_K);
+    const unsigned cw = warp - kWork - (keys ? 0u : W::CONV_K), kv4 = keys ? 0u : 4u;
     unsigned done = 0;
     for (unsigned i = 0; i < n_tiles; i++) {
       const unsigned char* raw = smem + W::raw + i % W::RING * W::raw_bytes;
-      if (!__all_sync(0xffffffffu, mb_wait(bar(B_RAW_FULL + i % W::RING), i / W::RING & 1u, kWait))) break;
+      if (!__all_sync(0xffffffffu, mb_wait(bar(B_RAW_FULL + kv4 + i % W::RING), i / W::RING & 1u, kWait))) break;
       if (keys) {
         const unsigned b = i % W::NK;
         if (i >= W::NK && !__all_sync(0xffffffffu, mb_wait(bar(B_K_FREE + b), (i / W::NK - 1u) & 1u, kWait))) break;
@@ -542,7 +545,7 @@ __global__ void __launch_bounds__(Wide<HD, T>::THREADS, 1) sdpa_q8_wide_kernel(c
       __syncwarp();
       if (lane == 0) {
         arrive1(bar(keys ? B_K_FULL + i % W::NK : B_V_FULL + i % W::NV));
-        arrive1(bar(B_RAW_FREE + i % W::RING));
+        arrive1(bar(B_RAW_FREE + kv4 + i % W::RING));
       }
       done++;
     }
@@ -606,8 +609,11 @@ __global__ void __launch_bounds__(Wide<HD, T>::THREADS, 1) sdpa_q8_wide_kernel(c
       }
       __syncwarp();
       mb_wait(bar(B_DONE), 0u, kWait);
-    } else if (warp == MMA_WARP + 1) {
-      // ---- codes: the runs of a tile that lie in one page, a lane each
+    } else if (warp <= MMA_WARP + 2) {
+      // ---- codes, K and the scales by one warp, V by another: the runs of a tile that lie in one page, a lane each
+      const bool keys = warp == MMA_WARP + 1;
+      const unsigned kv4 = keys ? 0u : 4u;
+      const uint8_t* codes = keys ? a.kc : a.vc;
       const unsigned page = 1u << a.page_log, run = min(page, (unsigned)W::TILE), runs = W::TILE / run;
       auto page_of = [&](unsigned i) -> int {  // as the table has it, -1 where no row of the block sees the run
         const int p = t_begin + (int)(i * W::TILE + lane * run);
@@ -616,13 +622,13 @@ __global__ void __launch_bounds__(Wide<HD, T>::THREADS, 1) sdpa_q8_wide_kernel(c
       auto checked = [&](unsigned i, int id) -> int {
         if ((unsigned)id < a.n_pages) return id;
         const int p = t_begin + (int)(i * W::TILE + lane * run);
-        if (i < n_tiles && lane < runs && p < seen_to && p + (int)run > seen_from) atomicOr(a.bad, KS_BAD_PAGE);
+        if (keys && i < n_tiles && lane < runs && p < seen_to && p + (int)run > seen_from) atomicOr(a.bad, KS_BAD_PAGE);
         return -1;
       };
       auto scales_of = [&](int id) -> float2 {  // of 16 positions
         const int gid = __shfl_sync(0xffffffffu, id, lane * 16u / run);
         const size_t at = (size_t)max(gid, 0) * a.n_kv + kvh;
-        return lane < W::GROUPS && gid >= 0 ? make_float2(a.ks[at], a.vs[at]) : make_float2(0.0f, 0.0f);
+        return keys && lane < W::GROUPS && gid >= 0 ? make_float2(a.ks[at], a.vs[at]) : make_float2(0.0f, 0.0f);
       };
       // a tile's pages are read two tiles ahead, its scales one
       unsigned sent = 0;
@@ -632,17 +638,15 @@ __global__ void __launch_bounds__(Wide<HD, T>::THREADS, 1) sdpa_q8_wide_kernel(c
         const unsigned st = i % W::RING;
         const int p = t_begin + (int)(i * W::TILE + lane * run);
         const unsigned there = __popc(__ballot_sync(0xffffffffu, id >= 0));
-        if (i >= W::RING && !__all_sync(0xffffffffu, mb_wait(bar(B_RAW_FREE + st), (i / W::RING - 1u) & 1u, kWait))) break;
-        if (lane == 0) mb_expect(bar(B_RAW_FULL + st), there * 2u * run * HD);
+        if (i >= W::RING && !__all_sync(0xffffffffu, mb_wait(bar(B_RAW_FREE + kv4 + st), (i / W::RING - 1u) & 1u, kWait))) break;
+        if (lane == 0) mb_expect(bar(B_RAW_FULL + kv4 + st), there * run * HD);
         __syncwarp();
         if (id >= 0) {
           const size_t from = ((((size_t)id * a.n_kv + kvh) << a.page_log) + ((unsigned)p & (page - 1u))) * HD;
-          const uint32_t to = sb + W::raw + st * W::raw_bytes + lane * run * HD;
-          bulk_in(to, a.kc + from, run * HD, bar(B_RAW_FULL + st));
-          bulk_in(to + W::TILE * HD, a.vc + from, run * HD, bar(B_RAW_FULL + st));
+          bulk_in(sb + W::raw + st * W::raw_bytes + (keys ? 0u : W::TILE * HD) + lane * run * HD, codes + from, run * HD, bar(B_RAW_FULL + kv4 + st));
         }
         sent++;
-        if (lane < W::GROUPS) {
+        if (keys && lane < W::GROUPS) {
           const float f = fmaxf(q8_scale(sc.x) * fabsf(a.scale) * 1.44269504088896340736f, 1.0e-37f);
           float4 w;
           if constexpr (W::TERMS == 1) {
@@ -656,14 +660,14 @@ __global__ void __launch_bounds__(Wide<HD, T>::THREADS, 1) sdpa_q8_wide_kernel(c
           reinterpret_cast<float4*>(smem + W::scale)[i % W::SCALES * W::GROUPS + lane] = w;
         }
         __syncwarp();
-        if (lane == 0) arrive1(bar(B_SCALE + i % W::SCALES));
+        if (keys && lane == 0) arrive1(bar(B_SCALE + i % W::SCALES));
         id = checked(i + 1u, next);
         next = page_of(i + 2u);
         sc = scales_of(id);
       }
       if (sent < n_tiles && lane == 0) *fail = 1;
       // the copies must have landed before this block's shared memory goes away (bounded)
-      for (unsigned i = sent > W::RING ? sent - W::RING : 0u; i < sent; i++) mb_wait(bar(B_RAW_FULL + i % W::RING), i / W::RING & 1u, kWait);
+      for (unsigned i = sent > W::RING ? sent - W::RING : 0u; i < sent; i++) mb_wait(bar(B_RAW_FULL + kv4 + i % W::RING), i / W::RING & 1u, kWait);
     }
   }
   tc_fence_before();
