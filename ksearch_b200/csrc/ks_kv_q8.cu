@@ -13,7 +13,8 @@
 
 namespace {
 
-constexpr int kRowsPerWarp = 8;  // rows of a page a warp keeps in registers between their maximum and their codes
+constexpr int kRowsPerWarp = 4;  // rows of a page a warp keeps in registers between their maximum and their codes
+constexpr int kHeadsPerWarp = 2;  // (row, query head) pairs of a warp
 
 struct AppendArgs {
   uint8_t *kc, *vc;      // codes [n_pages, n_kv, page, hd]
@@ -88,76 +89,79 @@ __device__ __forceinline__ void store_codes(uint8_t* p, const float (&x)[V], flo
   }
 }
 
-// One head of one row behind its norm and RoPE (w == nullptr: the norm alone, as V has it).  A lane holds dims V lane.. of both halves, so
-// RoPE partners sit in one lane.
+// What a head of a row is normed and turned by.  A lane holds dims V lane.. of both halves, so RoPE partners sit in one lane.
+template <int V>
+struct Turn {
+  float w0[V], w1[V], c[V], s[V];
+};
 template <int HD, int V, typename T>
-__device__ __forceinline__ void norm_rope(float (&x)[2][V], float eps, const T* w, const float* cs) {
+__device__ __forceinline__ void load_turn(Turn<V>& t, const T* w, const float* cs) {
+  load_act<V, T>(w, t.w0);
+  load_act<V, T>(w + HD / 2, t.w1);
+  load_act<V, float>(cs, t.c);
+  load_act<V, float>(cs + HD / 2, t.s);
+}
+template <int HD, int V>
+__device__ __forceinline__ float norm_of(const float (&x)[2][V], float eps) {
   float ss = 0.0f;
 #pragma unroll
   for (int e = 0; e < V; e++) ss = fmaf(x[0][e], x[0][e], fmaf(x[1][e], x[1][e], ss));
   ss = q8_warp_sum(ss);
-  const float inv = 1.0f / sqrtf(ss / (float)HD + eps);
-  if (w == nullptr) {
-#pragma unroll
-    for (int e = 0; e < V; e++) {
-      x[0][e] *= inv;
-      x[1][e] *= inv;
-    }
-    return;
-  }
-  float w0[V], w1[V], c[V], s[V];
-  load_act<V, T>(w, w0);
-  load_act<V, T>(w + HD / 2, w1);
-  load_act<V, float>(cs, c);
-  load_act<V, float>(cs + HD / 2, s);
+  return 1.0f / sqrtf(ss / (float)HD + eps);
+}
+template <int V>
+__device__ __forceinline__ void norm_rope(float (&x)[2][V], float inv, const Turn<V>& t) {
 #pragma unroll
   for (int e = 0; e < V; e++) {
-    const float a = __fmul_rn(__fmul_rn(x[0][e], inv), w0[e]), b = __fmul_rn(__fmul_rn(x[1][e], inv), w1[e]);
-    x[0][e] = __fsub_rn(__fmul_rn(a, c[e]), __fmul_rn(b, s[e]));
-    x[1][e] = __fadd_rn(__fmul_rn(a, s[e]), __fmul_rn(b, c[e]));
+    const float a = __fmul_rn(__fmul_rn(x[0][e], inv), t.w0[e]), b = __fmul_rn(__fmul_rn(x[1][e], inv), t.w1[e]);
+    x[0][e] = __fsub_rn(__fmul_rn(a, t.c[e]), __fmul_rn(b, t.s[e]));
+    x[1][e] = __fadd_rn(__fmul_rn(a, t.s[e]), __fmul_rn(b, t.c[e]));
   }
 }
 
-// Grid: (touched pages x n_kv x 2) blocks of page / 8 warps, K and V of a head next to each other; NORM: behind them the blocks of the
-// query heads, four (row, head) pairs a warp.
+// Grid: (touched pages x n_kv x 2) blocks of page / kRowsPerWarp warps, K and V of a head next to each other; NORM: in front of them the blocks of the
+// query heads.
 template <int HD, typename T, bool FP8, bool NORM>
-__global__ void __launch_bounds__(512) append_q8_kernel(const AppendArgs a) {
+__global__ void __launch_bounds__(1024) append_q8_kernel(const AppendArgs a, unsigned q_blocks) {
   constexpr int V = HD / 64;
-  __shared__ float red[16];
+  __shared__ float red[32];
   ks_pdl_entry();
   const unsigned lane = threadIdx.x & 31u, warp = threadIdx.x >> 5, nwarp = blockDim.x >> 5;
   const unsigned page = 1u << a.page_log, per_job = 2u * a.n_kv;
-  if (NORM && blockIdx.x >= a.n_jobs * per_job) {
-    const unsigned rows = min((unsigned)max(a.plan[1], 0), a.max_rows), items = rows * a.n_q;
-    const unsigned it0 = ((blockIdx.x - a.n_jobs * per_job) * nwarp + warp) * 4u;
-    float x[4][2][V];
-    int pos[4];
+  if (NORM && blockIdx.x < q_blocks) {
+    const unsigned it0 = (blockIdx.x * nwarp + warp) * kHeadsPerWarp, most = a.max_rows * a.n_q;
+    float x[kHeadsPerWarp][2][V];
+    int pos[kHeadsPerWarp];
+    const unsigned items = min((unsigned)max(a.plan[1], 0), a.max_rows) * a.n_q;
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-      const unsigned it = it0 + i;
-      if (it >= items) continue;
+    for (int i = 0; i < kHeadsPerWarp; i++) {  // (rows behind the plan's last are in the buffers too: nothing waits for how many there are)
+      const unsigned it = min(it0 + i, most - 1u);
       const T* src = (const T*)a.q + (size_t)it * HD + lane * V;
       load_act<V, T>(src, x[i][0]);
       load_act<V, T>(src + HD / 2, x[i][1]);
       pos[i] = a.plan[a.at.row_pos + it / a.n_q];
     }
+    Turn<V> t[kHeadsPerWarp];
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
+    for (int i = 0; i < kHeadsPerWarp; i++) load_turn<HD, V, T>(t[i], (const T*)a.qw + lane * V, a.rope + (size_t)min((unsigned)max(pos[i], 0), a.rope_rows - 1u) * HD + lane * V);
+#pragma unroll
+    for (int i = 0; i < kHeadsPerWarp; i++) {
       const unsigned it = it0 + i;
+      const float inv = norm_of<HD, V>(x[i], a.eps);
       if (it >= items) continue;
       if ((unsigned)pos[i] >= a.rope_rows) {
         if (lane == 0) atomicOr(a.bad, KS_BAD_POSITION);
         continue;
       }
-      norm_rope<HD, V, T>(x[i], a.eps, (const T*)a.qw + lane * V, a.rope + (size_t)pos[i] * HD + lane * V);
+      norm_rope<V>(x[i], inv, t[i]);
       T* dst = (T*)a.q_out + (size_t)it * HD + lane * V;
       store_act<V, T>(dst, x[i][0]);
       store_act<V, T>(dst + HD / 2, x[i][1]);
     }
     return;
   }
-  const unsigned j = blockIdx.x / per_job, head = blockIdx.x % per_job >> 1;
-  const bool vals = blockIdx.x & 1u;
+  const unsigned index = blockIdx.x - (NORM ? q_blocks : 0u), j = index / per_job, head = index % per_job >> 1;
+  const bool vals = index & 1u;
   const int4 job = reinterpret_cast<const int4*>(a.plan + a.at.jobs)[j];
   if (job.x < 0) return;
   const unsigned row0 = (unsigned)job.x, rows = (unsigned)job.y, slot = (unsigned)job.z, off = slot & (page - 1u);
@@ -185,7 +189,17 @@ __global__ void __launch_bounds__(512) append_q8_kernel(const AppendArgs a) {
   for (int i = 0; i < kRowsPerWarp; i++) {
     const unsigned r = warp + (unsigned)i * nwarp;
     if (r >= rows) continue;
-    if constexpr (NORM) norm_rope<HD, V, T>(x[i], a.eps, vals ? (const T*)nullptr : (const T*)a.kw + lane * V, a.rope + (size_t)((unsigned)job.w + r) * HD + lane * V);
+    if constexpr (NORM) {
+      const float inv = norm_of<HD, V>(x[i], a.eps);
+      if (vals) {
+#pragma unroll
+        for (int e = 0; e < 2 * V; e++) x[i][e / V][e % V] *= inv;
+      } else {
+        Turn<V> t;
+        load_turn<HD, V, T>(t, (const T*)a.kw + lane * V, a.rope + (size_t)((unsigned)job.w + r) * HD + lane * V);
+        norm_rope<V>(x[i], inv, t);
+      }
+    }
 #pragma unroll
     for (int e = 0; e < 2 * V; e++) {
       float& y = x[i][e / V][e % V];
@@ -221,7 +235,8 @@ __global__ void __launch_bounds__(512) append_q8_kernel(const AppendArgs a) {
   if (threadIdx.x == 0 && s != held) *scale_at = s;
 }
 
-// Eight codes a thread; K and V in blockIdx.y.
+// Eight codes at a time, kReadsPerThread such reads on their way; K and V in blockIdx.y.
+constexpr int kReadsPerThread = 4;
 template <typename T, bool FP8>
 __global__ void __launch_bounds__(256) read_q8_kernel(const uint8_t* kc, const uint8_t* vc, const float* ks, const float* vs, unsigned hd_log, unsigned n_kv, unsigned page_log,
                                                       unsigned n_slots, unsigned n_rows, const int* slots, T* k, T* v, unsigned* bad) {
@@ -231,21 +246,52 @@ __global__ void __launch_bounds__(256) read_q8_kernel(const uint8_t* kc, const u
   T* out = blockIdx.y ? v : k;
   const unsigned chunk_log = hd_log - 3u, per_row = n_kv << chunk_log;
   const size_t n = (size_t)n_rows * per_row, step = (size_t)gridDim.x * blockDim.x;
-  for (size_t i = (size_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += step) {
-    const unsigned row = (unsigned)(i / per_row), rest = (unsigned)(i - (size_t)row * per_row), head = rest >> chunk_log, c = rest & ((1u << chunk_log) - 1u);
-    const int slot = slots[row];
-    if (slot == -1) continue;
-    if ((unsigned)slot >= n_slots) {
-      atomicOr(bad, KS_BAD_SLOT);
-      continue;
+  for (size_t i0 = (size_t)blockIdx.x * blockDim.x + threadIdx.x; i0 < n; i0 += step * kReadsPerThread) {
+    int slot[kReadsPerThread];
+    unsigned rest[kReadsPerThread];
+#pragma unroll
+    for (int u = 0; u < kReadsPerThread; u++) {
+      const size_t i = i0 + u * step;
+      const size_t row = i / per_row;
+      rest[u] = (unsigned)(i - row * per_row);
+      slot[u] = i < n ? slots[row] : -1;
     }
-    const size_t block = (size_t)((unsigned)slot >> page_log) * n_kv + head;
-    const float s = q8_scale(scales[block]);
-    const uint2 w = *reinterpret_cast<const uint2*>(codes + ((((block << page_log) + ((unsigned)slot & ((1u << page_log) - 1u))) << hd_log) + 8u * c));
-    const float2 f0 = q8_decode2f<FP8>(w.x), f1 = q8_decode2f<FP8>(w.x >> 16), f2 = q8_decode2f<FP8>(w.y), f3 = q8_decode2f<FP8>(w.y >> 16);
-    const float lo[4] = {f0.x * s, f0.y * s, f1.x * s, f1.y * s}, hi[4] = {f2.x * s, f2.y * s, f3.x * s, f3.y * s};
-    store_act<4, T>(out + i * 8, lo);
-    store_act<4, T>(out + i * 8 + 4, hi);
+    uint2 w[kReadsPerThread];
+    float s[kReadsPerThread];
+#pragma unroll
+    for (int u = 0; u < kReadsPerThread; u++) {
+      if (slot[u] != -1 && (unsigned)slot[u] >= n_slots) {
+        atomicOr(bad, KS_BAD_SLOT);
+        slot[u] = -1;
+      }
+      const unsigned at = (unsigned)max(slot[u], 0), head = rest[u] >> chunk_log, c = rest[u] & ((1u << chunk_log) - 1u);
+      const size_t block = (size_t)(at >> page_log) * n_kv + head;
+      w[u] = make_uint2(0u, 0u);
+      s[u] = 0.0f;
+      if (slot[u] >= 0) {
+        s[u] = scales[block];
+        w[u] = *reinterpret_cast<const uint2*>(codes + ((((block << page_log) + (at & ((1u << page_log) - 1u))) << hd_log) + 8u * c));
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < kReadsPerThread; u++) {
+      if (slot[u] < 0) continue;
+      const float f = q8_scale(s[u]);
+      const float2 f0 = q8_decode2f<FP8>(w[u].x), f1 = q8_decode2f<FP8>(w[u].x >> 16), f2 = q8_decode2f<FP8>(w[u].y), f3 = q8_decode2f<FP8>(w[u].y >> 16);
+      T* to = out + (i0 + u * step) * 8;
+      if constexpr (sizeof(T) == 4) {
+        const float lo[4] = {f0.x * f, f0.y * f, f1.x * f, f1.y * f}, hi[4] = {f2.x * f, f2.y * f, f3.x * f, f3.y * f};
+        store_act<4, T>(to, lo);
+        store_act<4, T>(to + 4, hi);
+      } else {
+        uint4 y;
+        y.x = q8_u32(__floats2half2_rn(f0.x * f, f0.y * f));
+        y.y = q8_u32(__floats2half2_rn(f1.x * f, f1.y * f));
+        y.z = q8_u32(__floats2half2_rn(f2.x * f, f2.y * f));
+        y.w = q8_u32(__floats2half2_rn(f3.x * f, f3.y * f));
+        *reinterpret_cast<uint4*>(to) = y;
+      }
+    }
   }
 }
 
@@ -269,12 +315,11 @@ AppendArgs append_args(ks_ctx* ctx, const ks_q8_cache* c, const ks_page_tables* 
 template <bool NORM>
 int launch_append(ks_ctx* ctx, const ks_q8_cache* c, ks_dtype act, const AppendArgs& a, const char* who) {
   const unsigned warps = (unsigned)c->page / kRowsPerWarp;
-  size_t blocks = (size_t)a.n_jobs * 2 * a.n_kv;
-  if (NORM) blocks += ((size_t)a.max_rows * a.n_q + 4 * warps - 1) / (4 * warps);
+  const size_t q_blocks = NORM ? ((size_t)a.max_rows * a.n_q + kHeadsPerWarp * warps - 1) / (kHeadsPerWarp * warps) : 0, blocks = q_blocks + (size_t)a.n_jobs * 2 * a.n_kv;
   KS_REQUIRE(ctx, blocks < (1u << 31), "%s: too many rows and heads for one launch", who);
   KS_REQUIRE_DEVICE(ctx, who);
   ks_on_device on(ctx);
-#define KS_AP(HD_, T_, F_) KS_LAUNCH(ctx, (append_q8_kernel<HD_, T_, F_, NORM>), (unsigned)blocks, warps * 32, 0, a)
+#define KS_AP(HD_, T_, F_) KS_LAUNCH(ctx, (append_q8_kernel<HD_, T_, F_, NORM>), (unsigned)blocks, warps * 32, 0, a, (unsigned)q_blocks)
 #define KS_AP_T(HD_, F_) do { if (act == KS_F32) KS_AP(HD_, float, F_); else KS_AP(HD_, __half, F_); } while (0)
 #define KS_AP_F(HD_) do { if (c->dtype == KS_E4M3) KS_AP_T(HD_, true); else KS_AP_T(HD_, false); } while (0)
   if (c->hd == 256) KS_AP_F(256);
@@ -368,7 +413,7 @@ int ks_kv_read_q8(ks_ctx* ctx, const ks_q8_cache* c, size_t n_rows, const ks_buf
   KS_REQUIRE_DEVICE(ctx, "kv_read_q8");
   ks_on_device on(ctx);
   const size_t items = n_rows * c->n_kv * c->hd / 8;
-  const size_t most = (size_t)ctx->sm_count * 8, blocks = (items + 255) / 256;
+  const size_t most = (size_t)ctx->sm_count * 8, blocks = (items + 256 * kReadsPerThread - 1) / (256 * kReadsPerThread);
   const dim3 grid((unsigned)(blocks < most ? blocks : most), 2);
   const int* at = (const int*)slots->dptr + slot_off;
   const unsigned hd_log = (unsigned)__builtin_ctzll(c->hd), page_log = (unsigned)__builtin_ctzll(c->page);

@@ -166,18 +166,20 @@ __global__ void __launch_bounds__(Split<HD, T>::THREADS, Split<HD, T>::PER_SM) s
         if (lane < 2u) copy4(scales_at + ((st * S::NP + b) * 2u + lane) * 4u, (lane ? a.vs : a.ks) + block, page);
       }
     };
-    int id[S::NP];
-    auto pages = [&](unsigned i) {
+    auto pages = [&](unsigned i, int (&id)[S::NP]) {
 #pragma unroll
       for (int b = 0; b < S::NP; b++) id[b] = i < n ? page_of(p_first + (int)i * S::TILE + 16 * b) : -1;
     };
+    int ids[S::STAGES][S::NP], id[S::NP];
+#pragma unroll
+    for (int i = 0; i < S::STAGES; i++) pages((unsigned)i, ids[i]);
 #pragma unroll
     for (int i = 0; i < S::STAGES - 1; i++) {
-      pages((unsigned)i);
-      if ((unsigned)i < n) send(p_first + i * S::TILE, id, (unsigned)i);
+      if ((unsigned)i < n) send(p_first + i * S::TILE, ids[i], (unsigned)i);
       copies_sent();
     }
-    pages(S::STAGES - 1);
+#pragma unroll
+    for (int b = 0; b < S::NP; b++) id[b] = ids[S::STAGES - 1][b];
 
     // ---- q: row g, dims 16 c .. 16 c + 15 of every 64: what the codes of a 16-byte read meet.  f32 rows are brought to 2^14 by a power of
     // two and split into two f16 terms
@@ -256,7 +258,7 @@ __global__ void __launch_bounds__(Split<HD, T>::THREADS, Split<HD, T>::PER_SM) s
         const unsigned to = st == 0 ? S::STAGES - 1 : st - 1u;
         if (i + S::STAGES - 1 < n) send(p0 + (S::STAGES - 1) * S::TILE, id, to);
         copies_sent();
-        pages(i + S::STAGES);
+        pages(i + S::STAGES, id);
       }
       const unsigned char* at_k = ring + st * S::stage_bytes;
       const unsigned char* at_v = at_k + S::SUB * HD;
@@ -624,7 +626,9 @@ int ks_sdpa_paged_q8(ks_ctx* ctx, const ks_q8_cache* c, const ks_page_tables* t,
   a.out = out->dptr;
   a.merges = (int4*)tmp->dptr;
   a.part = (float*)tmp->dptr + 8 * (size_t)split_blocks(ctx, c->hd);
-  a.few = rows_most * G > KS_Q8_FEW ? KS_Q8_FEW : (unsigned)(rows_most * G);
+  // (a lone sequence that may have many rows needs one kernel only, whatever it has)
+  const bool wide = rows_most * G > KS_Q8_FEW, split = !wide || t->n_seqs > 1;
+  a.few = !split ? 0u : wide ? KS_Q8_FEW : (unsigned)(rows_most * G);
   a.least = 1;
   a.bad = (unsigned*)ctx->ws + KS_WS_INDEX_WORD;
   a.n_seqs = (unsigned)t->n_seqs;
@@ -642,11 +646,11 @@ int ks_sdpa_paged_q8(ks_ctx* ctx, const ks_q8_cache* c, const ks_page_tables* t,
 #define KS_AT(HD_, T_, F_) launch_split<HD_, T_, F_>(ctx, a, blocks)
 #define KS_AT_T(HD_, F_) (act == KS_F32 ? KS_AT(HD_, float, F_) : KS_AT(HD_, __half, F_))
 #define KS_AT_F(HD_) (c->dtype == KS_E4M3 ? KS_AT_T(HD_, true) : KS_AT_T(HD_, false))
-  rc = c->hd == 256 ? KS_AT_F(256) : c->hd == 128 ? KS_AT_F(128) : KS_AT_F(64);
+  if (split) rc = c->hd == 256 ? KS_AT_F(256) : c->hd == 128 ? KS_AT_F(128) : KS_AT_F(64);
 #undef KS_AT_F
 #undef KS_AT_T
 #undef KS_AT
-  if (rc || rows_most * G <= KS_Q8_FEW) return rc;
+  if (rc || !wide) return rc;
   return ks_launch_sdpa_q8_wide(ctx, a, c->hd, act, c->dtype == KS_E4M3, (float*)tmp->dptr + split_floats(ctx, c), ctx_most);
 }
 

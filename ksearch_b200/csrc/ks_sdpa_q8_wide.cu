@@ -509,10 +509,12 @@ __global__ void __launch_bounds__(Wide<HD, T>::THREADS, 1) sdpa_q8_wide_kernel(c
         if (i >= W::NK && !__all_sync(0xffffffffu, mb_wait(bar(B_K_FREE + b), (i / W::NK - 1u) & 1u, kWait))) break;
         unsigned char* to = smem + W::k + b * W::kv_bytes;
         // 32 rows and one 16-byte chunk of each, a different one for neighbouring lanes: neither the read nor the writes meet a bank twice
-        constexpr unsigned CH = HD / 16, STEPS = W::TILE / 32 * CH, RING = HD == 64 ? 4 : 8;
-#pragma unroll 2
-        for (unsigned n = cw; n < STEPS; n += W::CONV_K) {
-          const unsigned r = n / CH * 32u + lane, k = n % CH, ch = k / RING * RING + ((HD == 64 ? lane >> 1 : lane) + k) % RING;
+        constexpr unsigned CH = HD / 16, STEPS = W::TILE / 32 * CH, PER = STEPS / W::CONV_K, RUN = HD == 64 ? 4 : 8;
+        static_assert(STEPS % W::CONV_K == 0 && (PER % CH == 0 || CH % PER == 0), "steps of a warp");
+        const unsigned n0 = cw * PER, r0 = n0 / CH * 32u + lane, k0 = n0 % CH, turn = HD == 64 ? lane >> 1 : lane;
+#pragma unroll 4
+        for (unsigned j = 0; j < PER; j++) {
+          const unsigned r = r0 + j / CH * 32u, k = k0 + j % CH, ch = k / RUN * RUN + (turn + k) % RUN;
           const uint4 w = *reinterpret_cast<const uint4*>(raw + r * HD + ch * 16u);
           uint4 x, y;
           widen4<FP8>(w.x, x.x, x.y);
@@ -528,10 +530,11 @@ __global__ void __launch_bounds__(Wide<HD, T>::THREADS, 1) sdpa_q8_wide_kernel(c
         raw += W::TILE * HD;
         unsigned char* to = smem + W::v + b * W::kv_bytes;
         // eight positions and four dims a lane; dim 4 w + j becomes column j HD / 4 + w of O, so that neighbouring lanes write neighbouring chunks
-        constexpr unsigned WORDS = HD / 4, PG = HD == 64 ? 2 : 1, PER = WORDS >= 32 ? WORDS / 32 : 1, STEPS = W::TILE / 8 * WORDS / 32;
-#pragma unroll 1
-        for (unsigned n = cw; n < STEPS; n += W::CONV_V) {
-          const unsigned w = PG == 2 ? lane & 15u : n % PER * 32u + lane, pg = PG == 2 ? 2u * n + (lane >> 4) : n / PER;
+        constexpr unsigned WORDS = HD / 4, PARTS = WORDS >= 32 ? WORDS / 32 : 1, PG = WORDS >= 32 ? 1 : 2, STEPS = W::TILE / 8 * WORDS / 32, PER = STEPS / W::CONV_V;
+        static_assert(STEPS % W::CONV_V == 0, "steps of a warp");
+#pragma unroll 2
+        for (unsigned j = 0; j < PER; j++) {
+          const unsigned n = cw * PER + j, w = PG == 2 ? lane & 15u : n % PARTS * 32u + lane, pg = PG == 2 ? 2u * n + (lane >> 4) : n / PARTS;
           uint32_t v[8], p[4][4];
 #pragma unroll
           for (int e = 0; e < 8; e++) v[e] = *reinterpret_cast<const uint32_t*>(raw + (8u * pg + e) * HD + 4u * w);
