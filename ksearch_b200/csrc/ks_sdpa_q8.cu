@@ -29,7 +29,9 @@ struct Split {
   static constexpr int KK = HD / 64;                    // runs of 64 dims
   static constexpr int W = HD == 64 ? 64 : 128, WN = HD / W, WW = W / 32;  // windows of dims a lane's read of the values lies in, words of such a read
   static constexpr int CH = HD / 16, LR = 32 / CH, COPIES = SUB / LR;      // chunks of a row, rows a warp copies at once, such copies
-  static constexpr unsigned stage_bytes = 2 * SUB * HD, ring = STAGES * stage_bytes, scales = WARPS * ring, total = scales + WARPS * STAGES * NP * 8;
+  static constexpr unsigned stage_bytes = 2 * SUB * HD, ring = STAGES * stage_bytes, scales = WARPS * ring, q = scales + WARPS * STAGES * NP * 8,
+                            total = q + TERMS * KK * 1024;
+  static_assert(WARPS == 8, "a warp prepares a row of q");
   static constexpr unsigned OP = HD + 4;                // the warps' results on their way together: [warp][8][OP] in the rings' place
   static constexpr unsigned record = 8 * (HD + 2);      // floats: m[8], l[8], O[8][HD]
   static_assert(WARPS * 8 * OP * 4 <= WARPS * ring, "the results fit the rings");
@@ -38,6 +40,7 @@ __device__ __forceinline__ uint32_t smem_at(const void* p) { return (uint32_t)__
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool there) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
 }
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory"); }
 __device__ __forceinline__ void copy4(uint32_t dst, const void* src, bool there) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(there ? 4 : 0) : "memory");
 }
@@ -55,56 +58,91 @@ __device__ __forceinline__ uint32_t turn8x8(uint32_t x) {
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
   return y;
 }
+// 2, 4 or 8 neighbouring dims.
+template <int D>
+__device__ __forceinline__ void load_dims(const float* p, float (&x)[D]) {
+  if constexpr (D == 2) {
+    const float2 v = *reinterpret_cast<const float2*>(p);
+    x[0] = v.x; x[1] = v.y;
+  } else {
+#pragma unroll
+    for (int e = 0; e < D; e += 4) {
+      const float4 v = *reinterpret_cast<const float4*>(p + e);
+      x[e] = v.x; x[e + 1] = v.y; x[e + 2] = v.z; x[e + 3] = v.w;
+    }
+  }
+}
+template <int D>
+__device__ __forceinline__ void load_dims(const __half* p, float (&x)[D]) {
+  uint32_t w[D / 2];
+  if constexpr (D == 2) w[0] = *reinterpret_cast<const uint32_t*>(p);
+  else if constexpr (D == 4) {
+    const uint2 v = *reinterpret_cast<const uint2*>(p);
+    w[0] = v.x; w[1] = v.y;
+  } else {
+    const uint4 v = *reinterpret_cast<const uint4*>(p);
+    w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
+  }
+#pragma unroll
+  for (int e = 0; e < D; e += 2) {
+    const float2 f = __half22float2(q8_h2(w[e / 2]));
+    x[e] = f.x; x[e + 1] = f.y;
+  }
+}
+
 template <int HD, typename T, bool FP8>
 __global__ void __launch_bounds__(Split<HD, T>::THREADS, Split<HD, T>::PER_SM) sdpa_q8_split_kernel(const ks_sdpa_q8_args a) {
   using S = Split<HD, T>;
   extern __shared__ __align__(128) unsigned char smem[];
-  __shared__ unsigned long long scan[S::WARPS], seq_first, line[2];
-  __shared__ unsigned seq_at;
-  __shared__ float row_m[S::WARPS][8], row_l[S::WARPS][8];
+  __shared__ unsigned scan[S::WARPS], seq_first, line[2], seq_at;
+  __shared__ float row_m[S::WARPS][8], row_l[S::WARPS][8], row_up[8];
   ks_pdl_entry();
   const unsigned tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5, g = lane >> 2, c = lane & 3u;
 
   // ---- the line of units: a thread counts for up to four neighbouring sequences
-  auto units_of = [&](const Seq& s) -> unsigned long long {
+  auto units_of = [&](const Seq& s) -> unsigned {
     const unsigned m = (unsigned)s.rows * a.G;
-    if (m > a.few) return 0ull;
+    if (m > a.few) return 0u;
     const int t0 = s.begin / S::TILE, t1 = (s.len + S::TILE - 1) / S::TILE;
-    return (unsigned long long)((m + 7u) / 8u) * a.n_kv * (unsigned)max(t1 - t0, 1);  // (a row that sees nothing still gets its zeros)
+    return (m + 7u) / 8u * a.n_kv * (unsigned)max(t1 - t0, 1);  // (a row that sees nothing still gets its zeros)
   };
   const unsigned per = (a.n_seqs + S::THREADS - 1u) / S::THREADS;
-  unsigned long long mine[KS_PAGES_MAX_SEQS / 256], sum = 0;
+  unsigned mine[KS_PAGES_MAX_SEQS / 256], sum = 0;
 #pragma unroll
   for (unsigned k = 0; k < KS_PAGES_MAX_SEQS / 256; k++) {
     const unsigned i = tid * per + k;
     Seq s;
-    mine[k] = k < per && i < a.n_seqs && seq_of(a, i, s) ? units_of(s) : 0ull;
+    mine[k] = k < per && i < a.n_seqs && seq_of(a, i, s) ? units_of(s) : 0u;
     sum += mine[k];
   }
-  unsigned long long before = sum;
+  unsigned before = sum;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const unsigned long long up = __shfl_up_sync(0xffffffffu, before, o);
+    const unsigned up = __shfl_up_sync(0xffffffffu, before, o);
     if (lane >= (unsigned)o) before += up;
   }
   if (lane == 31u) scan[warp] = before;
   __syncthreads();
-  unsigned long long total = 0;
+  unsigned total = 0;
   before -= sum;
+#pragma unroll
   for (unsigned w = 0; w < S::WARPS; w++) {
-    before += w < warp ? scan[w] : 0ull;
-    total += scan[w];
+    const unsigned x = scan[w];
+    before += w < warp ? x : 0u;
+    total += x;
   }
-  const unsigned long long blocks = min((unsigned long long)gridDim.x, (total + a.least - 1u) / a.least);
+  const unsigned blocks = min(gridDim.x, (total + a.least - 1u) / a.least);
   if (blockIdx.x >= blocks) {
     if (tid == 0) a.merges[2u * blockIdx.x] = make_int4(0, 0, 0, 0);
     return;
   }
+  // the first `more` blocks take `each` + 1 units, the others `each`
+  const unsigned each = total / blocks, more = total - each * blocks;
+  const unsigned u_begin = blockIdx.x * each + min(blockIdx.x, more), u_end = u_begin + each + (blockIdx.x < more ? 1u : 0u);
   if (tid == 0) {
-    line[0] = total;
-    line[1] = blocks;
+    line[0] = each;
+    line[1] = more;
   }
-  const unsigned long long u_begin = blockIdx.x * total / blocks, u_end = (blockIdx.x + 1u) * total / blocks;
 #pragma unroll
   for (unsigned k = 0; k < KS_PAGES_MAX_SEQS / 256; k++) {
     const unsigned i = tid * per + k;
@@ -124,23 +162,30 @@ __global__ void __launch_bounds__(Split<HD, T>::THREADS, Split<HD, T>::PER_SM) s
   const float to_log2 = a.scale * 1.44269504088896340736f;
 
   // ---- piece after piece
-  unsigned seq = seq_at, in_block = 0;
-  unsigned long long u = u_begin, at = seq_first;
+  unsigned seq = seq_at, in_block = 0, u = u_begin, at = seq_first;
   Seq s;
-  bool have = seq_of(a, seq, s);
+  unsigned units = seq_of(a, seq, s) ? units_of(s) : 0u;
   while (u < u_end) {
-    while (u - at >= (have ? units_of(s) : 0ull)) {
-      at += have ? units_of(s) : 0ull;
-      have = seq_of(a, ++seq, s);
+    while (u - at >= units) {
+      at += units;
+      units = seq_of(a, ++seq, s) ? units_of(s) : 0u;
     }
     const int tile0 = s.begin / S::TILE, n_tiles = max((s.len + S::TILE - 1) / S::TILE - tile0, 1);
     const unsigned m_rows = (unsigned)s.rows * a.G, m_tiles = (m_rows + 7u) / 8u;
-    const unsigned piece = (unsigned)((u - at) / (unsigned)n_tiles), t_first = (unsigned)((u - at) % (unsigned)n_tiles);
+    const unsigned piece = (u - at) / (unsigned)n_tiles, t_first = u - at - piece * (unsigned)n_tiles;
     const unsigned kvh = piece / m_tiles, m0 = piece % m_tiles * 8u;
-    const unsigned n = (unsigned)min((unsigned long long)((unsigned)n_tiles - t_first), u_end - u);  // tiles of this piece that are ours
+    const unsigned n = min((unsigned)n_tiles - t_first, u_end - u);  // tiles of this piece that are ours
     const int p_first = (tile0 + (int)t_first) * S::TILE + (int)warp * S::SUB;                       // this warp's positions of the first
     const int* table = a.tables + (size_t)seq * a.max_blocks;
 
+    // q: a warp a row, its values in the order in which the codes of a 16-byte read meet them (16 c .. 16 c + 15 of every 64 dims).  f32 rows are
+    // brought to 2^14 by a power of two and split into two f16 terms.  (Every warp for itself took 2500 clocks of a one-step call.)
+    constexpr int QD = HD / 32;
+    float qx[QD];
+    {
+      const unsigned m = min(m0 + warp, m_rows - 1u);  // (columns behind the last row repeat it)
+      load_dims<QD>((const T*)a.q + ((size_t)(s.row0 + (int)(m / a.G)) * a.n_q + kvh * a.G + m % a.G) * HD + QD * lane, qx);
+    }
     // the page of 16 positions (a page has no fewer) as the table has it: read a step before it is looked at
     auto page_of = [&](int p) -> int { return p + 15 < s.begin || p >= s.len ? -1 : table[(unsigned)p >> a.page_log]; };
     // copies of SUB positions into stage st: 16 bytes a lane, chunks swapped about so that the reads below meet no bank twice; positions that
@@ -155,6 +200,16 @@ __global__ void __launch_bounds__(Split<HD, T>::THREADS, Split<HD, T>::PER_SM) s
         const size_t block = (size_t)(page ? id[b] : 0) * a.n_kv + kvh;
         const size_t from = (((block << a.page_log) + ((unsigned)p & ((1u << a.page_log) - 1u)) + r0) * HD) + ch * 16u;
         const uint32_t to = ring_at + st * S::stage_bytes + (unsigned)b * 16u * HD;
+        if (page && p >= s.begin && p + 16 <= s.len) {  // (the usual case: 16 rows follow one another in memory)
+          const uint8_t *from_k = a.kc + from, *from_v = a.vc + from;
+#pragma unroll
+          for (int i = 0; i < S::COPIES / S::NP; i++) {
+            const unsigned r = r0 + (unsigned)(i * S::LR);
+            const unsigned kch = HD >= 128 ? ch ^ ((r & 1u) << 2) : ch, vch = HD >= 128 ? ch ^ ((r >> 1 & 3u) << 1) : ch ^ ((r >> 1 & 1u) << 1);
+            copy16(to + r * HD + kch * 16u, from_k + i * S::LR * HD);
+            copy16(to + S::SUB * HD + r * HD + vch * 16u, from_v + i * S::LR * HD);
+          }
+        } else
 #pragma unroll
         for (int i = 0; i < S::COPIES / S::NP; i++) {
           const unsigned r = r0 + (unsigned)(i * S::LR);
@@ -181,51 +236,50 @@ __global__ void __launch_bounds__(Split<HD, T>::THREADS, Split<HD, T>::PER_SM) s
 #pragma unroll
     for (int b = 0; b < S::NP; b++) id[b] = ids[S::STAGES - 1][b];
 
-    // ---- q: row g, dims 16 c .. 16 c + 15 of every 64: what the codes of a 16-byte read meet.  f32 rows are brought to 2^14 by a power of
-    // two and split into two f16 terms
+    // ---- q's terms through shared memory
     uint32_t qb[S::TERMS][S::KK][4][2];
     float up[2] = {1.0f, 1.0f};
     {
-      const unsigned m = m0 + g;
-      const bool in = m < m_rows;
-      const T* src = (const T*)a.q + ((size_t)(s.row0 + (int)(m / a.G)) * a.n_q + kvh * a.G + m % a.G) * HD + 16u * c;
-      if constexpr (S::TERMS == 1) {
+      uint32_t* qs = reinterpret_cast<uint32_t*>(smem + S::q);
+      float down = 1.0f;
+      if constexpr (S::TERMS == 2) {
+        float big = 0.0f;
 #pragma unroll
-        for (int kk = 0; kk < S::KK; kk++) {
-          const uint4 x = in ? *reinterpret_cast<const uint4*>(src + 64 * kk) : make_uint4(0, 0, 0, 0), y = in ? *reinterpret_cast<const uint4*>(src + 64 * kk + 8) : make_uint4(0, 0, 0, 0);
-          const uint32_t w[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+        for (int e = 0; e < QD; e++) big = fmaxf(big, fabsf(qx[e]));
 #pragma unroll
-          for (int k = 0; k < 4; k++) {
-            qb[0][kk][k][0] = w[2 * k];
-            qb[0][kk][k][1] = w[2 * k + 1];
-          }
-        }
-      } else {
-        float x[S::KK][16], big = 0.0f;
-#pragma unroll
-        for (int kk = 0; kk < S::KK; kk++)
-#pragma unroll
-          for (int e = 0; e < 16; e += 4) {
-            const float4 v = in ? *reinterpret_cast<const float4*>((const float*)src + 64 * kk + e) : make_float4(0.f, 0.f, 0.f, 0.f);
-            x[kk][e] = v.x; x[kk][e + 1] = v.y; x[kk][e + 2] = v.z; x[kk][e + 3] = v.w;
-            big = fmaxf(fmaxf(big, fmaxf(fabsf(v.x), fabsf(v.y))), fmaxf(fabsf(v.z), fabsf(v.w)));
-          }
-        big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
-        big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
+        for (int o = 16; o > 0; o >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
         const int ex = big > 0.0f && big < 3.0e38f ? max((int)(__float_as_uint(big) >> 23) - 127 - 14, -100) : 0;
-        const float mul = __uint_as_float((uint32_t)(127 + ex) << 23), down = __uint_as_float((uint32_t)(127 - ex) << 23);
-        up[0] = __shfl_sync(0xffffffffu, mul, 8u * c);
-        up[1] = __shfl_sync(0xffffffffu, mul, 8u * c + 4u);
+        down = __uint_as_float((uint32_t)(127 - ex) << 23);
+        if (lane == 0) row_up[warp] = __uint_as_float((uint32_t)(127 + ex) << 23);
+      }
+#pragma unroll
+      for (int e = 0; e < QD; e += 2) {
+        const unsigned dim = QD * lane + e, kk = dim >> 6, cc = dim >> 4 & 3u, k = dim >> 2 & 3u, h = dim >> 1 & 1u;
+        uint32_t* to = qs + ((kk * 2u + (k >> 1)) * 32u + 4u * warp + cc) * 4u + (k & 1u) * 2u + h;
+        const float x0 = qx[e] * down, x1 = qx[e + 1] * down;
+        const __half2 big = __floats2half2_rn(x0, x1);
+        *to = q8_u32(big);
+        if constexpr (S::TERMS == 2) {
+          const float2 f = __half22float2(big);
+          to[S::KK * 256] = q8_u32(__floats2half2_rn(x0 - f.x, x1 - f.y));
+        }
+      }
+      __syncthreads();
+#pragma unroll
+      for (int t = 0; t < S::TERMS; t++)
 #pragma unroll
         for (int kk = 0; kk < S::KK; kk++)
 #pragma unroll
-          for (int e = 0; e < 16; e += 2) {
-            const float x0 = x[kk][e] * down, x1 = x[kk][e + 1] * down;
-            const __half2 hi = __floats2half2_rn(x0, x1);
-            const float2 f = __half22float2(hi);
-            qb[0][kk][e / 4][(e & 2) / 2] = q8_u32(hi);
-            qb[S::TERMS - 1][kk][e / 4][(e & 2) / 2] = q8_u32(__floats2half2_rn(x0 - f.x, x1 - f.y));
+          for (int k = 0; k < 4; k += 2) {
+            const uint4 w = *reinterpret_cast<const uint4*>(qs + t * S::KK * 256 + ((kk * 2 + k / 2) * 32 + lane) * 4);
+            qb[t][kk][k][0] = w.x;
+            qb[t][kk][k][1] = w.y;
+            qb[t][kk][k + 1][0] = w.z;
+            qb[t][kk][k + 1][1] = w.w;
           }
+      if constexpr (S::TERMS == 2) {
+        up[0] = row_up[2u * c];
+        up[1] = row_up[2u * c + 1u];
       }
     }
     // ---- this lane's scores: positions g (+ 8) of query rows 2 c and 2 c + 1, which see positions lo .. hi
@@ -486,9 +540,9 @@ __global__ void __launch_bounds__(Split<HD, T>::THREADS, Split<HD, T>::PER_SM) s
     // what the merge has to do for this block: the piece that began in an earlier one and ends here, if there is one
     if (in_block == 0 && tid == 0) {
       const bool ends = t_first > 0 && t_first + n == (unsigned)n_tiles;
-      const unsigned long long u0 = u - t_first, total = line[0], blocks = line[1];
-      const unsigned b0 = (unsigned)(((u0 + 1u) * blocks - 1u) / total);
-      a.merges[2u * blockIdx.x] = make_int4((int)b0, ends ? (int)(blockIdx.x - b0 + 1u) : 0, b0 * total / blocks >= u0 ? 0 : 1, (int)m0);
+      const unsigned u0 = u - t_first, each = line[0], more = line[1], big = more * (each + 1u);
+      const unsigned b0 = u0 < big ? u0 / (each + 1u) : more + (u0 - big) / each, b0_begin = b0 * each + min(b0, more);
+      a.merges[2u * blockIdx.x] = make_int4((int)b0, ends ? (int)(blockIdx.x - b0 + 1u) : 0, b0_begin == u0 ? 0 : 1, (int)m0);
       a.merges[2u * blockIdx.x + 1u] = make_int4(s.row0, (int)kvh, (int)m_rows, 0);
     }
     u += n;
@@ -504,7 +558,7 @@ template <int HD, typename T>
 __global__ void __launch_bounds__(1024) sdpa_q8_merge_kernel(const ks_sdpa_q8_args a) {
   using S = Split<HD, T>;
   constexpr int D = HD / 32, V = D == 2 ? 2 : 4;
-  __shared__ float red[3][8][HD];
+  __shared__ float red[3][8][HD], tops[4][8], sums[4][8];
   ks_pdl_entry();
   const unsigned lane = threadIdx.x & 31u, warp = threadIdx.x >> 5, r = warp & 7u, share = warp >> 3;
   const int4 job = a.merges[2u * blockIdx.x], where = a.merges[2u * blockIdx.x + 1u];
@@ -512,53 +566,65 @@ __global__ void __launch_bounds__(1024) sdpa_q8_merge_kernel(const ks_sdpa_q8_ar
   if (n == 0u) return;
   const float* rec = a.part + (size_t)job.x * 2u * S::record;
   auto record = [&](unsigned k) { return rec + (k ? k * 2u : (unsigned)job.z) * (size_t)S::record; };  // (the first block's record is its second one unless the piece starts with the block)
+  // a share's records four at a time: maxima, sums and values on one trip, then together as a running softmax
   float top = kNone, l = 0.0f, v[D];
 #pragma unroll
   for (int d = 0; d < D; d++) v[d] = 0.0f;
   const bool live = m < (unsigned)where.z;
   if (live) {
-    for (unsigned k = lane; k < n; k += 32u) top = fmaxf(top, record(k)[r]);
+    constexpr unsigned FLY = 4;
+    for (unsigned k0 = share; k0 < n; k0 += 4u * FLY) {
+      float mk[FLY], lk[FLY], o[FLY][D];
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    for (unsigned k = lane; k < n; k += 32u) l = fmaf(exp2_fast(record(k)[r] - top), record(k)[8 + r], l);
-    l = q8_warp_sum(l);
-#pragma unroll 4
-    for (unsigned k = share; k < n; k += 4u) {
-      const float* x = record(k);
-      const float e = exp2_fast(x[r] - top);
-#pragma unroll
-      for (int d = 0; d < D; d += V) {
-        const float* from = x + 16 + r * HD + V * lane + 32 * d;
-        if constexpr (V == 4) {
-          const float4 y = *reinterpret_cast<const float4*>(from);
-          v[d] = fmaf(y.x, e, v[d]);
-          v[d + 1] = fmaf(y.y, e, v[d + 1]);
-          v[d + 2] = fmaf(y.z, e, v[d + 2]);
-          v[d + 3] = fmaf(y.w, e, v[d + 3]);
-        } else {
-          const float2 y = *reinterpret_cast<const float2*>(from);
-          v[d] = fmaf(y.x, e, v[d]);
-          v[d + 1] = fmaf(y.y, e, v[d + 1]);
-        }
+      for (unsigned f = 0; f < FLY; f++) {
+        const bool there = k0 + 4u * f < n;
+        const float* x = record(there ? k0 + 4u * f : k0);
+        mk[f] = there ? x[r] : kNone;
+        lk[f] = there ? x[8 + r] : 0.0f;
+        load_dims<D>(x + 16 + r * HD + D * lane, o[f]);
       }
+      float most = top;
+#pragma unroll
+      for (unsigned f = 0; f < FLY; f++) most = fmaxf(most, mk[f]);
+      const float turn = exp2_fast(top - most);
+      top = most;
+      l *= turn;
+#pragma unroll
+      for (int d = 0; d < D; d++) v[d] *= turn;
+#pragma unroll
+      for (unsigned f = 0; f < FLY; f++) {
+        const float e = k0 + 4u * f < n ? exp2_fast(mk[f] - top) : 0.0f;
+        l = fmaf(lk[f], e, l);
+#pragma unroll
+        for (int d = 0; d < D; d++) v[d] = fmaf(o[f][d], e, v[d]);
+      }
+    }
+    if (lane == 0) {
+      tops[share][r] = top;
+      sums[share][r] = l;
     }
     if (share > 0)
 #pragma unroll
-      for (int d = 0; d < D; d += V) put_dims(&red[share - 1u][r][V * lane + 32 * d], v + d, V);
+      for (int d = 0; d < D; d++) red[share - 1u][r][d * 32 + lane] = v[d];
   }
   __syncthreads();
   if (!live || share > 0) return;
-  const float f = over(l);
-  T* to = (T*)a.out + ((size_t)(where.x + (int)(m / a.G)) * a.n_q + (unsigned)where.y * a.G + m % a.G) * HD;
+  float most = kNone, e[4];
 #pragma unroll
-  for (int d = 0; d < D; d += V) {
+  for (int k = 0; k < 4; k++) most = fmaxf(most, tops[k][r]);
+  l = 0.0f;
 #pragma unroll
-    for (int k = 0; k < V; k++) {
-      const unsigned at = V * lane + 32 * d + k;
-      v[d + k] = (v[d + k] + red[0][r][at] + (red[1][r][at] + red[2][r][at])) * f;
-    }
-    put_dims(to + V * lane + 32 * d, v + d, V);
+  for (int k = 0; k < 4; k++) {
+    e[k] = exp2_fast(tops[k][r] - most);
+    l = fmaf(sums[k][r], e[k], l);
   }
+  const float f = over(l);
+  T* to = (T*)a.out + ((size_t)(where.x + (int)(m / a.G)) * a.n_q + (unsigned)where.y * a.G + m % a.G) * HD + D * lane;
+#pragma unroll
+  for (int d = 0; d < D; d++)
+    v[d] = (v[d] * e[0] + red[0][r][d * 32 + lane] * e[1] + (red[1][r][d * 32 + lane] * e[2] + red[2][r][d * 32 + lane] * e[3])) * f;
+#pragma unroll
+  for (int d = 0; d < D; d += V) put_dims(to + d, v + d, V);
 }
 
 unsigned split_blocks(const ks_ctx* ctx, size_t hd) { return (unsigned)ctx->sm_count * (hd == 256 ? Split<256, float>::PER_SM : Split<128, float>::PER_SM); }  // as many as run at once
@@ -612,6 +678,9 @@ int ks_sdpa_paged_q8(ks_ctx* ctx, const ks_q8_cache* c, const ks_page_tables* t,
   KS_REQUIRE(ctx, qa + bytes <= oa || oa + bytes <= qa, "%s: q and out overlap", who);
   KS_REQUIRE(ctx, ks_fits(tmp, 0, ks_sdpa_paged_tmp_floats(ctx, c, t, n_q, rows_most) * 4) && ks_aligned(tmp, 16), "%s: tmp buffer too small, or not on 16 bytes", who);
   if (rows_most == 0) return KS_OK;
+  // units of the split kernel's line are counted in 32 bits
+  const size_t tiles_most = (t->max_blocks * t->page + 127) / 128, m_most = (KS_Q8_FEW + 7) / 8;
+  if (t->n_seqs * tiles_most >= (size_t(1) << 31) / (m_most * c->n_kv)) return ks_fail(ctx, KS_ERR_UNSUPPORTED, "%s: %zu sequences of up to %zu positions and %zu KV heads are too much for one call", who, t->n_seqs, t->max_blocks * t->page, c->n_kv);
   KS_REQUIRE_DEVICE(ctx, who);
   ks_on_device on(ctx);
   ks_sdpa_q8_args a{};
