@@ -1,9 +1,9 @@
 // Pages of a paged cache handed out on the GPU: tables, lengths, the stack of free pages and the plan of a step's rows.
 //
 // A step is integer arithmetic on three exclusive sums over the sequences (rows, new pages, touched pages) and one record per row, so it
-// is bound by latency: one trip for lengths and counts, the sums, one trip for a row's page, the stores.  Every block makes the sums
-// for itself and takes a run of rows; nothing that a block reads is written by another, except lengths and the stack's count, which the
-// block that arrives last at a counter writes (all have read them by then).
+// is bound by latency: one trip for lengths and counts, the sums, one trip for a row's page, the stores.  Many rows are shared by the blocks
+// of one cluster: each makes the sums for itself and takes rows; nothing that a block reads is written by another, except lengths and
+// the stack's count, which block 0 writes behind the cluster's barrier (all have read them by then).
 #include "ks_q8.h"
 
 namespace {
@@ -12,7 +12,7 @@ struct TablesArgs {
   unsigned n_seqs, max_blocks, n_pages, page_log, max_rows;
   int *lens, *tables, *free_pages, *plan;
   ks_plan_layout at;
-  unsigned *bad, *arrived;
+  unsigned* bad;
 };
 
 // Exclusive sums of three counts over the block's threads (a multiple of 32, up to 1024); totals in tot.
@@ -31,25 +31,28 @@ __device__ __forceinline__ void scan3(unsigned (&v)[3], unsigned (&tot)[3], unsi
   }
   __syncthreads();
 #pragma unroll
-  for (int k = 0; k < 3; k++) {
-    unsigned before = 0, all = 0;
-    for (unsigned w = 0; w < nwarp; w++) {
-      const unsigned x = red[w][k];
-      before += w < warp ? x : 0u;
-      all += x;
+  for (int k = 0; k < 3; k++) {  // every warp adds up the warps' totals
+    unsigned all = lane < nwarp ? red[lane][k] : 0u, before = lane < warp ? all : 0u;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      all += __shfl_xor_sync(0xffffffffu, all, o);
+      before += __shfl_xor_sync(0xffffffffu, before, o);
     }
     v[k] = before + inc[k] - v[k];
     tot[k] = all;
   }
 }
 
-__global__ void __launch_bounds__(1024) pages_step_kernel(const TablesArgs a, const int* n_new) {
+constexpr unsigned kCluster = 8;
+// A thread takes four neighbouring rows: one search for the sequence of the first, 16-byte stores.
+template <bool CLUSTER>
+__device__ __forceinline__ void step_rows(const TablesArgs& a, const int* n_new) {
   __shared__ unsigned red[32][3];
-  __shared__ unsigned first_row[KS_PAGES_MAX_SEQS], first_page[KS_PAGES_MAX_SEQS], first_job[KS_PAGES_MAX_SEQS];
-  __shared__ int len_of[KS_PAGES_MAX_SEQS];
-  __shared__ unsigned last;
-  ks_pdl_entry();
+  __shared__ unsigned first_row[KS_PAGES_MAX_SEQS + 1], first_page[KS_PAGES_MAX_SEQS], first_job[KS_PAGES_MAX_SEQS];
+  __shared__ int len_of[KS_PAGES_MAX_SEQS], worst_s;
   const unsigned tid = threadIdx.x, page = 1u << a.page_log, cap = a.max_blocks << a.page_log;
+  if (tid == 0) worst_s = 0;
+  ks_pdl_entry();
   const int count = a.free_pages[0];
   int len = 0, add = 0;
   if (tid < a.n_seqs) {
@@ -65,41 +68,61 @@ __global__ void __launch_bounds__(1024) pages_step_kernel(const TablesArgs a, co
   if (status == KS_PLAN_BAD_LENGTH) len = 0;
   const unsigned after = (unsigned)len + (unsigned)add, held = ((unsigned)len + page - 1u) >> a.page_log;
   unsigned v[3] = {(unsigned)add, ((after + page - 1u) >> a.page_log) - held, add ? ((after - 1u) >> a.page_log) - ((unsigned)len >> a.page_log) + 1u : 0u}, tot[3];
-  scan3(v, tot, red);
+  __syncthreads();
+  if (status) atomicMax(&worst_s, status);
+  scan3(v, tot, red);  // (a barrier inside: worst_s is complete behind it)
+  int worst = worst_s;
+  if (worst < KS_PLAN_TOO_MANY_ROWS && tot[0] > a.max_rows) worst = KS_PLAN_TOO_MANY_ROWS;
+  if (worst == 0 && (count < 0 || (unsigned)count > a.n_pages || tot[1] > (unsigned)count)) worst = KS_PLAN_NO_PAGES;
+  const unsigned rows = worst ? 0u : tot[0], jobs = worst ? 0u : tot[2];
   if (tid < a.n_seqs) {
     first_row[tid] = v[0];
     first_page[tid] = v[1];
     first_job[tid] = v[2];
     len_of[tid] = len;
   }
-  int worst = status;
+  if (tid == 0) first_row[a.n_seqs] = rows;
+  __syncthreads();
+  if (CLUSTER) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");  // lengths and count have been read by this block
+  const unsigned step = gridDim.x * blockDim.x, quads = (a.max_rows + 3u) >> 2, me = blockIdx.x * blockDim.x + tid;
+  int4 *seqs = reinterpret_cast<int4*>(a.plan + a.at.row_seq), *poss = reinterpret_cast<int4*>(a.plan + a.at.row_pos), *slots = reinterpret_cast<int4*>(a.plan + a.at.row_slot);
+  for (unsigned q = me; q < quads; q += step) {
+    int seq[4], pos[4], slot[4];
+    unsigned lo = 0;
+    if (4u * q < rows) {
+      unsigned hi = a.n_seqs;  // the last sequence that starts at row 4 q or before
+      while (hi - lo > 1u) {
+        const unsigned mid = (lo + hi) >> 1;
+        if (first_row[mid] <= 4u * q) lo = mid;
+        else hi = mid;
+      }
+    }
 #pragma unroll
-  for (int s = KS_PLAN_BAD_LENGTH; s > 0; s--)
-    if (__syncthreads_or(status == s)) {
-      worst = s;
-      break;
+    for (int k = 0; k < 4; k++) {
+      const unsigned r = 4u * q + k;
+      seq[k] = pos[k] = slot[k] = -1;
+      if (r >= rows) continue;
+      while (first_row[lo + 1u] <= r) lo++;
+      const unsigned l0 = (unsigned)len_of[lo], p = l0 + (r - first_row[lo]), b = p >> a.page_log, had = (l0 + page - 1u) >> a.page_log, off = p & (page - 1u);
+      int id;
+      if (b >= had) {
+        id = a.free_pages[(unsigned)count - first_page[lo] - (b - had)];
+        if (off == 0u) a.tables[(size_t)lo * a.max_blocks + b] = id;
+      } else {
+        id = a.tables[(size_t)lo * a.max_blocks + b];
+      }
+      seq[k] = (int)lo;
+      pos[k] = (int)p;
+      if (id >= 0 && (unsigned)id < a.n_pages) slot[k] = (int)(((unsigned)id << a.page_log) + off);
+      else atomicOr(a.bad, KS_BAD_PAGE);
+      if (r == first_row[lo] || off == 0u)
+        reinterpret_cast<int4*>(a.plan + a.at.jobs)[first_job[lo] + (b - (l0 >> a.page_log))] = make_int4((int)r, (int)min(page - off, first_row[lo + 1u] - r), slot[k], (int)p);
     }
-  if (worst < KS_PLAN_TOO_MANY_ROWS && tot[0] > a.max_rows) worst = KS_PLAN_TOO_MANY_ROWS;
-  if (worst == 0 && (count < 0 || (unsigned)count > a.n_pages || tot[1] > (unsigned)count)) worst = KS_PLAN_NO_PAGES;
-  const unsigned rows = worst ? 0u : tot[0], jobs = worst ? 0u : tot[2];
-  // lengths and count have been read by every thread of this block
-  if (gridDim.x > 1u) {
-    if (tid == 0) {
-      __threadfence();
-      last = atomicAdd(a.arrived, 1u) == gridDim.x - 1u;
-    }
-    __syncthreads();
-  } else {
-    if (tid == 0) last = 1u;
-    __syncthreads();
+    seqs[q] = make_int4(seq[0], seq[1], seq[2], seq[3]);
+    poss[q] = make_int4(pos[0], pos[1], pos[2], pos[3]);
+    slots[q] = make_int4(slot[0], slot[1], slot[2], slot[3]);
   }
-  if (last) {
-    if (tid < a.n_seqs && !worst) a.lens[tid] = (int)after;
-    if (tid == 0) {
-      if (!worst) a.free_pages[0] = count - (int)tot[1];
-      if (gridDim.x > 1u) *a.arrived = 0u;
-    }
-  }
+  for (unsigned j = jobs + me; j < a.at.n_jobs; j += step) reinterpret_cast<int4*>(a.plan + a.at.jobs)[j] = make_int4(-1, -1, -1, -1);
   if (blockIdx.x == 0) {
     if (tid < a.n_seqs) a.plan[a.at.row_start + tid] = worst ? 0 : (int)v[0];
     if (tid < KS_PAGES_PLAN_HEADER) {
@@ -107,40 +130,13 @@ __global__ void __launch_bounds__(1024) pages_step_kernel(const TablesArgs a, co
       a.plan[tid] = tid < 4u ? head[tid] : 0;
     }
     if (tid == 0) a.plan[a.at.row_start + a.n_seqs] = (int)rows;
+    if (CLUSTER) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    if (tid < a.n_seqs && !worst) a.lens[tid] = (int)after;
+    if (tid == 0 && !worst) a.free_pages[0] = count - (int)tot[1];
   }
-  const unsigned step = gridDim.x * blockDim.x, words = (a.max_rows + 3u) & ~3u;
-  for (unsigned r = blockIdx.x * blockDim.x + tid; r < words; r += step) {
-    int seq = -1, pos = -1, slot = -1;
-    if (r < rows) {
-      unsigned lo = 0, hi = a.n_seqs;  // the last sequence that starts at r or before and has rows
-      while (hi - lo > 1u) {
-        const unsigned mid = (lo + hi) >> 1;
-        if (first_row[mid] <= r) lo = mid;
-        else hi = mid;
-      }
-      const unsigned l0 = (unsigned)len_of[lo], p = l0 + (r - first_row[lo]), b = p >> a.page_log, had = (l0 + page - 1u) >> a.page_log;
-      int id;
-      if (b >= had) {
-        id = a.free_pages[(unsigned)count - first_page[lo] - (b - had)];
-        if ((p & (page - 1u)) == 0u) a.tables[(size_t)lo * a.max_blocks + b] = id;
-      } else {
-        id = a.tables[(size_t)lo * a.max_blocks + b];
-      }
-      seq = (int)lo;
-      pos = (int)p;
-      if (id >= 0 && (unsigned)id < a.n_pages) slot = (int)(((unsigned)id << a.page_log) + (p & (page - 1u)));
-      else atomicOr(a.bad, KS_BAD_PAGE);
-      if (r == first_row[lo] || (p & (page - 1u)) == 0u) {
-        const unsigned end = lo + 1u < a.n_seqs ? first_row[lo + 1u] : rows;
-        reinterpret_cast<int4*>(a.plan + a.at.jobs)[first_job[lo] + (b - (l0 >> a.page_log))] = make_int4((int)r, (int)min(page - (p & (page - 1u)), end - r), slot, (int)p);
-      }
-    }
-    a.plan[a.at.row_seq + r] = seq;
-    a.plan[a.at.row_pos + r] = pos;
-    a.plan[a.at.row_slot + r] = slot;
-  }
-  for (unsigned j = jobs + blockIdx.x * blockDim.x + tid; j < a.at.n_jobs; j += step) reinterpret_cast<int4*>(a.plan + a.at.jobs)[j] = make_int4(-1, -1, -1, -1);
 }
+__global__ void __launch_bounds__(1024) pages_step_kernel(const TablesArgs a, const int* n_new) { step_rows<false>(a, n_new); }
+__global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(1024) pages_step_cluster_kernel(const TablesArgs a, const int* n_new) { step_rows<true>(a, n_new); }
 
 // One block: the sum over the sequences, then one page per thread and step.
 __global__ void __launch_bounds__(1024) pages_trim_kernel(const TablesArgs a, const int* keep) {
@@ -207,7 +203,6 @@ TablesArgs args_of(ks_ctx* ctx, const ks_page_tables* t) {
   a.plan = (int*)t->plan->dptr;
   a.at = ks_plan_parts(t->n_seqs, t->max_rows, t->page);
   a.bad = (unsigned*)ctx->ws + KS_WS_INDEX_WORD;
-  a.arrived = (unsigned*)ctx->ws + KS_WS_COUNT_WORD;
   return a;
 }
 unsigned round32(size_t n) { return (unsigned)((n + 31) & ~size_t(31)); }
@@ -260,10 +255,14 @@ int ks_pages_step(ks_ctx* ctx, const ks_page_tables* t, const ks_buf* n_new) {
   KS_REQUIRE(ctx, ks_fits(n_new, 0, t->n_seqs * 4) && ks_aligned(n_new, 4), "pages_step: n_new buffer too small or not on 4 bytes");
   KS_REQUIRE_DEVICE(ctx, "pages_step");
   ks_on_device on(ctx);
-  const unsigned threads = t->n_seqs > 256 || t->max_rows > 2048 ? (t->n_seqs > 512 ? 1024 : 512) : t->n_seqs > 128 || t->max_rows > 256 ? 256 : 128;
-  const size_t blocks = (t->max_rows + 4 * threads - 1) / (4 * threads);
-  const unsigned most = 64u;
-  KS_LAUNCH(ctx, pages_step_kernel, (unsigned)(blocks < most ? blocks : most), threads, 0, args_of(ctx, t), (const int*)n_new->dptr);
+  // a thread four rows: one block up to 2048 of them, else a cluster
+  if (t->max_rows > 2048) {
+    const unsigned threads = t->n_seqs > 512 || t->max_rows > 4 * 512 * kCluster ? 1024 : 512;
+    KS_LAUNCH(ctx, pages_step_cluster_kernel, kCluster, threads, 0, args_of(ctx, t), (const int*)n_new->dptr);
+  } else {
+    const size_t most = t->n_seqs > t->max_rows / 4 ? t->n_seqs : t->max_rows / 4;
+    KS_LAUNCH(ctx, pages_step_kernel, 1, round32(most) < 128u ? 128u : round32(most), 0, args_of(ctx, t), (const int*)n_new->dptr);
+  }
   return ks_after_launch(ctx, "pages_step");
 }
 

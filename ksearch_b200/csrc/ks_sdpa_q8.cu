@@ -21,6 +21,18 @@ namespace {
 // Codes become f16 exactly, f32 queries and probabilities are two f16 terms each (the small one first), and in f32 the values of every SUB
 // positions are added to registers: a chain of accumulating MMAs loses low bits at every step.  The maximum that probabilities refer to
 // moves only when a score exceeds it by 2^4.
+// The longest context lies in no more blocks than this: each leaves a record that the merge has to read (16384 positions of one KV head: 27 us in 128
+// blocks).
+constexpr unsigned kMostParts = 64;
+// x / d: one multiplication where the numbers are small enough for it to be off by less than one.
+__device__ __forceinline__ unsigned quotient(unsigned x, unsigned d) {
+  if ((x | d) >> 20) return x / d;
+  unsigned q = (unsigned)__fdividef((float)x, (float)d);
+  const int r = (int)(x - q * d);
+  if (r < 0) q--;
+  else if (r >= (int)d) q++;
+  return q;
+}
 template <int HD_, typename T_>
 struct Split {
   static constexpr int HD = HD_, TERMS = sizeof(T_) == 4 ? 2 : 1;
@@ -94,26 +106,26 @@ template <int HD, typename T, bool FP8>
 __global__ void __launch_bounds__(Split<HD, T>::THREADS, Split<HD, T>::PER_SM) sdpa_q8_split_kernel(const ks_sdpa_q8_args a) {
   using S = Split<HD, T>;
   extern __shared__ __align__(128) unsigned char smem[];
-  __shared__ unsigned scan[S::WARPS], seq_first, line[2], seq_at;
+  __shared__ unsigned scan[S::WARPS], longest[S::WARPS], seq_first, line[2], seq_at;
   __shared__ float row_m[S::WARPS][8], row_l[S::WARPS][8], row_up[8];
   ks_pdl_entry();
   const unsigned tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5, g = lane >> 2, c = lane & 3u;
 
   // ---- the line of units: a thread counts for up to four neighbouring sequences
+  auto tiles_of = [&](const Seq& s) -> unsigned { return (unsigned)max((s.len + S::TILE - 1) / S::TILE - s.begin / S::TILE, 1); };  // (a row that sees nothing still gets its zeros)
   auto units_of = [&](const Seq& s) -> unsigned {
     const unsigned m = (unsigned)s.rows * a.G;
-    if (m > a.few) return 0u;
-    const int t0 = s.begin / S::TILE, t1 = (s.len + S::TILE - 1) / S::TILE;
-    return (m + 7u) / 8u * a.n_kv * (unsigned)max(t1 - t0, 1);  // (a row that sees nothing still gets its zeros)
+    return m > a.few ? 0u : (m + 7u) / 8u * a.n_kv * tiles_of(s);
   };
   const unsigned per = (a.n_seqs + S::THREADS - 1u) / S::THREADS;
-  unsigned mine[KS_PAGES_MAX_SEQS / 256], sum = 0;
+  unsigned mine[KS_PAGES_MAX_SEQS / 256], sum = 0, most = 0;
 #pragma unroll
   for (unsigned k = 0; k < KS_PAGES_MAX_SEQS / 256; k++) {
     const unsigned i = tid * per + k;
     Seq s;
     mine[k] = k < per && i < a.n_seqs && seq_of(a, i, s) ? units_of(s) : 0u;
     sum += mine[k];
+    if (mine[k]) most = max(most, tiles_of(s));
   }
   unsigned before = sum;
 #pragma unroll
@@ -121,7 +133,11 @@ __global__ void __launch_bounds__(Split<HD, T>::THREADS, Split<HD, T>::PER_SM) s
     const unsigned up = __shfl_up_sync(0xffffffffu, before, o);
     if (lane >= (unsigned)o) before += up;
   }
-  if (lane == 31u) scan[warp] = before;
+  most = __reduce_max_sync(0xffffffffu, most);
+  if (lane == 31u) {
+    scan[warp] = before;
+    longest[warp] = most;
+  }
   __syncthreads();
   unsigned total = 0;
   before -= sum;
@@ -130,14 +146,15 @@ __global__ void __launch_bounds__(Split<HD, T>::THREADS, Split<HD, T>::PER_SM) s
     const unsigned x = scan[w];
     before += w < warp ? x : 0u;
     total += x;
+    most = max(most, longest[w]);
   }
-  const unsigned blocks = min(gridDim.x, (total + a.least - 1u) / a.least);
+  const unsigned least = max((most + kMostParts - 1u) / kMostParts, 1u), blocks = min(gridDim.x, quotient(total + least - 1u, least));
   if (blockIdx.x >= blocks) {
     if (tid == 0) a.merges[2u * blockIdx.x] = make_int4(0, 0, 0, 0);
     return;
   }
   // the first `more` blocks take `each` + 1 units, the others `each`
-  const unsigned each = total / blocks, more = total - each * blocks;
+  const unsigned each = quotient(total, blocks), more = total - each * blocks;
   const unsigned u_begin = blockIdx.x * each + min(blockIdx.x, more), u_end = u_begin + each + (blockIdx.x < more ? 1u : 0u);
   if (tid == 0) {
     line[0] = each;
@@ -170,10 +187,10 @@ __global__ void __launch_bounds__(Split<HD, T>::THREADS, Split<HD, T>::PER_SM) s
       at += units;
       units = seq_of(a, ++seq, s) ? units_of(s) : 0u;
     }
-    const int tile0 = s.begin / S::TILE, n_tiles = max((s.len + S::TILE - 1) / S::TILE - tile0, 1);
+    const int tile0 = s.begin / S::TILE, n_tiles = (int)tiles_of(s);
     const unsigned m_rows = (unsigned)s.rows * a.G, m_tiles = (m_rows + 7u) / 8u;
-    const unsigned piece = (u - at) / (unsigned)n_tiles, t_first = u - at - piece * (unsigned)n_tiles;
-    const unsigned kvh = piece / m_tiles, m0 = piece % m_tiles * 8u;
+    const unsigned piece = quotient(u - at, (unsigned)n_tiles), t_first = u - at - piece * (unsigned)n_tiles;
+    const unsigned kvh = m_tiles == 1u ? piece : quotient(piece, m_tiles), m0 = (piece - kvh * m_tiles) * 8u;
     const unsigned n = min((unsigned)n_tiles - t_first, u_end - u);  // tiles of this piece that are ours
     const int p_first = (tile0 + (int)t_first) * S::TILE + (int)warp * S::SUB;                       // this warp's positions of the first
     const int* table = a.tables + (size_t)seq * a.max_blocks;
@@ -541,7 +558,7 @@ __global__ void __launch_bounds__(Split<HD, T>::THREADS, Split<HD, T>::PER_SM) s
     if (in_block == 0 && tid == 0) {
       const bool ends = t_first > 0 && t_first + n == (unsigned)n_tiles;
       const unsigned u0 = u - t_first, each = line[0], more = line[1], big = more * (each + 1u);
-      const unsigned b0 = u0 < big ? u0 / (each + 1u) : more + (u0 - big) / each, b0_begin = b0 * each + min(b0, more);
+      const unsigned b0 = u0 < big ? quotient(u0, each + 1u) : more + quotient(u0 - big, each), b0_begin = b0 * each + min(b0, more);
       a.merges[2u * blockIdx.x] = make_int4((int)b0, ends ? (int)(blockIdx.x - b0 + 1u) : 0, b0_begin == u0 ? 0 : 1, (int)m0);
       a.merges[2u * blockIdx.x + 1u] = make_int4(s.row0, (int)kvh, (int)m_rows, 0);
     }
@@ -552,36 +569,36 @@ __global__ void __launch_bounds__(Split<HD, T>::THREADS, Split<HD, T>::PER_SM) s
 }
 
 // ---- the records of pieces that lie in several blocks ----------------------------------------------------------
-// out = sum_b e_b O_b / sum_b e_b l_b, e_b = exp2(m_b - max m), in the order of the blocks.  A block for each of the split kernel's, for the piece that
-// ends there; its warps are 8 rows x 4 shares of the records.
+// out = sum_b e_b O_b / sum_b e_b l_b, e_b = exp2(m_b - max m), in the order of the blocks.  A block for each of the split kernel's and 64 dims, for the
+// piece that ends there; its threads are 8 rows x 8 shares of the records x 16 times 4 dims.
 template <int HD, typename T>
 __global__ void __launch_bounds__(1024) sdpa_q8_merge_kernel(const ks_sdpa_q8_args a) {
   using S = Split<HD, T>;
-  constexpr int D = HD / 32, V = D == 2 ? 2 : 4;
-  __shared__ float red[3][8][HD], tops[4][8], sums[4][8];
+  __shared__ float4 red[8][8][16];
+  __shared__ float tops[8][8], sums[8][8];
   ks_pdl_entry();
-  const unsigned lane = threadIdx.x & 31u, warp = threadIdx.x >> 5, r = warp & 7u, share = warp >> 3;
+  const unsigned d = threadIdx.x & 15u, r = threadIdx.x >> 4 & 7u, share = threadIdx.x >> 7, dim = blockIdx.y * 64u + 4u * d;
   const int4 job = a.merges[2u * blockIdx.x], where = a.merges[2u * blockIdx.x + 1u];
   const unsigned n = (unsigned)job.y, m = (unsigned)job.w + r;
   if (n == 0u) return;
   const float* rec = a.part + (size_t)job.x * 2u * S::record;
   auto record = [&](unsigned k) { return rec + (k ? k * 2u : (unsigned)job.z) * (size_t)S::record; };  // (the first block's record is its second one unless the piece starts with the block)
   // a share's records four at a time: maxima, sums and values on one trip, then together as a running softmax
-  float top = kNone, l = 0.0f, v[D];
-#pragma unroll
-  for (int d = 0; d < D; d++) v[d] = 0.0f;
+  float top = kNone, l = 0.0f;
+  float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
   const bool live = m < (unsigned)where.z;
   if (live) {
     constexpr unsigned FLY = 4;
-    for (unsigned k0 = share; k0 < n; k0 += 4u * FLY) {
-      float mk[FLY], lk[FLY], o[FLY][D];
+    for (unsigned k0 = share; k0 < n; k0 += 8u * FLY) {
+      float mk[FLY], lk[FLY];
+      float4 o[FLY];
 #pragma unroll
       for (unsigned f = 0; f < FLY; f++) {
-        const bool there = k0 + 4u * f < n;
-        const float* x = record(there ? k0 + 4u * f : k0);
+        const bool there = k0 + 8u * f < n;
+        const float* x = record(there ? k0 + 8u * f : k0);
         mk[f] = there ? x[r] : kNone;
         lk[f] = there ? x[8 + r] : 0.0f;
-        load_dims<D>(x + 16 + r * HD + D * lane, o[f]);
+        o[f] = there ? *reinterpret_cast<const float4*>(x + 16 + r * HD + dim) : make_float4(0.f, 0.f, 0.f, 0.f);
       }
       float most = top;
 #pragma unroll
@@ -589,42 +606,44 @@ __global__ void __launch_bounds__(1024) sdpa_q8_merge_kernel(const ks_sdpa_q8_ar
       const float turn = exp2_fast(top - most);
       top = most;
       l *= turn;
-#pragma unroll
-      for (int d = 0; d < D; d++) v[d] *= turn;
+      v.x *= turn; v.y *= turn; v.z *= turn; v.w *= turn;
 #pragma unroll
       for (unsigned f = 0; f < FLY; f++) {
-        const float e = k0 + 4u * f < n ? exp2_fast(mk[f] - top) : 0.0f;
+        const float e = exp2_fast(mk[f] - top);
         l = fmaf(lk[f], e, l);
-#pragma unroll
-        for (int d = 0; d < D; d++) v[d] = fmaf(o[f][d], e, v[d]);
+        v.x = fmaf(o[f].x, e, v.x);
+        v.y = fmaf(o[f].y, e, v.y);
+        v.z = fmaf(o[f].z, e, v.z);
+        v.w = fmaf(o[f].w, e, v.w);
       }
     }
-    if (lane == 0) {
-      tops[share][r] = top;
-      sums[share][r] = l;
-    }
-    if (share > 0)
-#pragma unroll
-      for (int d = 0; d < D; d++) red[share - 1u][r][d * 32 + lane] = v[d];
   }
+  if (d == 0) {
+    tops[share][r] = top;
+    sums[share][r] = l;
+  }
+  red[share][r][d] = v;
   __syncthreads();
   if (!live || share > 0) return;
-  float most = kNone, e[4];
+  float most = kNone;
 #pragma unroll
-  for (int k = 0; k < 4; k++) most = fmaxf(most, tops[k][r]);
+  for (int k = 0; k < 8; k++) most = fmaxf(most, tops[k][r]);
+  float y[4] = {0.f, 0.f, 0.f, 0.f};
   l = 0.0f;
 #pragma unroll
-  for (int k = 0; k < 4; k++) {
-    e[k] = exp2_fast(tops[k][r] - most);
-    l = fmaf(sums[k][r], e[k], l);
+  for (int k = 0; k < 8; k++) {
+    const float e = exp2_fast(tops[k][r] - most);
+    const float4 o = red[k][r][d];
+    l = fmaf(sums[k][r], e, l);
+    y[0] = fmaf(o.x, e, y[0]);
+    y[1] = fmaf(o.y, e, y[1]);
+    y[2] = fmaf(o.z, e, y[2]);
+    y[3] = fmaf(o.w, e, y[3]);
   }
   const float f = over(l);
-  T* to = (T*)a.out + ((size_t)(where.x + (int)(m / a.G)) * a.n_q + (unsigned)where.y * a.G + m % a.G) * HD + D * lane;
 #pragma unroll
-  for (int d = 0; d < D; d++)
-    v[d] = (v[d] * e[0] + red[0][r][d * 32 + lane] * e[1] + (red[1][r][d * 32 + lane] * e[2] + red[2][r][d * 32 + lane] * e[3])) * f;
-#pragma unroll
-  for (int d = 0; d < D; d += V) put_dims(to + d, v + d, V);
+  for (int k = 0; k < 4; k++) y[k] *= f;
+  put_dims((T*)a.out + ((size_t)(where.x + (int)(m / a.G)) * a.n_q + (unsigned)where.y * a.G + m % a.G) * HD + dim, y, 4);
 }
 
 unsigned split_blocks(const ks_ctx* ctx, size_t hd) { return (unsigned)ctx->sm_count * (hd == 256 ? Split<256, float>::PER_SM : Split<128, float>::PER_SM); }  // as many as run at once
@@ -641,7 +660,7 @@ int launch_split(ks_ctx* ctx, const ks_sdpa_q8_args& a, unsigned blocks) {
   KS_LAUNCH(ctx, (sdpa_q8_split_kernel<HD, T, FP8>), blocks, S::THREADS, S::total, a);
   int rc = ks_after_launch(ctx, "sdpa_paged_q8");
   if (rc || blocks == 1) return rc;
-  KS_LAUNCH(ctx, (sdpa_q8_merge_kernel<HD, T>), blocks, 1024, 0, a);
+  KS_LAUNCH(ctx, (sdpa_q8_merge_kernel<HD, T>), dim3(blocks, HD / 64), 1024, 0, a);
   return ks_after_launch(ctx, "sdpa_paged_q8 merge");
 }
 
@@ -698,7 +717,6 @@ int ks_sdpa_paged_q8(ks_ctx* ctx, const ks_q8_cache* c, const ks_page_tables* t,
   // (a lone sequence that may have many rows needs one kernel only, whatever it has)
   const bool wide = rows_most * G > KS_Q8_FEW, split = !wide || t->n_seqs > 1;
   a.few = !split ? 0u : wide ? KS_Q8_FEW : (unsigned)(rows_most * G);
-  a.least = 1;
   a.bad = (unsigned*)ctx->ws + KS_WS_INDEX_WORD;
   a.n_seqs = (unsigned)t->n_seqs;
   a.max_blocks = (unsigned)t->max_blocks;

@@ -14,7 +14,6 @@ struct ks_sdpa_q8_args {
   unsigned* bad;
   unsigned n_seqs, max_blocks, n_pages, page_log, max_rows, rows_most, n_q, n_kv, G, window;
   unsigned few;              // sequences of up to so many rows (times G) take the split kernel
-  unsigned least;            // units a block takes at least
   float scale;
 };
 
