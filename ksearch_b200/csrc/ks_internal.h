@@ -150,6 +150,7 @@ int ks_launch_matvec_q4k_fx(ks_ctx* ctx, const ks_mv_seg* segs, int n_seg, ks_mv
 #define KS_WS_FENCE_WORD 4001  // cleared behind the load-time quantiser and otherwise unused
 #define KS_WS_INDEX_WORD 4002  // an index in device data was out of range: KS_BAD_*; ks_synchronize reports and clears it
 enum { KS_BAD_PAGE = 1u, KS_BAD_SLOT = 2u, KS_BAD_POSITION = 4u, KS_BAD_ROWS = 8u, KS_BAD_STACK = 16u };
+#define KS_WS_STEP_WORD 4003   // arrivals of a page step's blocks; zero between launches
 #define KS_WS_BYTES 16384
 
 int ks_launch_rmsnorm(ks_ctx* ctx, size_t n, size_t rows, float eps, ks_dtype act, const void* x, const void* w,

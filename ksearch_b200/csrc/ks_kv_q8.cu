@@ -119,17 +119,17 @@ __device__ __forceinline__ void norm_rope(float (&x)[2][V], float inv, const Tur
   }
 }
 
-// Grid: (touched pages x n_kv x 2) blocks of page / kRowsPerWarp warps, K and V of a head next to each other; NORM: in front of them the blocks of the
-// query heads.
+// Grid: (touched pages x n_kv x 2) blocks of page / kRowsPerWarp warps, K and V of a head next to each other; NORM: behind them, which take longer, the blocks of
+// the query heads.
 template <int HD, typename T, bool FP8, bool NORM>
-__global__ void __launch_bounds__(1024) append_q8_kernel(const AppendArgs a, unsigned q_blocks) {
+__global__ void __launch_bounds__(1024) append_q8_kernel(const AppendArgs a) {
   constexpr int V = HD / 64;
   __shared__ float red[32];
   ks_pdl_entry();
   const unsigned lane = threadIdx.x & 31u, warp = threadIdx.x >> 5, nwarp = blockDim.x >> 5;
   const unsigned page = 1u << a.page_log, per_job = 2u * a.n_kv;
-  if (NORM && blockIdx.x < q_blocks) {
-    const unsigned it0 = (blockIdx.x * nwarp + warp) * kHeadsPerWarp, most = a.max_rows * a.n_q;
+  if (NORM && blockIdx.x >= a.n_jobs * per_job) {
+    const unsigned it0 = ((blockIdx.x - a.n_jobs * per_job) * nwarp + warp) * kHeadsPerWarp, most = a.max_rows * a.n_q;
     float x[kHeadsPerWarp][2][V];
     int pos[kHeadsPerWarp];
     const unsigned items = min((unsigned)max(a.plan[1], 0), a.max_rows) * a.n_q;
@@ -160,8 +160,8 @@ __global__ void __launch_bounds__(1024) append_q8_kernel(const AppendArgs a, uns
     }
     return;
   }
-  const unsigned index = blockIdx.x - (NORM ? q_blocks : 0u), j = index / per_job, head = index % per_job >> 1;
-  const bool vals = index & 1u;
+  const unsigned j = blockIdx.x / per_job, head = blockIdx.x % per_job >> 1;
+  const bool vals = blockIdx.x & 1u;
   const int4 job = reinterpret_cast<const int4*>(a.plan + a.at.jobs)[j];
   if (job.x < 0) return;
   const unsigned row0 = (unsigned)job.x, rows = (unsigned)job.y, slot = (unsigned)job.z, off = slot & (page - 1u);
@@ -319,7 +319,7 @@ int launch_append(ks_ctx* ctx, const ks_q8_cache* c, ks_dtype act, const AppendA
   KS_REQUIRE(ctx, blocks < (1u << 31), "%s: too many rows and heads for one launch", who);
   KS_REQUIRE_DEVICE(ctx, who);
   ks_on_device on(ctx);
-#define KS_AP(HD_, T_, F_) KS_LAUNCH(ctx, (append_q8_kernel<HD_, T_, F_, NORM>), (unsigned)blocks, warps * 32, 0, a, (unsigned)q_blocks)
+#define KS_AP(HD_, T_, F_) KS_LAUNCH(ctx, (append_q8_kernel<HD_, T_, F_, NORM>), (unsigned)blocks, warps * 32, 0, a)
 #define KS_AP_T(HD_, F_) do { if (act == KS_F32) KS_AP(HD_, float, F_); else KS_AP(HD_, __half, F_); } while (0)
 #define KS_AP_F(HD_) do { if (c->dtype == KS_E4M3) KS_AP_T(HD_, true); else KS_AP_T(HD_, false); } while (0)
   if (c->hd == 256) KS_AP_F(256);

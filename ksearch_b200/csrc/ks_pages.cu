@@ -1,9 +1,9 @@
 // Pages of a paged cache handed out on the GPU: tables, lengths, the stack of free pages and the plan of a step's rows.
 //
 // A step is integer arithmetic on three exclusive sums over the sequences (rows, new pages, touched pages) and one record per row, so it
-// is bound by latency: one trip for lengths and counts, the sums, one trip for a row's page, the stores.  Many rows are shared by the blocks
-// of one cluster: each makes the sums for itself and takes rows; nothing that a block reads is written by another, except lengths and
-// the stack's count, which block 0 writes behind the cluster's barrier (all have read them by then).
+// is bound by latency: one trip for lengths and counts, the sums, one trip for a row's page, the stores.  Every block makes the sums
+// for itself and takes rows; nothing that a block reads is written by another, except lengths and the stack's count, which the block that
+// arrived last at a counter writes in the end (every block arrives when it has read them; nobody waits for what the counter says).
 #include "ks_q8.h"
 
 namespace {
@@ -12,7 +12,7 @@ struct TablesArgs {
   unsigned n_seqs, max_blocks, n_pages, page_log, max_rows;
   int *lens, *tables, *free_pages, *plan;
   ks_plan_layout at;
-  unsigned* bad;
+  unsigned *bad, *arrived;
 };
 
 // Exclusive sums of three counts over the block's threads (a multiple of 32, up to 1024); totals in tot.
@@ -43,13 +43,12 @@ __device__ __forceinline__ void scan3(unsigned (&v)[3], unsigned (&tot)[3], unsi
   }
 }
 
-constexpr unsigned kCluster = 8;
 // A thread takes four neighbouring rows: one search for the sequence of the first, 16-byte stores.
-template <bool CLUSTER>
-__device__ __forceinline__ void step_rows(const TablesArgs& a, const int* n_new) {
+__global__ void __launch_bounds__(1024) pages_step_kernel(const TablesArgs a, const int* n_new) {
   __shared__ unsigned red[32][3];
   __shared__ unsigned first_row[KS_PAGES_MAX_SEQS + 1], first_page[KS_PAGES_MAX_SEQS], first_job[KS_PAGES_MAX_SEQS];
   __shared__ int len_of[KS_PAGES_MAX_SEQS], worst_s;
+  __shared__ bool last;
   const unsigned tid = threadIdx.x, page = 1u << a.page_log, cap = a.max_blocks << a.page_log;
   if (tid == 0) worst_s = 0;
   ks_pdl_entry();
@@ -83,7 +82,11 @@ __device__ __forceinline__ void step_rows(const TablesArgs& a, const int* n_new)
   }
   if (tid == 0) first_row[a.n_seqs] = rows;
   __syncthreads();
-  if (CLUSTER) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");  // lengths and count have been read by this block
+  unsigned before_me = 0;  // thread 0: blocks that have arrived, once all of this one have read lengths and count
+  if (tid == 0 && gridDim.x > 1u) {
+    __threadfence();
+    before_me = atomicAdd(a.arrived, 1u);
+  }
   const unsigned step = gridDim.x * blockDim.x, quads = (a.max_rows + 3u) >> 2, me = blockIdx.x * blockDim.x + tid;
   int4 *seqs = reinterpret_cast<int4*>(a.plan + a.at.row_seq), *poss = reinterpret_cast<int4*>(a.plan + a.at.row_pos), *slots = reinterpret_cast<int4*>(a.plan + a.at.row_slot);
   for (unsigned q = me; q < quads; q += step) {
@@ -130,13 +133,17 @@ __device__ __forceinline__ void step_rows(const TablesArgs& a, const int* n_new)
       a.plan[tid] = tid < 4u ? head[tid] : 0;
     }
     if (tid == 0) a.plan[a.at.row_start + a.n_seqs] = (int)rows;
-    if (CLUSTER) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+  }
+  if (tid == 0) last = before_me == gridDim.x - 1u;
+  __syncthreads();
+  if (last) {
     if (tid < a.n_seqs && !worst) a.lens[tid] = (int)after;
-    if (tid == 0 && !worst) a.free_pages[0] = count - (int)tot[1];
+    if (tid == 0) {
+      if (!worst) a.free_pages[0] = count - (int)tot[1];
+      if (gridDim.x > 1u) *a.arrived = 0u;
+    }
   }
 }
-__global__ void __launch_bounds__(1024) pages_step_kernel(const TablesArgs a, const int* n_new) { step_rows<false>(a, n_new); }
-__global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(1024) pages_step_cluster_kernel(const TablesArgs a, const int* n_new) { step_rows<true>(a, n_new); }
 
 // One block: the sum over the sequences, then one page per thread and step.
 __global__ void __launch_bounds__(1024) pages_trim_kernel(const TablesArgs a, const int* keep) {
@@ -203,6 +210,7 @@ TablesArgs args_of(ks_ctx* ctx, const ks_page_tables* t) {
   a.plan = (int*)t->plan->dptr;
   a.at = ks_plan_parts(t->n_seqs, t->max_rows, t->page);
   a.bad = (unsigned*)ctx->ws + KS_WS_INDEX_WORD;
+  a.arrived = (unsigned*)ctx->ws + KS_WS_STEP_WORD;
   return a;
 }
 unsigned round32(size_t n) { return (unsigned)((n + 31) & ~size_t(31)); }
@@ -255,14 +263,9 @@ int ks_pages_step(ks_ctx* ctx, const ks_page_tables* t, const ks_buf* n_new) {
   KS_REQUIRE(ctx, ks_fits(n_new, 0, t->n_seqs * 4) && ks_aligned(n_new, 4), "pages_step: n_new buffer too small or not on 4 bytes");
   KS_REQUIRE_DEVICE(ctx, "pages_step");
   ks_on_device on(ctx);
-  // a thread four rows: one block up to 2048 of them, else a cluster
-  if (t->max_rows > 2048) {
-    const unsigned threads = t->n_seqs > 512 || t->max_rows > 4 * 512 * kCluster ? 1024 : 512;
-    KS_LAUNCH(ctx, pages_step_cluster_kernel, kCluster, threads, 0, args_of(ctx, t), (const int*)n_new->dptr);
-  } else {
-    const size_t most = t->n_seqs > t->max_rows / 4 ? t->n_seqs : t->max_rows / 4;
-    KS_LAUNCH(ctx, pages_step_kernel, 1, round32(most) < 128u ? 128u : round32(most), 0, args_of(ctx, t), (const int*)n_new->dptr);
-  }
+  const unsigned threads = round32(t->n_seqs) < 256u ? (t->max_rows <= 512 && t->n_seqs <= 128 ? 128 : 256) : round32(t->n_seqs);
+  const size_t blocks = (t->max_rows + 4 * threads - 1) / (4 * threads), most = 64;
+  KS_LAUNCH(ctx, pages_step_kernel, (unsigned)(blocks < most ? blocks : most), threads, 0, args_of(ctx, t), (const int*)n_new->dptr);
   return ks_after_launch(ctx, "pages_step");
 }
 

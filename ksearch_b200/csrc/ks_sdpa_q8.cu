@@ -570,14 +570,14 @@ __global__ void __launch_bounds__(Split<HD, T>::THREADS, Split<HD, T>::PER_SM) s
 
 // ---- the records of pieces that lie in several blocks ----------------------------------------------------------
 // out = sum_b e_b O_b / sum_b e_b l_b, e_b = exp2(m_b - max m), in the order of the blocks.  A block for each of the split kernel's and 64 dims, for the
-// piece that ends there; its threads are 8 rows x 8 shares of the records x 16 times 4 dims.
+// piece that ends there; its threads are 8 rows x (up to 8) shares of the records x 16 times 4 dims.
 template <int HD, typename T>
 __global__ void __launch_bounds__(1024) sdpa_q8_merge_kernel(const ks_sdpa_q8_args a) {
   using S = Split<HD, T>;
   __shared__ float4 red[8][8][16];
   __shared__ float tops[8][8], sums[8][8];
   ks_pdl_entry();
-  const unsigned d = threadIdx.x & 15u, r = threadIdx.x >> 4 & 7u, share = threadIdx.x >> 7, dim = blockIdx.y * 64u + 4u * d;
+  const unsigned d = threadIdx.x & 15u, r = threadIdx.x >> 4 & 7u, share = threadIdx.x >> 7, shares = blockDim.x >> 7, dim = blockIdx.y * 64u + 4u * d;
   const int4 job = a.merges[2u * blockIdx.x], where = a.merges[2u * blockIdx.x + 1u];
   const unsigned n = (unsigned)job.y, m = (unsigned)job.w + r;
   if (n == 0u) return;
@@ -589,13 +589,13 @@ __global__ void __launch_bounds__(1024) sdpa_q8_merge_kernel(const ks_sdpa_q8_ar
   const bool live = m < (unsigned)where.z;
   if (live) {
     constexpr unsigned FLY = 4;
-    for (unsigned k0 = share; k0 < n; k0 += 8u * FLY) {
+    for (unsigned k0 = share; k0 < n; k0 += shares * FLY) {
       float mk[FLY], lk[FLY];
       float4 o[FLY];
 #pragma unroll
       for (unsigned f = 0; f < FLY; f++) {
-        const bool there = k0 + 8u * f < n;
-        const float* x = record(there ? k0 + 8u * f : k0);
+        const bool there = k0 + shares * f < n;
+        const float* x = record(there ? k0 + shares * f : k0);
         mk[f] = there ? x[r] : kNone;
         lk[f] = there ? x[8 + r] : 0.0f;
         o[f] = there ? *reinterpret_cast<const float4*>(x + 16 + r * HD + dim) : make_float4(0.f, 0.f, 0.f, 0.f);
@@ -626,12 +626,10 @@ __global__ void __launch_bounds__(1024) sdpa_q8_merge_kernel(const ks_sdpa_q8_ar
   __syncthreads();
   if (!live || share > 0) return;
   float most = kNone;
-#pragma unroll
-  for (int k = 0; k < 8; k++) most = fmaxf(most, tops[k][r]);
+  for (unsigned k = 0; k < shares; k++) most = fmaxf(most, tops[k][r]);
   float y[4] = {0.f, 0.f, 0.f, 0.f};
   l = 0.0f;
-#pragma unroll
-  for (int k = 0; k < 8; k++) {
+  for (unsigned k = 0; k < shares; k++) {
     const float e = exp2_fast(tops[k][r] - most);
     const float4 o = red[k][r][d];
     l = fmaf(sums[k][r], e, l);
@@ -660,7 +658,9 @@ int launch_split(ks_ctx* ctx, const ks_sdpa_q8_args& a, unsigned blocks) {
   KS_LAUNCH(ctx, (sdpa_q8_split_kernel<HD, T, FP8>), blocks, S::THREADS, S::total, a);
   int rc = ks_after_launch(ctx, "sdpa_paged_q8");
   if (rc || blocks == 1) return rc;
-  KS_LAUNCH(ctx, (sdpa_q8_merge_kernel<HD, T>), dim3(blocks, HD / 64), 1024, 0, a);
+  // many pieces lie in two or three blocks each: small blocks, so that all are there at once
+  const size_t pieces = (size_t)a.n_seqs * a.n_kv * ((a.few + 7u) / 8u);
+  KS_LAUNCH(ctx, (sdpa_q8_merge_kernel<HD, T>), dim3(blocks, HD / 64), pieces >= blocks / 4 ? 256 : 1024, 0, a);
   return ks_after_launch(ctx, "sdpa_paged_q8 merge");
 }
 
