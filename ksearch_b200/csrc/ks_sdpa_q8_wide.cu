@@ -27,15 +27,15 @@ template <int HD_, typename T_>
 struct Wide {
   static constexpr int HD = HD_, TERMS = sizeof(T_) == 4 ? 2 : 1;
   static constexpr int QT = TERMS == 1 && HD <= 128 ? 2 : 1, ROWS = QT * kRows;  // tiles of query rows a block takes
-  static constexpr int TILE = HD == 256 || QT == 2 ? 64 : 128, GROUPS = TILE / 16, COLS = TILE / (QT == 2 ? 1 : 2);
-  static constexpr int NK = 2, NV = HD == 256 ? 1 : 2;                            // buffers of converted K and V
-  static constexpr int RING = HD == 256 || (HD == 128 && TERMS == 2) ? 2 : 4;     // tiles of codes
+  static constexpr int TILE = HD == 256 ? 64 : 128, GROUPS = TILE / 16, COLS = TILE / 2;  // (a softmax thread has COLS positions in registers at a time)
+  static constexpr int NK = 2, NV = HD == 256 || (HD == 128 && QT == 2) ? 1 : 2;                            // buffers of converted K and V
+  static constexpr int RING = HD == 64 ? 4 : 2;     // tiles of codes
   // The loader of K is RING tiles ahead of its converters at most, those NK ahead of the products and the softmax warps one behind those: a tile's scales are
   // read before their place comes again
   static constexpr int SCALES = RING == 2 ? 6 : 8;
   static_assert(SCALES >= RING + NK + 2 && SCALES <= 8, "scales");
   static constexpr int CONV_K = TERMS == 1 ? 4 : 2, CONV_V = CONV_K, WARPS = kWork + CONV_K + CONV_V + 4, THREADS = WARPS * 32;
-  static constexpr int R_WORK = TERMS == 1 ? 128 : 208, R_CONV = TERMS == 1 ? 80 : 64, R_REST = TERMS == 1 ? 64 : 32;
+  static constexpr int R_WORK = TERMS == 1 ? 136 : 208, R_CONV = TERMS == 1 ? 72 : 64, R_REST = TERMS == 1 ? 56 : 32;
   static_assert(kWork * 32 * R_WORK + (CONV_K + CONV_V) * 32 * R_CONV + 128 * R_REST <= THREADS * (65536 / THREADS / 8 * 8), "registers: the shares fit the launch");
   // shared memory: barriers, the tensor-memory address and the failure flag; per row: scale, maxima of its two threads; per 16 positions: the score's
   // factor, what is added to it, the probability's factor, the sum's
@@ -46,8 +46,9 @@ struct Wide {
   static_assert(q % 128 == 0 && (TERMS == 1 || q_bytes <= (NK + NV) * kv_bytes), "q's first term passes through K's and V's place");
   static constexpr unsigned OP = HD + 2;
   static_assert(ROWS * OP * 4 <= total - q && total <= 232448, "the result fits the operands, and all of it a block");
-  // tensor memory: scores, probabilities (two terms), O, of each row tile; q's first term
-  static constexpr unsigned t_s = 0, t_p = t_s + TILE, t_o = t_p + TERMS * TILE / 2, t_tile = t_o + HD, t_q = QT * t_tile;
+  // tensor memory: scores, probabilities (two terms), O, of each row tile; q's first term.  Two row tiles fill it (HD = 128) with the probabilities
+  // in the place of the scores' second half
+  static constexpr unsigned t_s = 0, t_p = QT == 2 ? t_s + TILE / 2 : t_s + TILE, t_o = QT == 2 ? t_s + TILE : t_p + TERMS * TILE / 2, t_tile = t_o + HD, t_q = QT * t_tile;
   static_assert(t_q + (TERMS == 2 ? HD / 2 : 0) <= 512, "tensor memory");
   static constexpr unsigned record = ROWS * (HD + 2);  // floats: m[ROWS], l[ROWS], O[ROWS][HD]
 };
@@ -333,28 +334,42 @@ __global__ void __launch_bounds__(Wide<HD, T>::THREADS, 1) sdpa_q8_wide_kernel(c
       uint32_t r[COLS / 16][16];
       float top = kNone;
       const float4* scale = reinterpret_cast<const float4*>(smem + W::scale) + i % W::SCALES * W::GROUPS + half * (W::GROUPS / 2);
-      if (ok) {
-        tc_fence_after();
+      const int p0 = t_begin + (int)i * W::TILE + (int)half * COLS;
+      // scores from column c0 on, masked; (with two row tiles a thread has the whole row: its halves one after the other)
+      auto fetch = [&](unsigned c0) {
 #pragma unroll
-        for (int c = 0; c < COLS / 16; c++) tc_ld16(tlane + W::t_s + half * COLS + 16u * c, r[c]);
+        for (int c = 0; c < COLS / 16; c++) tc_ld16(tlane + W::t_s + half * COLS + c0 + 16u * c, r[c]);
 #pragma unroll
         for (int c = 0; c < COLS / 16; c++) tc_wait_ld16(r[c]);
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) arrive1(bar(B_S_FREE + qt));
-        const int p0 = t_begin + (int)i * W::TILE + (int)half * COLS;
-        if (!__all_sync(0xffffffffu, lo <= p0 && hi >= p0 + COLS - 1)) {
+        const int p = p0 + (int)c0;
+        if (!__all_sync(0xffffffffu, lo <= p && hi >= p + COLS - 1)) {
 #pragma unroll
           for (int c = 0; c < COLS; c++)
-            if (p0 + c < lo || p0 + c > hi) r[c / 16][c % 16] = 0xFF800000u;  // -infinity
+            if (p + c < lo || p + c > hi) r[c / 16][c % 16] = 0xFF800000u;  // -infinity
         }
+      };
+      auto largest = [&](unsigned c0) {
 #pragma unroll
         for (int c = 0; c < COLS / 16; c++) {
           float g = __uint_as_float(r[c][0]);
 #pragma unroll
           for (int e = 1; e < 16; e++) g = fmaxf(g, __uint_as_float(r[c][e]));
-          const float2 sc = *reinterpret_cast<const float2*>(scale + c);
+          const float2 sc = *reinterpret_cast<const float2*>(scale + c0 / 16u + c);
           top = fmaxf(top, fmaf(g, factor(sc.x), sc.y));
+        }
+      };
+      if (ok) {
+        tc_fence_after();
+        fetch(0);
+        if constexpr (W::QT == 1) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) arrive1(bar(B_S_FREE + qt));
+        }
+        largest(0);
+        if constexpr (W::QT == 2) {
+          fetch(COLS);
+          largest(COLS);
         }
       }
       float turn = 1.0f;
@@ -380,6 +395,47 @@ __global__ void __launch_bounds__(Wide<HD, T>::THREADS, 1) sdpa_q8_wide_kernel(c
         l *= turn;
         turned = true;
       }
+      if constexpr (W::QT == 2) {
+        auto put = [&](unsigned c0) {  // probabilities of the half in registers
+#pragma unroll
+          for (int c = 0; c < COLS / 16; c++) {
+            const float4 sc = scale[c0 / 16u + c];
+            const float d = sc.y - ref;
+            const uint64_t ff = pair(sc.x, sc.x), dd = pair(d, d);
+            uint64_t sum = 0;
+            uint32_t w[8];
+#pragma unroll
+            for (int e = 0; e < 16; e += 2) {
+              const float2 y = apart(fma2(pair(__uint_as_float(r[c][e]), __uint_as_float(r[c][e + 1])), ff, dd));
+              const float y0 = exp2_fast(y.x), y1 = exp2_fast(y.y);
+              sum = add2(sum, pair(y0, y1));
+              w[e / 2] = q8_u32(__floats2half2_rn(y0, y1));  // (V's scale is in the exponent)
+            }
+            const float2 t = apart(sum);
+            l = fmaf(t.x + t.y, sc.w, l);
+            tc_st8(tlane + W::t_p + c0 / 2u + 8u * c, w);
+          }
+        };
+        // the half in registers first: its probabilities and the others' lie where its scores were.  (The scores are there: so the values of the
+        // tile before are done, and O may be touched)
+        put(COLS);
+        fetch(0);
+        put(0);
+        if (turned && i > 0) {
+#pragma unroll 1
+          for (unsigned c = 0; c < HALF; c += 8u) {
+            uint32_t o[8];
+            tc_ld8(tlane + W::t_o + c, o);
+#pragma unroll
+            for (int e = 0; e < 8; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * turn);
+            tc_st8(tlane + W::t_o + c, o);
+          }
+        }
+        tc_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) arrive1(bar(B_P_FULL + qt));
+      } else {
       uint32_t pl[W::TERMS == 2 ? COLS / 2 : 1];
 #pragma unroll
       for (int c = 0; c < COLS / 16; c++) {
@@ -426,9 +482,6 @@ __global__ void __launch_bounds__(Wide<HD, T>::THREADS, 1) sdpa_q8_wide_kernel(c
           }
         }
       }
-      if constexpr (W::QT == 2) {
-        if (!ok) break;
-      }
       if (ok) {
 #pragma unroll
         for (int c = 0; c < COLS / 16; c++) {
@@ -443,6 +496,7 @@ __global__ void __launch_bounds__(Wide<HD, T>::THREADS, 1) sdpa_q8_wide_kernel(c
         tc_fence_before();
         __syncwarp();
         if (lane == 0) arrive1(bar(B_P_FULL + qt));
+      }
       }
     }
     if (my_tiles) ok = ok && __all_sync(0xffffffffu, mb_wait(bar(B_PV_DONE + qt), (n_tiles - 1u) & 1u, kWait));
@@ -556,7 +610,7 @@ __global__ void __launch_bounds__(Wide<HD, T>::THREADS, 1) sdpa_q8_wide_kernel(c
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(W::R_REST));
     if (warp == MMA_WARP) {
-      // ---- products: scores of the next tile in front of the values of this one, row tile after row tile
+      // ---- products
       const unsigned leader = elect_one(), tiles = __reduce_max_sync(0xffffffffu, n_tiles), qts = __reduce_max_sync(0xffffffffu, q_tiles);
       constexpr uint32_t idesc_s = (1u << 4) | ((W::TILE >> 3) << 17) | ((kRows >> 4) << 24), idesc_o = (1u << 4) | ((HD >> 3) << 17) | ((kRows >> 4) << 24);
       auto wait = [&](unsigned b, unsigned parity) { return __all_sync(0xffffffffu, mb_wait(bar(b), parity & 1u, kWait)); };
@@ -583,8 +637,8 @@ __global__ void __launch_bounds__(Wide<HD, T>::THREADS, 1) sdpa_q8_wide_kernel(c
 #pragma unroll
         for (unsigned t = 0; t < W::QT; t++) {
           if (!ok || t >= qts) continue;
-          if (i + 1u < tiles) {
-            ok = (t || wait(B_K_FULL + (i + 1u) % W::NK, (i + 1u) / W::NK)) && wait(B_S_FREE + t, i);
+          if (W::QT == 1 && i + 1u < tiles) {  // the next scores in front of these values
+            ok = wait(B_K_FULL + (i + 1u) % W::NK, (i + 1u) / W::NK) && wait(B_S_FREE, i);
             if (!ok) continue;
             tc_fence_after();
             scores(i + 1u, t);
@@ -604,6 +658,12 @@ __global__ void __launch_bounds__(Wide<HD, T>::THREADS, 1) sdpa_q8_wide_kernel(c
           }
           commit_if(leader, base + 8u * (B_PV_DONE + t));
           if (t + 1u == qts) commit_if(leader, base + 8u * (B_V_FREE + i % W::NV));
+          if (W::QT == 2 && i + 1u < tiles) {  // behind them: they take the probabilities' place.  Meanwhile the other row tile's softmax runs
+            ok = (t || wait(B_K_FULL + (i + 1u) % W::NK, (i + 1u) / W::NK)) && wait(B_PV_DONE + t, i);
+            if (!ok) continue;
+            tc_fence_after();
+            scores(i + 1u, t);
+          }
         }
       }
       if (leader) {  // every product issued must finish before shared and tensor memory go away (bounded)
