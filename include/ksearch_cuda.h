@@ -219,15 +219,15 @@ int ks_sdpa_decode(ks_ctx* ctx, size_t n_slots, size_t n_q, size_t n_kv, size_t 
  * tables and plans live on the device, so one captured step serves every length.
  *
  * Index errors in device data (a table entry outside the pool, a slot outside the cache, a row the RoPE table does not
- * reach, more rows of a sequence than rows_most) touch nothing out of range: the rows concerned are left out and the next
- * ks_synchronize returns KS_ERR_INVALID. */
+ * reach, more rows of a sequence than rows_most) touch nothing out of range: the rows concerned are left out (an attention row
+ * that sees a page of no such number gets some result) and the next ks_synchronize returns KS_ERR_INVALID. */
 #define KS_PAGES_MAX_SEQS 1024
 #define KS_PAGES_PLAN_HEADER 8
 typedef struct {
   size_t n_seqs;      /* sequences, 1..KS_PAGES_MAX_SEQS */
   size_t max_blocks;  /* pages a sequence may hold */
   size_t n_pages;     /* pages of the pool */
-  size_t page;        /* positions of a page: 16, 32, 64 or 128; n_pages * page and max_blocks * page below 2^31 */
+  size_t page;        /* positions of a page: 16, 32, 64 or 128; n_pages * page below 2^31, max_blocks * page below 2^30 */
   size_t max_rows;    /* new rows of one step, all sequences together: 1..2^20 */
   ks_buf* lens;       /* int32 [n_seqs]: positions a sequence holds */
   ks_buf* tables;     /* int32 [n_seqs, max_blocks]: its pages, -1 behind them */
@@ -278,7 +278,8 @@ int ks_kv_read_q8(ks_ctx* ctx, const ks_q8_cache* c, size_t n_rows, const ks_buf
  * max(0, p - window + 1) .. p (window 0: all up to p), so the lengths are those AFTER the step; a row that sees none gets zeros.  Scores are
  * scale * (q . k).  Only row_start, the lengths and the tables are read: a host may write its own.  rows_most: no sequence has
  * more rows (0: nothing is done); ctx_most: the longest context to expect (a hint for how the work is split).  Rows behind the last
- * sequence are left as they are.  tmp: ks_sdpa_paged_tmp_floats() f32, not shared with work that may overlap. */
+ * sequence are left as they are.  tmp: ks_sdpa_paged_tmp_floats() f32, not shared with work that may overlap.  n_seqs, max_blocks and
+ * n_kv together have a limit (KS_ERR_UNSUPPORTED): n_seqs * n_kv * max_blocks * page below 2^36. */
 size_t ks_sdpa_paged_tmp_floats(const ks_ctx* ctx, const ks_q8_cache* c, const ks_page_tables* t, size_t n_q, size_t rows_most);
 int ks_sdpa_paged_q8(ks_ctx* ctx, const ks_q8_cache* c, const ks_page_tables* t, size_t n_q, size_t rows_most, size_t ctx_most, size_t window,
                      float scale, ks_dtype act, const ks_buf* q, ks_buf* tmp, ks_buf* out);

@@ -13,7 +13,6 @@
 
 namespace {
 
-constexpr int kRowsPerWarp = 4;  // rows of a page a warp keeps in registers between their maximum and their codes
 constexpr int kHeadsPerWarp = 2;  // (row, query head) pairs of a warp
 
 struct AppendArgs {
@@ -107,7 +106,7 @@ __device__ __forceinline__ float norm_of(const float (&x)[2][V], float eps) {
 #pragma unroll
   for (int e = 0; e < V; e++) ss = fmaf(x[0][e], x[0][e], fmaf(x[1][e], x[1][e], ss));
   ss = q8_warp_sum(ss);
-  return 1.0f / sqrtf(ss / (float)HD + eps);
+  return rsqrtf(fmaf(ss, 1.0f / HD, eps));
 }
 template <int V>
 __device__ __forceinline__ void norm_rope(float (&x)[2][V], float inv, const Turn<V>& t) {
@@ -119,9 +118,58 @@ __device__ __forceinline__ void norm_rope(float (&x)[2][V], float inv, const Tur
   }
 }
 
-// Grid: (touched pages x n_kv x 2) blocks of page / kRowsPerWarp warps, K and V of a head next to each other; NORM: behind them, which take longer, the blocks of
+// The same for what is rounded to codes, as sums of two floats: a value that single ones move across the middle between two codes would be a whole step
+// off (one in 2^20 of them).  Error terms of products by fma, of sums by the usual six operations.  All values of 2048 rows of 2 KV heads take
+// 4.7 us more this way: the append makes only those rows so that need it.
+struct Two {
+  float hi, lo;
+};
+__device__ __forceinline__ Two times(Two a, float b) {
+  const float p = __fmul_rn(a.hi, b);
+  return {p, __fmaf_rn(a.lo, b, __fmaf_rn(a.hi, b, -p))};
+}
+__device__ __forceinline__ Two plus(Two a, Two b) {
+  const float s = __fadd_rn(a.hi, b.hi), t = __fsub_rn(s, a.hi);
+  return {s, __fadd_rn(__fadd_rn(__fsub_rn(a.hi, __fsub_rn(s, t)), __fsub_rn(b.hi, t)), __fadd_rn(a.lo, b.lo))};
+}
+// Rounded to one float toward the odd neighbour, so that rounding it again to 8 bits, and comparing it with a limit, give what the sum gives.
+__device__ __forceinline__ float to_odd(Two x) {
+  const float f = __fadd_rn(x.hi, x.lo), rest = __fsub_rn(x.lo, __fsub_rn(f, x.hi));
+  const uint32_t b = __float_as_uint(f);
+  if (rest == 0.0f || (b & 1u) || !(fabsf(f) < INFINITY) || f == 0.0f) return f;
+  return __uint_as_float((rest > 0.0f) == (f > 0.0f) ? b + 1u : b - 1u);
+}
+// 1 / sqrt(mean of squares + eps): the hardware's approximation r, and one Newton step r / 2 (1 - m r^2) as the second term.
+template <int HD, int V>
+__device__ __forceinline__ Two norm_of_two(const float (&x)[2][V], float eps) {
+  Two ss = {0.0f, 0.0f};
+#pragma unroll
+  for (int e = 0; e < 2 * V; e++) {
+    const float y = x[e / V][e % V];
+    ss = plus(ss, times(Two{y, 0.0f}, y));
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) ss = plus(ss, Two{__shfl_xor_sync(0xffffffffu, ss.hi, o), __shfl_xor_sync(0xffffffffu, ss.lo, o)});
+  const Two m = plus(Two{ss.hi * (1.0f / HD), ss.lo * (1.0f / HD)}, Two{eps, 0.0f});
+  const float r = rsqrtf(m.hi);
+  const Two r2 = times(Two{r, 0.0f}, r), mr2 = times(r2, m.hi);
+  const float rest = __fsub_rn(__fsub_rn(1.0f, mr2.hi), __fmaf_rn(r2.hi, m.lo, mr2.lo)), step = 0.5f * r * rest, hi = __fadd_rn(r, step);
+  return {hi, __fsub_rn(step, __fsub_rn(hi, r))};
+}
+template <int V>
+__device__ __forceinline__ void norm_rope_two(float (&x)[2][V], Two inv, const Turn<V>& t) {
+#pragma unroll
+  for (int e = 0; e < V; e++) {
+    const Two a = times(times(inv, x[0][e]), t.w0[e]), b = times(times(inv, x[1][e]), t.w1[e]);
+    x[0][e] = to_odd(plus(times(a, t.c[e]), times(b, -t.s[e])));
+    x[1][e] = to_odd(plus(times(a, t.s[e]), times(b, t.c[e])));
+  }
+}
+
+// Grid: (touched pages x n_kv x 2) blocks of page / ROWS warps, each of which keeps ROWS rows in registers between
+// their maximum and their codes; K and V of a head next to each other.  NORM: behind them, which take longer, the blocks of
 // the query heads.
-template <int HD, typename T, bool FP8, bool NORM>
+template <int HD, typename T, bool FP8, bool NORM, int ROWS>
 __global__ void __launch_bounds__(1024) append_q8_kernel(const AppendArgs a) {
   constexpr int V = HD / 64;
   __shared__ float red[32];
@@ -177,42 +225,83 @@ __global__ void __launch_bounds__(1024) append_q8_kernel(const AppendArgs a) {
   float* scale_at = (vals ? a.vs : a.ks) + block;
   const float held = off ? q8_scale(*scale_at) : 0.0f;
   const T* src = (const T*)(vals ? a.v : a.k) + (size_t)row0 * a.kv_ld + (size_t)head * HD + lane * V;
-  float x[kRowsPerWarp][2][V], amax = 0.0f;
-#pragma unroll
-  for (int i = 0; i < kRowsPerWarp; i++) {
+  float x[ROWS][2][V], amax = 0.0f;
+  auto fetch = [&](int i) {
     const unsigned r = warp + (unsigned)i * nwarp;
-    if (r >= rows) continue;
     load_act<V, T>(src + (size_t)r * a.kv_ld, x[i][0]);
     load_act<V, T>(src + (size_t)r * a.kv_ld + HD / 2, x[i][1]);
-  }
-#pragma unroll
-  for (int i = 0; i < kRowsPerWarp; i++) {
+  };
+  auto turned = [&](int i, bool fine) {  // a fetched row behind its norm and RoPE, in f32 or as sums of two
     const unsigned r = warp + (unsigned)i * nwarp;
-    if (r >= rows) continue;
-    if constexpr (NORM) {
-      const float inv = norm_of<HD, V>(x[i], a.eps);
-      if (vals) {
+    Turn<V> t;
+    if (!vals) load_turn<HD, V, T>(t, (const T*)a.kw + lane * V, a.rope + (size_t)((unsigned)job.w + r) * HD + lane * V);
+    if (fine) {
+      const Two inv = norm_of_two<HD, V>(x[i], a.eps);
+      if (!vals) return norm_rope_two<V>(x[i], inv, t);
 #pragma unroll
-        for (int e = 0; e < 2 * V; e++) x[i][e / V][e % V] *= inv;
-      } else {
-        Turn<V> t;
-        load_turn<HD, V, T>(t, (const T*)a.kw + lane * V, a.rope + (size_t)((unsigned)job.w + r) * HD + lane * V);
-        norm_rope<V>(x[i], inv, t);
-      }
+      for (int e = 0; e < 2 * V; e++) x[i][e / V][e % V] = to_odd(times(inv, x[i][e / V][e % V]));
+    } else {
+      const float inv = norm_of<HD, V>(x[i], a.eps);
+      if (!vals) return norm_rope<V>(x[i], inv, t);
+#pragma unroll
+      for (int e = 0; e < 2 * V; e++) x[i][e / V][e % V] *= inv;
     }
+  };
+  auto finite_most = [&](int i) {  // the largest finite value of a row's piece; NaN becomes 0
+    float most = 0.0f, odd = 0.0f;
 #pragma unroll
     for (int e = 0; e < 2 * V; e++) {
-      float& y = x[i][e / V][e % V];
-      const float m = fabsf(y);
-      if (m < INFINITY) amax = fmaxf(amax, m);
-      if (y != y) y = 0.0f;
+      const float y = x[i][e / V][e % V];
+      most = fmaxf(most, fabsf(y));
+      odd = fmaf(y, 0.0f, odd);
     }
-  }
+    if (odd != 0.0f) {  // an infinity or NaN among them
+      most = 0.0f;
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-  if (lane == 0) red[warp] = amax;
-  __syncthreads();
-  for (unsigned w = 0; w < nwarp; w++) amax = fmaxf(amax, red[w]);
+      for (int e = 0; e < 2 * V; e++) {
+        float& y = x[i][e / V][e % V];
+        if (y != y) y = 0.0f;
+        if (fabsf(y) < INFINITY) most = fmaxf(most, fabsf(y));
+      }
+    }
+    return most;
+  };
+  auto largest = [&] {  // of the block
+    amax = 0.0f;
+#pragma unroll
+    for (int i = 0; i < ROWS; i++)
+      if (warp + (unsigned)i * nwarp < rows) amax = fmaxf(amax, finite_most(i));
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+    if (lane == 0) red[warp] = amax;
+    __syncthreads();
+    amax = lane < nwarp ? red[lane] : 0.0f;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+  };
+#pragma unroll
+  for (int i = 0; i < ROWS; i++)
+    if (warp + (unsigned)i * nwarp < rows) fetch(i);
+  if constexpr (NORM)
+#pragma unroll
+    for (int i = 0; i < ROWS; i++)
+      if (warp + (unsigned)i * nwarp < rows) turned(i, false);
+  largest();
+  // f32 leaves a value off by a dozen roundings of its pair at most.  A maximum that near to a limit, and a row with a value that near to the middle
+  // between two codes, is made again as sums of two floats
+  constexpr float DOUBT = 0x1p-20f;
+  bool fine = false;
+  if (NORM && q8_scale_for<FP8>(amax * (1.0f - 2.0f * DOUBT)) != q8_scale_for<FP8>(amax * (1.0f + 2.0f * DOUBT))) {
+    fine = true;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < ROWS; i++)
+      if (warp + (unsigned)i * nwarp < rows) {
+        fetch(i);
+        turned(i, true);
+      }
+    largest();
+  }
   const float s = fmaxf(q8_scale_for<FP8>(amax), q8_power_above(held)), inv = 1.0f / s;  // (powers of two: exact)
   uint8_t* codes = (vals ? a.vc : a.kc) + (block << a.page_log) * HD;
   if (off && s != held) {  // the page's earlier rows under the larger scale
@@ -225,9 +314,28 @@ __global__ void __launch_bounds__(1024) append_q8_kernel(const AppendArgs a) {
     }
   }
 #pragma unroll
-  for (int i = 0; i < kRowsPerWarp; i++) {
+  for (int i = 0; i < ROWS; i++) {
     const unsigned r = warp + (unsigned)i * nwarp;
     if (r >= rows) continue;
+    if (NORM && !fine) {
+      uint32_t differ = 0;
+      float lo[2][V], hi[2][V];
+#pragma unroll
+      for (int e = 0; e < V; e++) {
+        const float y0 = x[i][0][e] * inv, y1 = x[i][1][e] * inv, both = fabsf(y0) + fabsf(y1), d0 = DOUBT * (vals ? fabsf(y0) : both), d1 = DOUBT * (vals ? fabsf(y1) : both);
+        lo[0][e] = y0 - d0; hi[0][e] = y0 + d0;
+        lo[1][e] = y1 - d1; hi[1][e] = y1 + d1;
+      }
+#pragma unroll
+      for (int h = 0; h < 2; h++)
+#pragma unroll
+        for (int e = 0; e < V; e += 2) differ |= q8_encode2<FP8>(lo[h][e], lo[h][V > 1 ? e + 1 : 0]) ^ q8_encode2<FP8>(hi[h][e], hi[h][V > 1 ? e + 1 : 0]);
+      if (__any_sync(0xffffffffu, differ != 0u)) {
+        fetch(i);
+        turned(i, true);
+        finite_most(i);
+      }
+    }
     uint8_t* dst = codes + (size_t)(off + r) * HD + lane * V;
     store_codes<V, FP8>(dst, x[i][0], inv);
     store_codes<V, FP8>(dst + HD / 2, x[i][1], inv);
@@ -314,12 +422,13 @@ AppendArgs append_args(ks_ctx* ctx, const ks_q8_cache* c, const ks_page_tables* 
 
 template <bool NORM>
 int launch_append(ks_ctx* ctx, const ks_q8_cache* c, ks_dtype act, const AppendArgs& a, const char* who) {
-  const unsigned warps = (unsigned)c->page / kRowsPerWarp;
+  const int rows = c->page == 128 ? 4 : 2;  // (up to 32 warps)
+  const unsigned warps = (unsigned)c->page / rows;
   const size_t q_blocks = NORM ? ((size_t)a.max_rows * a.n_q + kHeadsPerWarp * warps - 1) / (kHeadsPerWarp * warps) : 0, blocks = q_blocks + (size_t)a.n_jobs * 2 * a.n_kv;
   KS_REQUIRE(ctx, blocks < (1u << 31), "%s: too many rows and heads for one launch", who);
   KS_REQUIRE_DEVICE(ctx, who);
   ks_on_device on(ctx);
-#define KS_AP(HD_, T_, F_) KS_LAUNCH(ctx, (append_q8_kernel<HD_, T_, F_, NORM>), (unsigned)blocks, warps * 32, 0, a)
+#define KS_AP(HD_, T_, F_) do { if (rows == 4) KS_LAUNCH(ctx, (append_q8_kernel<HD_, T_, F_, NORM, 4>), (unsigned)blocks, warps * 32, 0, a); else KS_LAUNCH(ctx, (append_q8_kernel<HD_, T_, F_, NORM, 2>), (unsigned)blocks, warps * 32, 0, a); } while (0)
 #define KS_AP_T(HD_, F_) do { if (act == KS_F32) KS_AP(HD_, float, F_); else KS_AP(HD_, __half, F_); } while (0)
 #define KS_AP_F(HD_) do { if (c->dtype == KS_E4M3) KS_AP_T(HD_, true); else KS_AP_T(HD_, false); } while (0)
   if (c->hd == 256) KS_AP_F(256);

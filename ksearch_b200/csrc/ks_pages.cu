@@ -227,7 +227,7 @@ int ks_check_tables(ks_ctx* ctx, const char* who, const ks_page_tables* t) {
   KS_REQUIRE(ctx, t->n_seqs >= 1 && t->n_seqs <= KS_PAGES_MAX_SEQS, "%s: n_seqs=%zu outside 1..%d", who, t->n_seqs, KS_PAGES_MAX_SEQS);
   KS_REQUIRE(ctx, t->max_rows >= 1 && t->max_rows <= (1u << 20), "%s: max_rows=%zu outside 1..2^20", who, t->max_rows);
   const size_t most = 0x7FFFFFFFu / t->page;
-  KS_REQUIRE(ctx, t->n_pages >= 1 && t->n_pages <= most && t->max_blocks >= 1 && t->max_blocks <= most, "%s: %zu pages, %zu to a sequence: at least one, and below 2^31 positions", who,
+  KS_REQUIRE(ctx, t->n_pages >= 1 && t->n_pages <= most && t->max_blocks >= 1 && t->max_blocks <= most / 2, "%s: %zu pages, %zu to a sequence: at least one, below 2^31 positions and 2^30", who,
              t->n_pages, t->max_blocks);
   KS_REQUIRE(ctx, ks_fits(t->lens, 0, t->n_seqs * 4) && ks_fits(t->tables, 0, t->n_seqs * t->max_blocks * 4), "%s: lens or tables buffer too small", who);
   KS_REQUIRE(ctx, ks_fits(t->free_pages, 0, (1 + t->n_pages) * 4), "%s: free_pages buffer too small (1 + n_pages words)", who);

@@ -491,6 +491,64 @@ def test_attention_repeats_bit_for_bit(ctx, lens, rows):
     assert np.array_equal(a, b)
 
 
+def test_caches_of_more_than_4_gb(ctx):
+    """Pages whose byte offsets pass 32 bits: append, read back and attention, few rows and many."""
+    page, n_kv, hd = 128, 4, 256
+    n_pages = (1 << 32) // (page * n_kv * hd) + 40
+    rng = np.random.default_rng(13)
+    gpu = Q8Cache(ctx, n_pages, page, n_kv, hd, I8)
+    p = Pair(ctx, 2, 3, n_pages, page, 300)
+    stack = np.concatenate([[n_pages], rng.permutation(n_pages - 20), np.arange(n_pages - 20, n_pages)]).astype(np.int32)   # the last pages come first
+    ctx.write_buffer(p.gpu.free, stack)
+    p.cpu.stack = stack[1:].tolist()
+    c = ref.Cache(8, page, n_kv, hd, I8)
+    eng = Eng()
+    for new in ([260, 9], [1, 30]):
+        p.step(new)
+        k, v = (rng.normal(0, 1, (300, n_kv, hd)).astype(np.float32) for _ in range(2))
+        eng.kv_append_q8(ctx, gpu, p.gpu, ctx.buffer_bytes(k), ctx.buffer_bytes(v))
+        pages = sorted(set(p.cpu.tables[p.cpu.tables >= 0].tolist()))
+        near = {x: i for i, x in enumerate(pages)}          # the same pages in a small cache
+        jobs, p.cpu.jobs = p.cpu.jobs, [[r, n, near[s // page] * page + s % page, q] for r, n, s, q in p.cpu.jobs]
+        c.append(p.cpu, k, v)
+        p.cpu.jobs = jobs
+        n = len(p.cpu.rows)
+        back = [ctx.buffer_empty_f32(300 * n_kv * hd) for _ in range(2)]
+        eng.kv_read_q8(ctx, gpu, n, p.gpu.plan, p.gpu.row_slot, *back)
+        slots = np.array([near[s // page] * page + s % page for _, _, s in p.cpu.rows])
+        for w in range(2):
+            want = ref.decode(c.codes[w], I8)[slots // page, :, slots % page] * c.scales[w][slots // page][:, :, None]
+            assert np.array_equal(ctx.read_f32(back[w], n * n_kv * hd).reshape(want.shape), want)
+        q = rng.normal(0, 1, (300, 8, hd)).astype(np.float32)
+        out, most = ctx.buffer_empty_f32(q.size), max(new)
+        tmp = ctx.buffer_empty_f32(eng.sdpa_paged_tmp_floats(ctx, gpu, p.gpu, 8, most))
+        eng.sdpa_paged_q8(ctx, gpu, p.gpu, 8, most, 300, ctx.buffer_bytes(q), tmp, out, hd ** -0.5)
+        got = ctx.read_f32(out, q.size).reshape(q.shape).astype(np.float64)
+        for s in range(2):
+            a, b = p.cpu.row_start[s:s + 2]
+            table = [near.get(x, 0) for x in p.cpu.tables[s]]
+            want, spread, weight = ref.attention(c, table, int(p.cpu.lens[s]), int(b - a), q[a:b].astype(np.float64), hd ** -0.5, 0)
+            assert (np.abs(got[a:b] - want) <= weight * (2.0 ** -18 * spread[..., None] + 2.0 ** -18)).all()
+    ctx.synchronize()
+
+
+@pytest.mark.parametrize("hint", [1, 64, 1 << 20])
+def test_the_announced_context_is_a_hint(ctx, hint):
+    """A context longer or shorter than announced: the same answers."""
+    rng = np.random.default_rng(14)
+    for rows in ([1, 2, 1], [40, 1, 300], [300, 90, 17]):
+        run_attention(ctx, rng, [900, 130, 700], rows, 32, 8, 2, 128, F16, I8, slack=hint - 900)
+    run_attention(ctx, rng, [900], [150], 16, 4, 1, 256, F32, E4M3, slack=hint - 900)
+
+
+def test_negative_and_zero_scales(ctx):
+    rng = np.random.default_rng(15)
+    for scale in (-0.1, 0.0):
+        for rows in ([1, 3], [90, 60]):
+            run_attention(ctx, rng, [200, 70], rows, 32, 4, 2, 128, F32, I8, scale=scale)
+            run_attention(ctx, rng, [200, 70], rows, 16, 4, 2, 64, F16, E4M3, scale=scale)
+
+
 # ---- together --------------------------------------------------------------------------------------------
 
 @pytest.mark.parametrize("act,fmt,window", [(F32, I8, 0), (F16, E4M3, 40)])

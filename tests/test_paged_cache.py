@@ -91,7 +91,7 @@ CACHE_CALLS = ("append", "norm", "read", "attention")
 
 @pytest.mark.parametrize("name,change", [(n, c) for n in TABLE_CALLS for c in (
     dict(n_seqs=0), dict(n_seqs=1025), dict(max_rows=0), dict(max_rows=(1 << 20) + 1), dict(page=48), dict(page=0), dict(page=256), dict(page=8), dict(n_pages=0),
-    dict(max_blocks=0), dict(n_pages=1 << 27), dict(max_blocks=1 << 62), dict(n_pages=1 << 62))])
+    dict(max_blocks=0), dict(n_pages=1 << 27), dict(max_blocks=1 << 25), dict(max_blocks=1 << 62), dict(n_pages=1 << 62))])
 def test_table_sizes_are_refused(lib, cpu, name, change):
     a = Args(lib, cpu)
     before = a.call(name)
@@ -147,6 +147,15 @@ def test_head_counts(lib, cpu, n_q, code):
     a.n_q = n_q
     assert a.call("attention") == code
     assert (b"no device" in lib.ks_last_error(cpu)) == (n_q in (6, 128))
+
+
+def test_more_work_than_one_call_counts(lib, cpu):
+    a = Args(lib, cpu)
+    a.t.update(n_seqs=1024, max_blocks=1 << 20)
+    a.c.update(n_kv=4)
+    assert a.call("attention") == _lib.ERR_UNSUPPORTED and b"too much for one call" in lib.ks_last_error(cpu)
+    a.t.update(max_blocks=1 << 14)
+    assert a.call("attention") == _lib.ERR_UNSUPPORTED and b"no device" in lib.ks_last_error(cpu)
 
 
 def test_no_rows_are_no_work(lib, cpu):
