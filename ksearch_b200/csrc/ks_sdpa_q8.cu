@@ -108,7 +108,8 @@ __global__ void __launch_bounds__(Split<HD, T>::THREADS, Split<HD, T>::PER_SM) s
   extern __shared__ __align__(128) unsigned char smem[];
   __shared__ unsigned scan[S::WARPS], longest[S::WARPS], seq_first, line[2], seq_at;
   __shared__ float row_m[S::WARPS][8], row_l[S::WARPS][8], row_up[8];
-  ks_pdl_entry();
+  wait_before();
+  start_next();
   const unsigned tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5, g = lane >> 2, c = lane & 3u;
 
   // ---- the line of units: a thread counts for up to four neighbouring sequences
@@ -576,7 +577,8 @@ __global__ void __launch_bounds__(1024) sdpa_q8_merge_kernel(const ks_sdpa_q8_ar
   using S = Split<HD, T>;
   __shared__ float4 red[8][8][16];
   __shared__ float tops[8][8], sums[8][8];
-  ks_pdl_entry();
+  wait_before();
+  start_next();
   const unsigned d = threadIdx.x & 15u, r = threadIdx.x >> 4 & 7u, share = threadIdx.x >> 7, shares = blockDim.x >> 7, dim = blockIdx.y * 64u + 4u * d;
   const int4 job = a.merges[2u * blockIdx.x], where = a.merges[2u * blockIdx.x + 1u];
   const unsigned n = (unsigned)job.y, m = (unsigned)job.w + r;
@@ -656,8 +658,10 @@ int launch_split(ks_ctx* ctx, const ks_sdpa_q8_args& a, unsigned blocks) {
     set[ctx->device & 15] = true;
   }
   KS_LAUNCH(ctx, (sdpa_q8_split_kernel<HD, T, FP8>), blocks, S::THREADS, S::total, a);
-  int rc = ks_after_launch(ctx, "sdpa_paged_q8");
-  if (rc || blocks == 1) return rc;
+  return ks_after_launch(ctx, "sdpa_paged_q8");
+}
+template <int HD, typename T>
+int launch_split_merge(ks_ctx* ctx, const ks_sdpa_q8_args& a, unsigned blocks) {
   // many pieces lie in two or three blocks each: small blocks, so that all are there at once
   const size_t pieces = (size_t)a.n_seqs * a.n_kv * ((a.few + 7u) / 8u);
   KS_LAUNCH(ctx, (sdpa_q8_merge_kernel<HD, T>), dim3(blocks, HD / 64), pieces >= blocks / 4 ? 256 : 1024, 0, a);
@@ -737,8 +741,13 @@ int ks_sdpa_paged_q8(ks_ctx* ctx, const ks_q8_cache* c, const ks_page_tables* t,
 #undef KS_AT_F
 #undef KS_AT_T
 #undef KS_AT
-  if (rc || !wide) return rc;
-  return ks_launch_sdpa_q8_wide(ctx, a, c->hd, act, c->dtype == KS_E4M3, (float*)tmp->dptr + split_floats(ctx, c), ctx_most);
+  float* wide_tmp = (float*)tmp->dptr + split_floats(ctx, c);
+  if (!rc && wide) rc = ks_launch_sdpa_q8_wide(ctx, a, c->hd, act, c->dtype == KS_E4M3, wide_tmp, ctx_most, split);
+#define KS_AT(HD_) (act == KS_F32 ? launch_split_merge<HD_, float>(ctx, a, blocks) : launch_split_merge<HD_, __half>(ctx, a, blocks))
+  if (!rc && split) rc = c->hd == 256 ? KS_AT(256) : c->hd == 128 ? KS_AT(128) : KS_AT(64);
+#undef KS_AT
+  if (!rc && wide) rc = ks_launch_sdpa_q8_wide_merge(ctx, a, c->hd, act, wide_tmp, ctx_most, split);
+  return rc;
 }
 
 }  // extern "C"

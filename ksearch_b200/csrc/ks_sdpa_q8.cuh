@@ -21,9 +21,17 @@ struct ks_sdpa_q8_args {
 constexpr unsigned KS_Q8_FEW = 32;
 // Sequences of more rows; tmp: ks_sdpa_q8_wide_floats.
 size_t ks_sdpa_q8_wide_floats(const ks_ctx* ctx, size_t n_seqs, size_t max_rows, size_t n_kv, size_t G, size_t hd);
-int ks_launch_sdpa_q8_wide(ks_ctx* ctx, const ks_sdpa_q8_args& a, size_t hd, ks_dtype act, bool fp8, float* tmp, size_t ctx_most);
+int ks_launch_sdpa_q8_wide(ks_ctx* ctx, const ks_sdpa_q8_args& a, size_t hd, ks_dtype act, bool fp8, float* tmp, size_t ctx_most, bool beside);
+int ks_launch_sdpa_q8_wide_merge(ks_ctx* ctx, const ks_sdpa_q8_args& a, size_t hd, ks_dtype act, float* tmp, size_t ctx_most, bool beside);
 
 namespace {
+
+// Up to four kernels follow one another in a call: few rows, many rows, the merges of either.  Those of few and of many rows do not depend on each other,
+// nor do the merges, so the second of a pair lets the first run on: a kernel starts its successor only when everything before the pair is
+// done (start_next behind wait_before), the second kernel of a pair (`beside`) waits for the first one only before it ends, so that what
+// follows it follows both.
+__device__ __forceinline__ void wait_before() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void start_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
 // ---- what a sequence has to do ------------------------------------------------------------------------------
 struct Seq {

@@ -112,6 +112,7 @@ __device__ __forceinline__ void commit_if(unsigned leader, uint32_t bar) {
 struct ks_wide_args {
   ks_sdpa_q8_args a;
   unsigned n_splits, share;  // splits of the launch, tiles that one of them takes
+  bool beside;
   int4* meta;   // per block of split 0: first row of the sequence, first (row, head) of the tile, how many the sequence has, KV head + 2^16 splits
   float* part;
   unsigned* err;
@@ -124,7 +125,8 @@ __global__ void __launch_bounds__(Wide<HD, T>::THREADS, 1) sdpa_q8_wide_kernel(c
   const ks_sdpa_q8_args& a = wa.a;
   extern __shared__ __align__(1024) unsigned char smem[];
   unsigned *scan = reinterpret_cast<unsigned*>(smem + W::best), *mine = reinterpret_cast<unsigned*>(smem + W::slot);  // (before those are what they are called)
-  ks_pdl_entry();
+  if (!wa.beside) wait_before();
+  start_next();
   const unsigned tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5;
   const unsigned kvh = blockIdx.x % a.n_kv, index = blockIdx.x / a.n_kv, split = blockIdx.y;
 
@@ -157,6 +159,7 @@ __global__ void __launch_bounds__(Wide<HD, T>::THREADS, 1) sdpa_q8_wide_kernel(c
     }
     if (index >= total) {
       if (split == 0 && tid == 0) wa.meta[blockIdx.x] = make_int4(0, 0, 0, 0);
+      wait_before();
       return;
     }
 #pragma unroll
@@ -189,7 +192,10 @@ __global__ void __launch_bounds__(Wide<HD, T>::THREADS, 1) sdpa_q8_wide_kernel(c
   const int first = seen_from & ~(W::TILE - 1), span = seen_to > first ? (seen_to - first + W::TILE - 1) / W::TILE : 0;
   const int n_splits = min(max((span + (int)wa.share - 1) / (int)wa.share, 1), (int)wa.n_splits), share = (span + n_splits - 1) / n_splits;
   if (split == 0 && tid == 0) wa.meta[blockIdx.x] = make_int4(s.row0, (int)m0, (int)m_rows, (int)(kvh | (unsigned)n_splits << 16));
-  if ((int)split >= n_splits) return;
+  if ((int)split >= n_splits) {
+    wait_before();
+    return;
+  }
   const int t_begin = first + (int)split * share * W::TILE;
   const unsigned n_tiles = (unsigned)max(min(share, span - (int)split * share), 0);
   const bool whole = n_splits == 1;
@@ -205,6 +211,7 @@ __global__ void __launch_bounds__(Wide<HD, T>::THREADS, 1) sdpa_q8_wide_kernel(c
       for (unsigned i = tid; i < W::ROWS * HD; i += W::THREADS)
         if (m0 + i / HD < m_rows) out_row(m0 + i / HD)[i % HD] = (T)0.0f;
     }
+    wait_before();
     return;
   }
   const unsigned q_tiles = W::QT == 2 && m0 + kRows < m_rows ? 2u : 1u;  // a second tile of rows only where there are any
@@ -738,18 +745,23 @@ __global__ void __launch_bounds__(Wide<HD, T>::THREADS, 1) sdpa_q8_wide_kernel(c
   tc_fence_after();
   if (tid == 0 && *fail) atomicOr(wa.err, 16u);
   if (warp == MMA_WARP) tc_dealloc(*tslot, 512);
+  wait_before();
 }
 
 // Records of blocks whose tiles were split, in their order; a warp a row.
 template <int HD, typename T>
 __global__ void __launch_bounds__(1024) sdpa_q8_wide_merge_kernel(const __grid_constant__ ks_wide_args wa) {
   using W = Wide<HD, T>;
-  ks_pdl_entry();
+  if (!wa.beside) wait_before();
+  start_next();
   const ks_sdpa_q8_args& a = wa.a;
   const unsigned lane = threadIdx.x & 31u, r = blockIdx.y * 32u + (threadIdx.x >> 5);
   const int4 meta = wa.meta[blockIdx.x];
   const unsigned m = (unsigned)meta.y + r, n_splits = (unsigned)meta.w >> 16, kvh = (unsigned)meta.w & 0xFFFFu;
-  if (m >= (unsigned)meta.z || n_splits <= 1u) return;
+  if (m >= (unsigned)meta.z || n_splits <= 1u) {
+    wait_before();
+    return;
+  }
   const float* rec = wa.part + (size_t)blockIdx.x * wa.n_splits * W::record;
   float top = kNone, l = 0.0f, v[HD / 32];
   // a split's (m, l) per lane
@@ -779,6 +791,7 @@ __global__ void __launch_bounds__(1024) sdpa_q8_wide_merge_kernel(const __grid_c
     const float y[2] = {v[d] * f, v[d + 1] * f};
     put_dims(o + 2u * lane + 32 * d, y, 2);
   }
+  wait_before();
 }
 
 // Tiles of `rows` (row, head) pairs that the sequences above the line can make at most.
@@ -808,8 +821,23 @@ unsigned wide_splits(const ks_ctx* ctx, size_t blocks, size_t tiles, size_t set_
   return (unsigned)((tiles + s - 1) / s);
 }
 
+// Blocks of the launch, and what its kernels get.
+template <int HD, typename T>
+size_t wide_plan(ks_ctx* ctx, const ks_sdpa_q8_args& a, float* tmp, size_t ctx_most, bool beside, ks_wide_args* wa) {
+  using W = Wide<HD, T>;
+  const size_t blocks = wide_tiles(a.n_seqs, a.max_rows, a.G, W::ROWS) * a.n_kv;
+  wa->a = a;
+  wa->beside = beside;
+  const size_t window = a.window ? (size_t)a.window + W::ROWS / a.G + 1 : ctx_most;
+  wa->n_splits = wide_splits(ctx, blocks, ((window < ctx_most ? window : ctx_most) + W::TILE - 1) / W::TILE, W::TERMS == 1 ? 4 : 2, W::TERMS == 1 ? 12 : 5, &wa->share);
+  wa->meta = (int4*)tmp;
+  wa->part = tmp + 4 * blocks;
+  wa->err = (unsigned*)ctx->ws + KS_WS_ERR_WORD;
+  return blocks;
+}
+
 template <int HD, typename T, bool FP8>
-int launch_wide(ks_ctx* ctx, const ks_sdpa_q8_args& a, float* tmp, size_t ctx_most) {
+int launch_wide(ks_ctx* ctx, const ks_sdpa_q8_args& a, float* tmp, size_t ctx_most, bool beside) {
   using W = Wide<HD, T>;
   static bool set[16] = {false};
   if (!set[ctx->device & 15]) {
@@ -817,19 +845,19 @@ int launch_wide(ks_ctx* ctx, const ks_sdpa_q8_args& a, float* tmp, size_t ctx_mo
     if (e != cudaSuccess) return ks_fail(ctx, KS_ERR_CUDA, "sdpa_paged_q8: cannot set %u B shared memory: %s", W::total, cudaGetErrorString(e));
     set[ctx->device & 15] = true;
   }
-  const size_t blocks = wide_tiles(a.n_seqs, a.max_rows, a.G, W::ROWS) * a.n_kv;
-  KS_REQUIRE(ctx, blocks < (1u << 31), "sdpa_paged_q8: too many rows and heads for one launch");
   ks_wide_args wa;
-  wa.a = a;
-  const size_t window = a.window ? (size_t)a.window + W::ROWS / a.G + 1 : ctx_most;
-  wa.n_splits = wide_splits(ctx, blocks, ((window < ctx_most ? window : ctx_most) + W::TILE - 1) / W::TILE, W::TERMS == 1 ? 4 : 2, W::TERMS == 1 ? 12 : 5, &wa.share);
-  wa.meta = (int4*)tmp;
-  wa.part = tmp + 4 * blocks;
-  wa.err = (unsigned*)ctx->ws + KS_WS_ERR_WORD;
+  const size_t blocks = wide_plan<HD, T>(ctx, a, tmp, ctx_most, beside, &wa);
+  KS_REQUIRE(ctx, blocks < (1u << 31), "sdpa_paged_q8: too many rows and heads for one launch");
   KS_LAUNCH(ctx, (sdpa_q8_wide_kernel<HD, T, FP8>), dim3((unsigned)blocks, wa.n_splits), W::THREADS, W::total, wa);
-  int rc = ks_after_launch(ctx, "sdpa_paged_q8 wide");
-  if (rc || wa.n_splits == 1) return rc;
-  KS_LAUNCH(ctx, (sdpa_q8_wide_merge_kernel<HD, T>), dim3((unsigned)blocks, W::ROWS / 32), 1024, 0, wa);
+  return ks_after_launch(ctx, "sdpa_paged_q8 wide");
+}
+
+template <int HD, typename T>
+int launch_wide_merge(ks_ctx* ctx, const ks_sdpa_q8_args& a, float* tmp, size_t ctx_most, bool beside) {
+  ks_wide_args wa;
+  const size_t blocks = wide_plan<HD, T>(ctx, a, tmp, ctx_most, beside, &wa);
+  if (wa.n_splits == 1) return KS_OK;
+  KS_LAUNCH(ctx, (sdpa_q8_wide_merge_kernel<HD, T>), dim3((unsigned)blocks, Wide<HD, T>::ROWS / 32), 1024, 0, wa);
   return ks_after_launch(ctx, "sdpa_paged_q8 wide merge");
 }
 
@@ -845,12 +873,18 @@ size_t ks_sdpa_q8_wide_floats(const ks_ctx* ctx, size_t n_seqs, size_t max_rows,
   return most;
 }
 
-int ks_launch_sdpa_q8_wide(ks_ctx* ctx, const ks_sdpa_q8_args& a, size_t hd, ks_dtype act, bool fp8, float* tmp, size_t ctx_most) {
-#define KS_WD(HD_, T_, F_) launch_wide<HD_, T_, F_>(ctx, a, tmp, ctx_most)
+int ks_launch_sdpa_q8_wide(ks_ctx* ctx, const ks_sdpa_q8_args& a, size_t hd, ks_dtype act, bool fp8, float* tmp, size_t ctx_most, bool beside) {
+#define KS_WD(HD_, T_, F_) launch_wide<HD_, T_, F_>(ctx, a, tmp, ctx_most, beside)
 #define KS_WD_T(HD_, F_) (act == KS_F32 ? KS_WD(HD_, float, F_) : KS_WD(HD_, __half, F_))
 #define KS_WD_F(HD_) (fp8 ? KS_WD_T(HD_, true) : KS_WD_T(HD_, false))
   return hd == 256 ? KS_WD_F(256) : hd == 128 ? KS_WD_F(128) : KS_WD_F(64);
 #undef KS_WD_F
 #undef KS_WD_T
 #undef KS_WD
+}
+
+int ks_launch_sdpa_q8_wide_merge(ks_ctx* ctx, const ks_sdpa_q8_args& a, size_t hd, ks_dtype act, float* tmp, size_t ctx_most, bool beside) {
+#define KS_WM(HD_) (act == KS_F32 ? launch_wide_merge<HD_, float>(ctx, a, tmp, ctx_most, beside) : launch_wide_merge<HD_, __half>(ctx, a, tmp, ctx_most, beside))
+  return hd == 256 ? KS_WM(256) : hd == 128 ? KS_WM(128) : KS_WM(64);
+#undef KS_WM
 }

@@ -551,11 +551,62 @@ def test_negative_and_zero_scales(ctx):
 
 # ---- together --------------------------------------------------------------------------------------------
 
+@pytest.fixture(scope="module")
+def early(ctx):
+    """A context whose kernels may start while their predecessors run."""
+    c = CudaContext(0, 1)
+    yield c
+    c.close()
+
+
+def test_calls_back_to_back_that_start_early(ctx, early):
+    """Steps, appends and mixed attention enqueued many times over with nothing in between, plainly and as a captured graph: bit for bit what a
+    context without early starts gets, call by call."""
+    got = []
+    for c, waits in ((ctx, True), (early, False)):
+        rng = np.random.default_rng(40)
+        n_q, n_kv, hd, page, T = 8, 2, 128, 32, 300
+        eng, tables = Eng(F16), PageTables(c, 4, 20, 80, page, T)
+        cache = Q8Cache(c, 80, page, n_kv, hd, I8)
+        k, v, q = (c.buffer_bytes(rng.normal(0, 1, (T, n, hd)).astype(np.float16)) for n in (n_kv, n_kv, n_q))
+        new = [ints(c, x) for x in ([150, 1, 0, 40], [1, 1, 1, 1], [2, 130, 1, 0])]
+        keep = ints(c, [0, 0, 0, 0])
+        outs = [[c.buffer_bytes(np.zeros((T, n_q, hd), np.float16)) for _ in range(3)] for _ in range(6)]
+        tmp = c.buffer_empty_f32(eng.sdpa_paged_tmp_floats(c, cache, tables, n_q, 150))
+
+        def go(out):
+            eng.pages_trim(c, tables, keep)
+            for step in range(3):
+                eng.pages_step(c, tables, new[step])
+                eng.kv_append_q8(c, cache, tables, k, v)
+                eng.sdpa_paged_q8(c, cache, tables, n_q, 150, 400, q, tmp, out[step], hd ** -0.5)
+                if waits:
+                    c.synchronize()
+
+        for out in outs[:4]:
+            go(out)
+        if not waits:
+            c.graph_begin()
+            go(outs[4])
+            g = c.graph_end()
+            for _ in range(20):
+                c.graph_launch(g)
+        go(outs[5])
+        c.synchronize()
+        got.append([c.read_bytes(b) for out in (outs[:4] + outs[5:] if waits else outs) for b in out])
+        if not waits:
+            c.graph_free(g)
+    for i, x in enumerate(got[1]):
+        assert np.array_equal(x, got[0][i % 3]), i
+
+
+@pytest.mark.parametrize("flags", [0, 1])
 @pytest.mark.parametrize("act,fmt,window", [(F32, I8, 0), (F16, E4M3, 40)])
-def test_a_decoder_steps_over_pages(ctx, act, fmt, window):
+def test_a_decoder_steps_over_pages(ctx, early, flags, act, fmt, window):
     """Two layers over one set of tables, op by op as a host's loop runs them: prompts of three requests, single tokens, a draft that is turned
     down, a request that ends and another that takes its pages; the single-token step as one captured graph.  Every attention against
     64 bits over what the cache holds, every cache row against the norm and RoPE of what went in."""
+    ctx = early if flags else ctx
     rng = np.random.default_rng(21)
     n_q, n_kv, hd, page, eps, rows_most = 8, 2, 128, 32, 1e-6, 70
     p = Pair(ctx, 3, 8, 18, page, 120)
