@@ -6,6 +6,11 @@
 // division is exact: codes depend on nothing but the values, whatever the order of the operations around them, and however often a
 // scale doubles the error that re-rounding adds stays below one step in all (1/2 + 1/4 + ...); with a / qmax as the scale every new maximum
 // would add half a step.  The price is up to one bit of the int8 codes (none of e4m3's mantissa).
+//
+// Bound by: a few tokens by latency (record of the page, rows and scale, the block's maximum, stores: 2.1 us behind another kernel).  2047 rows of 8 heads of
+// 128 (f16, 12.6 MB): 5.6 us.  2048 rows behind norm and RoPE (f16, 8 query heads, 2 of 256, 25 MB): 10 us, bound by instructions, two thirds of
+// them the query heads'; eight rows a warp (100 registers, half the warps) took 12.  Read-back of 20000 rows of 2 heads of 256 to f16 (61 MB): 13.7 us,
+// 69 % of the measured copy rate.
 #include <cuda_fp16.h>
 
 #include "ks_q8.h"

@@ -3,7 +3,8 @@
 // A step is integer arithmetic on three exclusive sums over the sequences (rows, new pages, touched pages) and one record per row, so it
 // is bound by latency: one trip for lengths and counts, the sums, one trip for a row's page, the stores.  Every block makes the sums
 // for itself and takes rows; nothing that a block reads is written by another, except lengths and the stack's count, which the block that
-// arrived last at a counter writes in the end (every block arrives when it has read them; nobody waits for what the counter says).
+// arrived last at a counter writes in the end (every block arrives when it has read them; nobody waits for what the counter says).  256 sequences and some 16000 rows: 5 us, with a trim in
+// front 9.4; an arrival in front of the rows, or a cluster's barrier in its place, 11.
 #include "ks_q8.h"
 
 namespace {

@@ -2,6 +2,12 @@
 //
 // Row r of a sequence of `len` positions and `rows` rows sits at p = len - rows + r and sees positions max(0, p - window + 1) .. p:
 //   s_j = scale q . k_j,   out = sum_j exp(s_j - m) v_j / sum_j exp(s_j - m),   m = max_j s_j.
+// With v_j = vs_j c_j, vs_j = 2^e f (1 <= f < 2) the scale of its page, everything runs on t_j = s_j log2(e) + e and the codes c_j:
+//   w_j = 2^(t_j - M) f,   out = sum w_j c_j / sum 2^(t_j - M) 2^-e,   M = max_j t_j:
+// weights are below 2^5 whatever the scales (they are rounded to f16 with 2^10 in front), and a sequence whose pages differ by powers of ten
+// keeps what carries the sum.
+//
+// This file: sequences of up to few_of() rows times query heads of a group, and the merge; ks_sdpa_q8_wide.cu: the others.
 #include "ks_sdpa_q8.cuh"
 
 namespace {
@@ -18,11 +24,18 @@ namespace {
 //   S^T = K q^T:  a lane reads 16 bytes of two positions' codes, which are the A operand of four steps over 64 dims if q has its dims in that order;
 //   O^T = V^T P^T:  the probabilities, out of S^T's accumulators, become B operands by movmatrix; a lane reads 16 dims of four positions, pairs
 //   the codes of neighbouring positions by byte permutes, and has its 16 dims of two query rows in the accumulators.
-// Codes become f16 exactly, f32 queries and probabilities are two f16 terms each (the small one first), and in f32 the values of every SUB
-// positions are added to registers: a chain of accumulating MMAs loses low bits at every step.  The maximum that probabilities refer to
-// moves only when a score exceeds it by 2^4.
+// Codes become f16 exactly.  f32 queries and probabilities are two f16 terms each (the small one first), and the values of every SUB positions are added
+// to registers: a chain of accumulating MMAs loses low bits at every step.  f16: queries as they are, probabilities rounded to f16 (2^-12 of
+// each, as much again as rounding the result: 2.9e-4 against 2.1e-4 of a plain f32 form, both off 64 bits), values accumulate in the MMAs.
+// The maximum that probabilities refer to moves only when a score exceeds it by 2^4.
+//
+// Bound by: many long contexts by memory (48 sequences of about 6800 positions, f16, 32 heads on 8 of 128: 664 MB in 109 us, 93 % of the measured copy
+// rate; with 16 x 64 score tiles on the untransposed products and three block barriers a tile it was 314).  Turning codes into f16 is
+// most of what is issued: 5 instructions per 4 codes of K, 7 of V, half the issue slots.  A lone short context by its chain: 700 positions
+// (f32, 8 heads on 1 of 256) 10 us with the merge: lengths and counts 1.0, page, q and first codes 1.4, 16 positions 1.3, the warps' results 1.3,
+// merge and launches the rest.  Four slots of 1024 to 16384 positions (f32, 2 KV heads): 38.8 MB in 19.1 us, four steps of 1.4 us in the middle.
 // The longest context lies in no more blocks than this: each leaves a record that the merge has to read (16384 positions of one KV head: 27 us in 128
-// blocks).
+// blocks, 14 in 64).
 constexpr unsigned kMostParts = 64;
 // x / d: one multiplication where the numbers are small enough for it to be off by less than one.
 __device__ __forceinline__ unsigned quotient(unsigned x, unsigned d) {
@@ -670,6 +683,19 @@ int launch_split_merge(ks_ctx* ctx, const ks_sdpa_q8_args& a, unsigned blocks) {
 
 size_t split_floats(const ks_ctx* ctx, const ks_q8_cache* c) { return (size_t)split_blocks(ctx, c->hd) * (8 + 2 * 8 * (c->hd + 2)); }
 
+// Rows times heads up to which a sequence takes the split kernel: up to 32 always, and up to 512 as long as its blocks have no more than a dozen units
+// each.  Above that the wide kernel, which reads codes once for 128 rows instead of 8, is ahead of it: calls of 16, 32, 64, 128 (row, head)s a
+// sequence took, split / wide, 12 / 28, 13 / 30, 14 / 31, 19 / 34 us for one sequence of 4000 positions (f32, one KV head of 256; 0.2 to 3.5 units), 19 / 45, 25 / 32,
+// 34 / 35, 54 / 39 for four with two KV heads (3.5 to 28), 14 / 29, 16 / 30, 25 / 31, 41 / 26 for sixteen of 600 (f16, four of 128; 2 to 17), 31 / 73, 48 / 77, 86 / 79,
+// 160 / 57 for sixteen of 4000 (14 to 110), and 37 / 77, 57 / 54, 101 / 56, 188 / 70 for sixteen of 4000 in f32 with two of 256 (14 to 110).
+unsigned few_of(const ks_ctx* ctx, const ks_q8_cache* c, const ks_page_tables* t, size_t ctx_most, size_t window) {
+  if (ctx_most > (1u << 30)) ctx_most = 1u << 30;
+  const size_t tile = c->hd == 64 ? 256 : 128, seen = window && window < ctx_most ? window : ctx_most, heads = t->n_seqs * c->n_kv;
+  const size_t most = 12 * (size_t)split_blocks(ctx, c->hd) / (heads * ((seen + tile - 1) / tile + 1)) * 8, few = most < KS_Q8_FEW ? KS_Q8_FEW : most > 512 ? 512 : most;
+  // (units are counted in 32 bits, and contexts may be longer than announced)
+  return heads * (few / 8) * ((t->max_blocks * t->page + 127) / 128) < (size_t(1) << 31) ? (unsigned)few : KS_Q8_FEW;
+}
+
 }  // namespace
 
 extern "C" {
@@ -719,8 +745,9 @@ int ks_sdpa_paged_q8(ks_ctx* ctx, const ks_q8_cache* c, const ks_page_tables* t,
   a.merges = (int4*)tmp->dptr;
   a.part = (float*)tmp->dptr + 8 * (size_t)split_blocks(ctx, c->hd);
   // (a lone sequence that may have many rows needs one kernel only, whatever it has)
-  const bool wide = rows_most * G > KS_Q8_FEW, split = !wide || t->n_seqs > 1;
-  a.few = !split ? 0u : wide ? KS_Q8_FEW : (unsigned)(rows_most * G);
+  const unsigned few = few_of(ctx, c, t, ctx_most, window);
+  const bool wide = rows_most * G > few, split = !wide || t->n_seqs > 1;
+  a.few = !split ? 0u : wide ? few : (unsigned)(rows_most * G);
   a.bad = (unsigned*)ctx->ws + KS_WS_INDEX_WORD;
   a.n_seqs = (unsigned)t->n_seqs;
   a.max_blocks = (unsigned)t->max_blocks;

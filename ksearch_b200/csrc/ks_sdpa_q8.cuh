@@ -17,7 +17,7 @@ struct ks_sdpa_q8_args {
   float scale;
 };
 
-// Rows times query heads of a group up to which a sequence takes the kernel of few rows.
+// Rows times query heads of a group up to which a sequence takes the kernel of few rows, whatever else there is (more: ks_sdpa_q8.cu).
 constexpr unsigned KS_Q8_FEW = 32;
 // Sequences of more rows; tmp: ks_sdpa_q8_wide_floats.
 size_t ks_sdpa_q8_wide_floats(const ks_ctx* ctx, size_t n_seqs, size_t max_rows, size_t n_kv, size_t G, size_t hd);

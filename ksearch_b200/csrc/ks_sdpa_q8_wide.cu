@@ -1,15 +1,25 @@
-// Attention of many rows (prompt pieces, long drafts) over a paged 8-bit cache, on tcgen05.
+// Attention of many rows (prompt pieces, long drafts) over a paged 8-bit cache, on tcgen05 (formulas: ks_sdpa_q8.cu).
 //
-// A block takes 128 query rows (row and query head of the group, counted together) of a sequence against one KV head and walks over the tiles of
-// TILE positions that they see.  Five kinds of warps hand tiles on through mbarriers:
-//   loader      codes of a tile, page by page, by bulk copies into a ring of two; what scores and probabilities are scaled by per 16 positions;
-//   converters  codes -> f16 (exact) core matrices: K as positions x dims, V transposed as dims x positions;
-//   products    one elected lane issues S = q K^T into tensor memory and O (+)= P V with P out of tensor memory;
-//   softmax     eight warps, half a row a thread: S -> mask, maximum, probabilities -> P.
-// The maximum that probabilities refer to moves only when a score exceeds it by 2^4, so the two threads of a row mostly agree by one vote.
-// f16 activations: q as it is, P rounded to f16, O stays in tensor memory and is rescaled there when the maximum moves.  f32: q (first term in
-// tensor memory, second in shared memory) and P are two f16 terms each, small terms first, and O leaves tensor memory after every tile
-// for f32 registers, because its accumulator drops the low bits of what is added.
+// A block takes 128 query rows (row and query head of the group, counted together), or twice 128 (f16, heads up to 128), of a sequence against one KV
+// head and walks over the tiles of TILE positions that they see.  Five kinds of warps hand tiles on through mbarriers:
+//   loaders     codes of a tile, page by page, by bulk copies into rings, K by one warp and V by another; what scores and probabilities are
+//               scaled by per 16 positions;
+//   converters  codes -> f16 (exact) core matrices: K as positions x dims, V transposed as dims x positions, by warps of their own;
+//   products    S = q K^T into tensor memory and O (+)= P V with P out of tensor memory;
+//   softmax     eight warps: S -> mask, maximum, probabilities -> P.
+// The maximum that probabilities refer to moves only when a score exceeds it by 2^4.
+//   f16   q as it is, P rounded to f16, O stays in tensor memory and is rescaled there when the maximum moves.  Two row tiles share the converted
+//         codes (a conversion is worth half the softmax); a thread has a row.  They fill tensor memory, so P lies where half of S was, and the
+//         next scores of a row tile wait until its values are done while the other's softmax runs.
+//   f32   q (first term in tensor memory, second in shared memory) and P are two f16 terms each, small terms first, and O leaves tensor memory
+//         after every tile for f32 registers, because its accumulator drops the low bits of what is added.  Two threads share a row and agree by
+//         one vote a tile.  (f16 heads of 256 run this way too, with one term and O left where it is.)
+//
+// Bound by the chain scores - probabilities - values of a tile, not by a pipe.  4096 rows behind 4096 (f16, 16 heads on 4 of 128; 206 GFLOP): 250 us, 49 % of
+// the measured peak; where a block is at work its tensor pipe is busy half the time, the exponential unit a third, issue slots a third; a tile of
+// 256 x 128 takes 2.6 us, 1.1 of them products.  Sixteen softmax warps instead of eight: 269 us.  Single steps on the way there: products issued
+// behind a branch 381 (90 to 130 clocks each, now 32 and up), rings for K and V together 286, 64 positions a tile 284.  2047 rows (f32, 8 heads on
+// 1 of 256, two splits): 75 us, a tile of 128 x 64 2.6 us, 1.1 of them products.
 #include "ks_sdpa_q8.cuh"
 #include "ks_gemm_common.cuh"
 
@@ -91,7 +101,7 @@ __device__ __forceinline__ uint64_t mul2(uint64_t x, uint64_t y) {
 }
 
 // Products issued by the elected lane of a warp that runs the code as one: predicates instead of a branch keep addresses and descriptors in
-// uniform registers (behind a branch every product took 90 to 130 clocks to issue).  A descriptor's low word is its address in 16 bytes
+// uniform registers.  A descriptor's low word is its address in 16 bytes
 // and the stride between chunks, its high word is the same for all: 128 bytes between groups of 8 rows.
 constexpr uint32_t kDescHigh = (128u >> 4) | 1u << 14;
 __device__ __forceinline__ uint32_t desc_low(uint32_t smem_addr, unsigned chunk) { return (smem_addr >> 4 & 0x3FFFu) | (chunk >> 4 & 0x3FFFu) << 16; }

@@ -541,6 +541,21 @@ def test_the_announced_context_is_a_hint(ctx, hint):
     run_attention(ctx, rng, [900], [150], 16, 4, 1, 256, F32, E4M3, slack=hint - 900)
 
 
+@pytest.mark.parametrize("hint", [1, 1 << 20])
+@pytest.mark.parametrize("act,fmt", [(F32, E4M3), (F16, I8)])
+@pytest.mark.parametrize("n_q,n_kv,hd", HEADS)
+def test_pieces_of_rows_by_either_kernel(ctx, act, fmt, n_q, n_kv, hd, hint):
+    """Short contexts announced: the kernel of few rows takes up to 512 (row, head) pairs of a sequence; long ones: up to 32."""
+    rng = np.random.default_rng(n_q + hd + hint % 7)
+    G = n_q // n_kv
+    lens, rows = [200, 3, 140, 64, 1, 333, 90], [2, 3, 140, 0, 1, 33, 17]
+    for page, window in ((32, 0), (16, 37), (128, 1)):
+        run_attention(ctx, rng, lens, rows, page, n_q, n_kv, hd, act, fmt, window, slack=hint - max(lens))
+    for many in (32 // G, 32 // G + 1, 512 // G, 512 // G + 1):
+        run_attention(ctx, rng, [many + 70], [many], 64, n_q, n_kv, hd, act, fmt, 0, slack=hint - many - 70)
+        run_attention(ctx, rng, [many + 270, 77], [many, 1], 16, n_q, n_kv, hd, act, fmt, 100, slack=hint - many - 270)
+
+
 def test_negative_and_zero_scales(ctx):
     rng = np.random.default_rng(15)
     for scale in (-0.1, 0.0):
