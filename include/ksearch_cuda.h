@@ -227,7 +227,7 @@ typedef struct {
   size_t n_seqs;      /* sequences, 1..KS_PAGES_MAX_SEQS */
   size_t max_blocks;  /* pages a sequence may hold */
   size_t n_pages;     /* pages of the pool */
-  size_t page;        /* positions of a page: 16, 32, 64 or 128; n_pages * page below 2^31, max_blocks * page below 2^30 */
+  size_t page;        /* positions of a page: 16, 32, 64 or 128; n_pages * page and n_seqs * max_blocks below 2^31, max_blocks * page below 2^30 */
   size_t max_rows;    /* new rows of one step, all sequences together: 1..2^20 */
   ks_buf* lens;       /* int32 [n_seqs]: positions a sequence holds */
   ks_buf* tables;     /* int32 [n_seqs, max_blocks]: its pages, -1 behind them */

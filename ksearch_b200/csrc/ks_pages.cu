@@ -230,6 +230,7 @@ int ks_check_tables(ks_ctx* ctx, const char* who, const ks_page_tables* t) {
   const size_t most = 0x7FFFFFFFu / t->page;
   KS_REQUIRE(ctx, t->n_pages >= 1 && t->n_pages <= most && t->max_blocks >= 1 && t->max_blocks <= most / 2, "%s: %zu pages, %zu to a sequence: at least one, below 2^31 positions and 2^30", who,
              t->n_pages, t->max_blocks);
+  KS_REQUIRE(ctx, t->n_seqs * t->max_blocks < (size_t(1) << 31), "%s: tables of %zu x %zu entries: below 2^31", who, t->n_seqs, t->max_blocks);  // (counts of pages are 32 bits)
   KS_REQUIRE(ctx, ks_fits(t->lens, 0, t->n_seqs * 4) && ks_fits(t->tables, 0, t->n_seqs * t->max_blocks * 4), "%s: lens or tables buffer too small", who);
   KS_REQUIRE(ctx, ks_fits(t->free_pages, 0, (1 + t->n_pages) * 4), "%s: free_pages buffer too small (1 + n_pages words)", who);
   KS_REQUIRE(ctx, ks_fits(t->plan, 0, ks_pages_plan_ints(t->n_seqs, t->max_rows, t->page) * 4), "%s: plan buffer too small", who);

@@ -149,6 +149,15 @@ def test_head_counts(lib, cpu, n_q, code):
     assert (b"no device" in lib.ks_last_error(cpu)) == (n_q in (6, 128))
 
 
+@pytest.mark.parametrize("name", TABLE_CALLS)
+def test_more_table_entries_than_32_bits_count(lib, cpu, name):
+    """Lengths that lie could make a sum over all tables' pages pass 2^32."""
+    a = Args(lib, cpu)
+    good = a.tables
+    a.tables = lambda: _changed(good(), dict(n_seqs=1024, max_blocks=1 << 21))
+    assert a.call(name) == _lib.ERR_INVALID and b"entries: below 2^31" in lib.ks_last_error(cpu)
+
+
 def test_more_work_than_one_call_counts(lib, cpu):
     a = Args(lib, cpu)
     a.t.update(n_seqs=1024, max_blocks=1 << 20)
