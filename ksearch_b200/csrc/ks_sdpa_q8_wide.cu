@@ -9,17 +9,20 @@
 //   softmax     eight warps: S -> mask, maximum, probabilities -> P.
 // The maximum that probabilities refer to moves only when a score exceeds it by 2^4.
 //   f16   q as it is, P rounded to f16, O stays in tensor memory and is rescaled there when the maximum moves.  Two row tiles share the converted
-//         codes (a conversion is worth half the softmax); a thread has a row.  They fill tensor memory, so P lies where half of S was, and the
-//         next scores of a row tile wait until its values are done while the other's softmax runs.
+//         codes (a conversion is worth half the softmax); a thread has a row.  They fill tensor memory: P lies in the place of its scores, half a tile
+//         (64 positions) at a time.  While the softmax has one half, the other's values and the next scores in its place are made, for each row tile by a
+//         warp of its own.
 //   f32   q (first term in tensor memory, second in shared memory) and P are two f16 terms each, small terms first, and O leaves tensor memory
 //         after every tile for f32 registers, because its accumulator drops the low bits of what is added.  Two threads share a row and agree by
 //         one vote a tile.  (f16 heads of 256 run this way too, with one term and O left where it is.)
 //
-// Bound by the chain scores - probabilities - values of a tile, not by a pipe.  4096 rows behind 4096 (f16, 16 heads on 4 of 128; 206 GFLOP): 250 us, 49 % of
-// the measured peak; where a block is at work its tensor pipe is busy half the time, the exponential unit a third, issue slots a third; a tile of
-// 256 x 128 takes 2.6 us, 1.1 of them products.  Sixteen softmax warps instead of eight: 269 us.  Single steps on the way there: products issued
-// behind a branch 381 (90 to 130 clocks each, now 32 and up), rings for K and V together 286, 64 positions a tile 284.  2047 rows (f32, 8 heads on
-// 1 of 256, two splits): 75 us, a tile of 128 x 64 2.6 us, 1.1 of them products.
+// Bound by the softmax warps, two a scheduler (f16).  4096 rows behind 4096 (f16, 16 heads on 4 of 128; 206 GFLOP): 236 us, 52 % of the measured peak, 8 % of
+// it because blocks see 32 to 64 tiles.  64 positions of both row tiles take some 2050 clocks: 1250 for their exponentials (1024 at the unit's rate; the two
+// warps come to them together), 800 until the scores are out of tensor memory, their maximum is known and the probabilities are handed on; products
+// 1100 beside them.  Making the warps take turns at the unit: 245 us (their own chain of latencies is as long); every fourth exponential by a polynomial 231,
+// every third 244, left out.  Sixteen softmax warps instead of eight were 7 % slower.  Single steps on the way there: products issued
+// behind a branch 381 (90 to 130 clocks each, now 32 and up), rings for K and V together 286, 64 positions a tile 284, whole tiles handed on 251.  2047 rows (f32,
+// 8 heads on 1 of 256, two splits): 75 us, a tile of 128 x 64 2.6 us, 1.1 of them products.
 #include "ks_sdpa_q8.cuh"
 #include "ks_gemm_common.cuh"
 
@@ -31,14 +34,14 @@ constexpr int kWork = 8;  // softmax warps
 
 // Barriers: codes of a ring's stage there (copies) and converted, K and V; scales of a tile there; K, V converted and multiplied; scores there and read;
 // probabilities there; values done; all products done.
-enum { B_RAW_FULL = 0, B_RAW_FREE = 8, B_SCALE = 16, B_K_FULL = 24, B_K_FREE = 26, B_V_FULL = 28, B_V_FREE = 30, B_S_FULL = 32, B_S_FREE = 34, B_P_FULL = 36, B_PV_DONE = 38, B_DONE = 40, B_COUNT = 41 };
+enum { B_RAW_FULL = 0, B_RAW_FREE = 8, B_SCALE = 16, B_K_FULL = 24, B_K_FREE = 26, B_V_FULL = 28, B_V_FREE = 30, B_S_FULL = 32, B_S_FREE = 36, B_P_FULL = 38, B_PV_DONE = 42, B_DONE = 46, B_COUNT = 48 };
 
 template <int HD_, typename T_>
 struct Wide {
   static constexpr int HD = HD_, TERMS = sizeof(T_) == 4 ? 2 : 1;
   static constexpr int QT = TERMS == 1 && HD <= 128 ? 2 : 1, ROWS = QT * kRows;  // tiles of query rows a block takes
   static constexpr int TILE = HD == 256 ? 64 : 128, GROUPS = TILE / 16, COLS = TILE / 2;  // (a softmax thread has COLS positions in registers at a time)
-  static constexpr int NK = 2, NV = HD == 256 || (HD == 128 && QT == 2) ? 1 : 2;                            // buffers of converted K and V
+  static constexpr int NK = 2, NV = HD == 256 || QT == 2 ? 1 : 2;                            // buffers of converted K and V
   static constexpr int RING = HD == 64 ? 4 : 2;     // tiles of codes
   // The loader of K is RING tiles ahead of its converters at most, those NK ahead of the products and the softmax warps one behind those: a tile's scales are
   // read before their place comes again
@@ -49,7 +52,7 @@ struct Wide {
   static_assert(kWork * 32 * R_WORK + (CONV_K + CONV_V) * 32 * R_CONV + 128 * R_REST <= THREADS * (65536 / THREADS / 8 * 8), "registers: the shares fit the launch");
   // shared memory: barriers, the tensor-memory address and the failure flag; per row: scale, maxima of its two threads; per 16 positions: the score's
   // factor, what is added to it, the probability's factor, the sum's
-  static constexpr unsigned slot = 336, row = 352, best = row + (TERMS == 2 ? kRows * 4 : 0), scale = best + 2 * kRows * 4, q = (scale + SCALES * GROUPS * 16 + 127) / 128 * 128;
+  static constexpr unsigned slot = 384, row = 400, best = row + (TERMS == 2 ? kRows * 4 : 0), scale = best + 2 * kRows * 4, q = (scale + SCALES * GROUPS * 16 + 127) / 128 * 128;
   static_assert(8 * B_COUNT <= slot && slot + 16 <= row, "the words fit in front of the operands");
   static constexpr unsigned q_bytes = kRows * HD * 2, kv_bytes = TILE * HD * 2, k = q + QT * q_bytes, v = k + NK * kv_bytes, raw = v + NV * kv_bytes, raw_bytes = 2 * TILE * HD,
                             total = raw + RING * raw_bytes;
@@ -58,11 +61,16 @@ struct Wide {
   static_assert(ROWS * OP * 4 <= total - q && total <= 232448, "the result fits the operands, and all of it a block");
   // tensor memory: scores, probabilities (two terms), O, of each row tile; q's first term.  Two row tiles fill it (HD = 128) with the probabilities
   // in the place of the scores' second half
-  static constexpr unsigned t_s = 0, t_p = QT == 2 ? t_s + TILE / 2 : t_s + TILE, t_o = QT == 2 ? t_s + TILE : t_p + TERMS * TILE / 2, t_tile = t_o + HD, t_q = QT * t_tile;
+  static constexpr unsigned t_s = 0, t_p = QT == 2 ? t_s : t_s + TILE, t_o = QT == 2 ? t_s + TILE : t_p + TERMS * TILE / 2, t_tile = t_o + HD, t_q = QT * t_tile;
   static_assert(t_q + (TERMS == 2 ? HD / 2 : 0) <= 512, "tensor memory");
   static constexpr unsigned record = ROWS * (HD + 2);  // floats: m[ROWS], l[ROWS], O[ROWS][HD]
 };
 
+__device__ __forceinline__ bool mb_test(uint32_t bar, unsigned parity) {  // has the phase ended?
+  unsigned ok;
+  asm volatile("{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+  return ok != 0;
+}
 __device__ __forceinline__ void arrive1(uint32_t bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory"); }
 // `threads` threads (whole warps) meet at barrier `id`: does any, do all of them say so?
 __device__ __forceinline__ bool meet_any(unsigned id, unsigned threads, bool x) {
@@ -73,6 +81,11 @@ __device__ __forceinline__ bool meet_any(unsigned id, unsigned threads, bool x) 
 __device__ __forceinline__ bool meet_all(unsigned id, unsigned threads, bool x) { return !meet_any(id, threads, !x); }
 __device__ __forceinline__ void proxy_fence() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
+__device__ __forceinline__ float max3(float x, float y, float z) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(x), "f"(y), "f"(z));
+  return r;
+}
 // Two f32 at once.
 __device__ __forceinline__ uint64_t pair(float x, float y) {
   uint64_t r;
@@ -237,14 +250,16 @@ __global__ void __launch_bounds__(Wide<HD, T>::THREADS, 1) sdpa_q8_wide_kernel(c
     for (unsigned i = 0; i < 2u; i++) {
       mb_init(bar(B_K_FULL + i), W::CONV_K);
       mb_init(bar(B_V_FULL + i), W::CONV_V);
-      mb_init(bar(B_K_FREE + i), 1);
-      mb_init(bar(B_V_FREE + i), 1);
+      mb_init(bar(B_K_FREE + i), q_tiles);
+      mb_init(bar(B_V_FREE + i), q_tiles);
+      mb_init(bar(B_S_FREE + i), kWork);
+      mb_init(bar(B_DONE + i), 1);
+    }
+    for (unsigned i = 0; i < 4u; i++) {
       mb_init(bar(B_S_FULL + i), 1);
-      mb_init(bar(B_S_FREE + i), W::QT == 2 ? 4 : kWork);
       mb_init(bar(B_P_FULL + i), W::QT == 2 ? 4 : kWork);
       mb_init(bar(B_PV_DONE + i), 1);
     }
-    mb_init(bar(B_DONE), 1);
     *fail = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     proxy_fence();
@@ -346,61 +361,135 @@ __global__ void __launch_bounds__(Wide<HD, T>::THREADS, 1) sdpa_q8_wide_kernel(c
     };
     bool ok = true;
     const unsigned my_tiles = qt < q_tiles ? n_tiles : 0u;
+    const int all_lo = __reduce_max_sync(0xffffffffu, lo), all_hi = __reduce_min_sync(0xffffffffu, hi);  // every row of the warp sees these
+    // COLS scores of positions p and up, masked
+    auto fetch = [&](uint32_t (&r)[COLS / 16][16], uint32_t from, int p) {
+#pragma unroll
+      for (int c = 0; c < COLS / 16; c++) tc_ld16(from + 16u * c, r[c]);
+#pragma unroll
+      for (int c = 0; c < COLS / 16; c++) tc_wait_ld16(r[c]);
+      if (p < all_lo || p + COLS - 1 > all_hi) {
+#pragma unroll
+        for (int c = 0; c < COLS; c++)
+          if (p + c < lo || p + c > hi) r[c / 16][c % 16] = 0xFF800000u;  // -infinity
+      }
+    };
+    auto largest = [&](const uint32_t (&r)[COLS / 16][16], const float4* scale) {
+      float top = kNone;
+#pragma unroll
+      for (int c = 0; c < COLS / 16; c++) {
+        float g = max3(__uint_as_float(r[c][0]), __uint_as_float(r[c][1]), __uint_as_float(r[c][2])), g2 = max3(__uint_as_float(r[c][3]), __uint_as_float(r[c][4]), __uint_as_float(r[c][5]));
+#pragma unroll
+        for (int e = 6; e < 14; e += 4) {
+          g = max3(g, __uint_as_float(r[c][e]), __uint_as_float(r[c][e + 1]));
+          g2 = max3(g2, __uint_as_float(r[c][e + 2]), __uint_as_float(r[c][e + 3]));
+        }
+        g = max3(fmaxf(g, g2), __uint_as_float(r[c][14]), __uint_as_float(r[c][15]));
+        top = fmaxf(top, fmaf(g, factor(scale[c].x), scale[c].y));
+      }
+      return top;
+    };
+    if constexpr (W::QT == 2) {
+      // What a half needs is asked for while the half before is stored: whether its scores are there, and its scales
+      float4 sc[COLS / 16];
+      auto scales_at = [&](unsigned i, unsigned h) { return reinterpret_cast<const float4*>(smem + W::scale) + i % W::SCALES * W::GROUPS + h * (W::GROUPS / 2); };
+      auto scales_there = [&](unsigned i) { return __all_sync(0xffffffffu, mb_wait(bar(B_SCALE + i % W::SCALES), i / W::SCALES & 1u, kWait)); };
+      bool early = false, early_scales = false;  // they are
+      ok = my_tiles == 0u || scales_there(0);
+      if (ok)
+#pragma unroll
+        for (int c = 0; c < COLS / 16; c++) sc[c] = scales_at(0, 0)[c];
+      for (unsigned i = 0; ok && i < my_tiles; i++) {
+#pragma unroll 1
+        for (unsigned h = 0; h < 2u; h++) {
+          ok = __all_sync(0xffffffffu, early) || __all_sync(0xffffffffu, mb_wait(bar(B_S_FULL + 2u * qt + h), i & 1u, kWait));
+          if (!ok) break;
+          const uint32_t at = tlane + W::t_s + h * COLS;
+          uint32_t r[COLS / 16][16];
+          tc_fence_after();
+          fetch(r, at, t_begin + (int)(i * W::TILE + h * COLS));
+          const float top = largest(r, sc);
+          if (__any_sync(0xffffffffu, top > ref + kSlack)) {
+            const float turn = exp2_fast(ref - fmaxf(top, ref));
+            ref = fmaxf(top, ref);
+            l *= turn;
+            if (i + h > 0u) {  // O may be touched once the half before's values are done; the next ones wait for these probabilities
+              ok = __all_sync(0xffffffffu, mb_wait(bar(B_PV_DONE + 2u * qt + (h ^ 1u)), (h ? i : i - 1u) & 1u, kWait));
+              if (!ok) break;
+              tc_fence_after();
+#pragma unroll 1
+              for (unsigned c = 0; c < HALF; c += 8u) {
+                uint32_t o[8];
+                tc_ld8(tlane + W::t_o + c, o);
+#pragma unroll
+                for (int e = 0; e < 8; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * turn);
+                tc_st8(tlane + W::t_o + c, o);
+              }
+            }
+          }
+          // 16 columns' exponentials run while the 16 before are summed, packed and stored (in the scores' place)
+          auto powers = [&](int c) {
+            const float d = sc[c].y - ref;
+            const uint64_t ff = pair(sc[c].x, sc[c].x), dd = pair(d, d);
+#pragma unroll
+            for (int e = 0; e < 16; e += 2) {
+              const float2 y = apart(fma2(pair(__uint_as_float(r[c][e]), __uint_as_float(r[c][e + 1])), ff, dd));
+              r[c][e] = __float_as_uint(exp2_fast(y.x));
+              r[c][e + 1] = __float_as_uint(exp2_fast(y.y));
+            }
+          };
+          powers(0);
+#pragma unroll
+          for (int c = 0; c < COLS / 16; c++) {
+            if (c + 1 < COLS / 16) powers(c + 1);
+            if (c == 1) {
+              early = mb_test(bar(B_S_FULL + 2u * qt + (h ^ 1u)), (i + h) & 1u);
+              early_scales = mb_test(bar(B_SCALE + (i + 1u) % W::SCALES), (i + 1u) / W::SCALES & 1u);
+            }
+            uint64_t sum = 0, sum2 = 0;
+            uint32_t w[8];
+#pragma unroll
+            for (int e = 0; e < 16; e += 2) {
+              const float y0 = __uint_as_float(r[c][e]), y1 = __uint_as_float(r[c][e + 1]);
+              if (e & 2) sum2 = add2(sum2, pair(y0, y1));
+              else sum = add2(sum, pair(y0, y1));
+              w[e / 2] = q8_u32(__floats2half2_rn(y0, y1));  // (V's scale is in the exponent)
+            }
+            const float2 t = apart(add2(sum, sum2));
+            l = fmaf(t.x + t.y, sc[c].w, l);
+            tc_st8(at + 8u * c, w);
+          }
+          tc_wait_st();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) arrive1(bar(B_P_FULL + 2u * qt + h));
+          if (h == 1u && i + 1u == my_tiles) break;
+          if (h == 1u && !__all_sync(0xffffffffu, early_scales)) {
+            ok = scales_there(i + 1u);
+            if (!ok) break;
+          }
+#pragma unroll
+          for (int c = 0; c < COLS / 16; c++) sc[c] = scales_at(i + h, h ^ 1u)[c];
+        }
+      }
+    } else {
     for (unsigned i = 0; i < my_tiles; i++) {
-      ok = __all_sync(0xffffffffu, mb_wait(bar(B_SCALE + i % W::SCALES), i / W::SCALES & 1u, kWait)) && __all_sync(0xffffffffu, mb_wait(bar(B_S_FULL + qt), i & 1u, kWait));
+      ok = __all_sync(0xffffffffu, mb_wait(bar(B_SCALE + i % W::SCALES), i / W::SCALES & 1u, kWait)) && __all_sync(0xffffffffu, mb_wait(bar(B_S_FULL), i & 1u, kWait));
       uint32_t r[COLS / 16][16];
       float top = kNone;
       const float4* scale = reinterpret_cast<const float4*>(smem + W::scale) + i % W::SCALES * W::GROUPS + half * (W::GROUPS / 2);
       const int p0 = t_begin + (int)i * W::TILE + (int)half * COLS;
-      // scores from column c0 on, masked; (with two row tiles a thread has the whole row: its halves one after the other)
-      auto fetch = [&](unsigned c0) {
-#pragma unroll
-        for (int c = 0; c < COLS / 16; c++) tc_ld16(tlane + W::t_s + half * COLS + c0 + 16u * c, r[c]);
-#pragma unroll
-        for (int c = 0; c < COLS / 16; c++) tc_wait_ld16(r[c]);
-        const int p = p0 + (int)c0;
-        if (!__all_sync(0xffffffffu, lo <= p && hi >= p + COLS - 1)) {
-#pragma unroll
-          for (int c = 0; c < COLS; c++)
-            if (p + c < lo || p + c > hi) r[c / 16][c % 16] = 0xFF800000u;  // -infinity
-        }
-      };
-      auto largest = [&](unsigned c0) {
-#pragma unroll
-        for (int c = 0; c < COLS / 16; c++) {
-          float g = __uint_as_float(r[c][0]);
-#pragma unroll
-          for (int e = 1; e < 16; e++) g = fmaxf(g, __uint_as_float(r[c][e]));
-          const float2 sc = *reinterpret_cast<const float2*>(scale + c0 / 16u + c);
-          top = fmaxf(top, fmaf(g, factor(sc.x), sc.y));
-        }
-      };
       if (ok) {
         tc_fence_after();
-        fetch(0);
-        if constexpr (W::QT == 1) {
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) arrive1(bar(B_S_FREE + qt));
-        }
-        largest(0);
-        if constexpr (W::QT == 2) {
-          fetch(COLS);
-          largest(COLS);
-        }
+        fetch(r, tlane + W::t_s + half * COLS, p0);
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) arrive1(bar(B_S_FREE));
+        top = largest(r, scale);
       }
       float turn = 1.0f;
       bool turned = false;
-      if constexpr (W::QT == 2) {
-        if (!ok) break;
-        if (__any_sync(0xffffffffu, top > ref + kSlack)) {
-          top = fmaxf(top, ref);
-          turn = exp2_fast(ref - top);
-          ref = top;
-          l *= turn;
-          turned = true;
-        }
-      } else if (meet_any(1u + quad, 64u, !ok || top > ref + kSlack)) {  // the two warps that share 32 rows
+      if (meet_any(1u + quad, 64u, !ok || top > ref + kSlack)) {  // the two warps that share 32 rows
         best[half * kRows + row] = top;
         if (!meet_all(1u + quad, 64u, ok)) {
           ok = false;
@@ -412,47 +501,6 @@ __global__ void __launch_bounds__(Wide<HD, T>::THREADS, 1) sdpa_q8_wide_kernel(c
         l *= turn;
         turned = true;
       }
-      if constexpr (W::QT == 2) {
-        auto put = [&](unsigned c0) {  // probabilities of the half in registers
-#pragma unroll
-          for (int c = 0; c < COLS / 16; c++) {
-            const float4 sc = scale[c0 / 16u + c];
-            const float d = sc.y - ref;
-            const uint64_t ff = pair(sc.x, sc.x), dd = pair(d, d);
-            uint64_t sum = 0;
-            uint32_t w[8];
-#pragma unroll
-            for (int e = 0; e < 16; e += 2) {
-              const float2 y = apart(fma2(pair(__uint_as_float(r[c][e]), __uint_as_float(r[c][e + 1])), ff, dd));
-              const float y0 = exp2_fast(y.x), y1 = exp2_fast(y.y);
-              sum = add2(sum, pair(y0, y1));
-              w[e / 2] = q8_u32(__floats2half2_rn(y0, y1));  // (V's scale is in the exponent)
-            }
-            const float2 t = apart(sum);
-            l = fmaf(t.x + t.y, sc.w, l);
-            tc_st8(tlane + W::t_p + c0 / 2u + 8u * c, w);
-          }
-        };
-        // the half in registers first: its probabilities and the others' lie where its scores were.  (The scores are there: so the values of the
-        // tile before are done, and O may be touched)
-        put(COLS);
-        fetch(0);
-        put(0);
-        if (turned && i > 0) {
-#pragma unroll 1
-          for (unsigned c = 0; c < HALF; c += 8u) {
-            uint32_t o[8];
-            tc_ld8(tlane + W::t_o + c, o);
-#pragma unroll
-            for (int e = 0; e < 8; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * turn);
-            tc_st8(tlane + W::t_o + c, o);
-          }
-        }
-        tc_wait_st();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) arrive1(bar(B_P_FULL + qt));
-      } else {
       uint32_t pl[W::TERMS == 2 ? COLS / 2 : 1];
 #pragma unroll
       for (int c = 0; c < COLS / 16; c++) {
@@ -480,7 +528,7 @@ __global__ void __launch_bounds__(Wide<HD, T>::THREADS, 1) sdpa_q8_wide_kernel(c
         l = fmaf(t.x + t.y, sc.w, l);
       }
       // the tile before's values are done: P's place is free, O may be touched
-      if (i > 0) ok = __all_sync(0xffffffffu, mb_wait(bar(B_PV_DONE + qt), (i - 1u) & 1u, kWait));
+      if (i > 0) ok = __all_sync(0xffffffffu, mb_wait(bar(B_PV_DONE), (i - 1u) & 1u, kWait));
       if (ok && i > 0) {
         if constexpr (W::TERMS == 2) {
           fold();
@@ -512,11 +560,11 @@ __global__ void __launch_bounds__(Wide<HD, T>::THREADS, 1) sdpa_q8_wide_kernel(c
         tc_wait_st();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) arrive1(bar(B_P_FULL + qt));
-      }
+        if (lane == 0) arrive1(bar(B_P_FULL));
       }
     }
-    if (my_tiles) ok = ok && __all_sync(0xffffffffu, mb_wait(bar(B_PV_DONE + qt), (n_tiles - 1u) & 1u, kWait));
+    }
+    if (my_tiles) ok = ok && __all_sync(0xffffffffu, mb_wait(bar(B_PV_DONE + (W::QT == 2 ? 2u * qt + 1u : 0u)), (n_tiles - 1u) & 1u, kWait));
     if (!ok && lane == 0) *fail = 1;
     // ---- the rows through shared memory, so that they leave in whole lines; every product that read it is done.  Column n of O is dim
     // 4 (n mod HD / 4) + n / (HD / 4)
@@ -596,100 +644,124 @@ __global__ void __launch_bounds__(Wide<HD, T>::THREADS, 1) sdpa_q8_wide_kernel(c
           *reinterpret_cast<uint4*>(to + ((2u * ch + 1u) * W::TILE + r) * 16u) = y;
         }
       } else {
-        const unsigned b = i % W::NV;
-        if (i >= W::NV && !__all_sync(0xffffffffu, mb_wait(bar(B_V_FREE + b), (i / W::NV - 1u) & 1u, kWait))) break;
         raw += W::TILE * HD;
-        unsigned char* to = smem + W::v + b * W::kv_bytes;
-        // eight positions and four dims a lane; dim 4 w + j becomes column j HD / 4 + w of O, so that neighbouring lanes write neighbouring chunks
-        constexpr unsigned WORDS = HD / 4, PARTS = WORDS >= 32 ? WORDS / 32 : 1, PG = WORDS >= 32 ? 1 : 2, STEPS = W::TILE / 8 * WORDS / 32, PER = STEPS / W::CONV_V;
+        // eight positions and four dims a lane; dim 4 w + j becomes column j HD / 4 + w of O, so that neighbouring lanes write neighbouring chunks.  With
+        // two row tiles the halves of a tile are handed on one by one
+        constexpr unsigned PIECES = W::QT, WORDS = HD / 4, PARTS = WORDS >= 32 ? WORDS / 32 : 1, PG = WORDS >= 32 ? 1 : 2, STEPS = W::TILE / PIECES / 8 * WORDS / 32, PER = STEPS / W::CONV_V;
         static_assert(STEPS % W::CONV_V == 0, "steps of a warp");
+        bool there = true;
+#pragma unroll
+        for (unsigned h = 0; h < PIECES; h++) {
+          const unsigned b = W::QT == 2 ? h : i % W::NV, turn = W::QT == 2 ? i : i / W::NV;  // the buffer, and which time it is used
+          if (turn > 0u && !__all_sync(0xffffffffu, mb_wait(bar(B_V_FREE + b), (turn - 1u) & 1u, kWait))) {
+            there = false;
+            break;
+          }
+          unsigned char* to = smem + W::v + b * (W::kv_bytes / PIECES);
+          const unsigned char* half_at = raw + h * (W::TILE / PIECES) * HD;
 #pragma unroll 2
-        for (unsigned j = 0; j < PER; j++) {
-          const unsigned n = cw * PER + j, w = PG == 2 ? lane & 15u : n % PARTS * 32u + lane, pg = PG == 2 ? 2u * n + (lane >> 4) : n / PARTS;
-          uint32_t v[8], p[4][4];
+          for (unsigned j = 0; j < PER; j++) {
+            const unsigned n = cw * PER + j, w = PG == 2 ? lane & 15u : n % PARTS * 32u + lane, pg = PG == 2 ? 2u * n + (lane >> 4) : n / PARTS;
+            uint32_t v[8], p[4][4];
 #pragma unroll
-          for (int e = 0; e < 8; e++) v[e] = *reinterpret_cast<const uint32_t*>(raw + (8u * pg + e) * HD + 4u * w);
+            for (int e = 0; e < 8; e++) v[e] = *reinterpret_cast<const uint32_t*>(half_at + (8u * pg + e) * HD + 4u * w);
 #pragma unroll
-          for (int e = 0; e < 4; e++) widen_pairs<FP8>(v[2 * e], v[2 * e + 1], p[e]);
+            for (int e = 0; e < 4; e++) widen_pairs<FP8>(v[2 * e], v[2 * e + 1], p[e]);
 #pragma unroll
-          for (int j = 0; j < 4; j++) *reinterpret_cast<uint4*>(to + (pg * HD + j * WORDS + w) * 16u) = make_uint4(p[0][j], p[1][j], p[2][j], p[3][j]);
+            for (int j = 0; j < 4; j++) *reinterpret_cast<uint4*>(to + (pg * HD + j * WORDS + w) * 16u) = make_uint4(p[0][j], p[1][j], p[2][j], p[3][j]);
+          }
+          proxy_fence();
+          __syncwarp();
+          if (lane == 0) arrive1(bar(B_V_FULL + b));
         }
+        if (!there) break;
       }
-      proxy_fence();
-      __syncwarp();
-      if (lane == 0) {
-        arrive1(bar(keys ? B_K_FULL + i % W::NK : B_V_FULL + i % W::NV));
-        arrive1(bar(B_RAW_FREE + kv4 + i % W::RING));
+      if (keys) {
+        proxy_fence();
+        __syncwarp();
+        if (lane == 0) arrive1(bar(B_K_FULL + i % W::NK));
       }
+      if (lane == 0) arrive1(bar(B_RAW_FREE + kv4 + i % W::RING));
       done++;
     }
     if (done < n_tiles && lane == 0) *fail = 1;
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(W::R_REST));
-    if (warp == MMA_WARP) {
-      // ---- products
-      const unsigned leader = elect_one(), tiles = __reduce_max_sync(0xffffffffu, n_tiles), qts = __reduce_max_sync(0xffffffffu, q_tiles);
-      constexpr uint32_t idesc_s = (1u << 4) | ((W::TILE >> 3) << 17) | ((kRows >> 4) << 24), idesc_o = (1u << 4) | ((HD >> 3) << 17) | ((kRows >> 4) << 24);
+    if (warp == MMA_WARP || (W::QT == 2 && warp == MMA_WARP + 3u && q_tiles == 2u)) {
+      // ---- products, of each row tile by a warp
+      const unsigned leader = elect_one(), tiles = __reduce_max_sync(0xffffffffu, n_tiles), t = __reduce_max_sync(0xffffffffu, warp == MMA_WARP ? 0u : 1u);
+      constexpr unsigned COLS_S = W::TILE / W::QT;  // positions of the scores that are made at a time
+      constexpr uint32_t idesc_s = (1u << 4) | ((COLS_S >> 3) << 17) | ((kRows >> 4) << 24), idesc_o = (1u << 4) | ((HD >> 3) << 17) | ((kRows >> 4) << 24);
       auto wait = [&](unsigned b, unsigned parity) { return __all_sync(0xffffffffu, mb_wait(bar(b), parity & 1u, kWait)); };
       const uint32_t base = __reduce_max_sync(0xffffffffu, sb);
-      const uint32_t d_q = desc_low(base + W::q, kRows * 16u), d_k = desc_low(base + W::k, W::TILE * 16u), d_v = desc_low(base + W::v, HD * 16u);
-      auto scores = [&](unsigned i, unsigned t) {
-        const uint32_t k = d_k + i % W::NK * (W::kv_bytes / 16u), q = d_q + t * (W::q_bytes / 16u), to = t * W::t_tile + W::t_s;
+      const uint32_t d_q = desc_low(base + W::q + t * W::q_bytes, kRows * 16u), d_k = desc_low(base + W::k, W::TILE * 16u), d_v = desc_low(base + W::v, HD * 16u);
+      auto scores = [&](unsigned i, unsigned h) {  // of a tile, or of half of one
+        const uint32_t k = d_k + i % W::NK * (W::kv_bytes / 16u) + h * COLS_S, to = t * W::t_tile + W::t_s + h * COLS_S;
 #pragma unroll
-        for (unsigned ks = 0; ks < HD / 16u; ks++) issue_ss(leader, to, q + 2u * ks * kRows, k + 2u * ks * W::TILE, idesc_s, ks ? 1u : 0u);
+        for (unsigned ks = 0; ks < HD / 16u; ks++) issue_ss(leader, to, d_q + 2u * ks * kRows, k + 2u * ks * W::TILE, idesc_s, ks ? 1u : 0u);
         if constexpr (W::TERMS == 2)
 #pragma unroll
           for (unsigned ks = 0; ks < HD / 16u; ks++) issue_ts(leader, to, W::t_q + 8u * ks, k + 2u * ks * W::TILE, idesc_s, 1u);
-        commit_if(leader, base + 8u * (B_S_FULL + t));
-        if (t + 1u == qts) commit_if(leader, base + 8u * (B_K_FREE + i % W::NK));
+        commit_if(leader, base + 8u * (B_S_FULL + 2u * t + h));
+        if (h + 1u == W::QT) commit_if(leader, base + 8u * (B_K_FREE + i % W::NK));
       };
       bool ok = wait(B_K_FULL, 0u);
       if (ok) {
         tc_fence_after();
 #pragma unroll
-        for (unsigned t = 0; t < W::QT; t++)
-          if (t < qts) scores(0, t);
+        for (unsigned h = 0; h < W::QT; h++) scores(0, h);
       }
       for (unsigned i = 0; ok && i < tiles; i++) {
+        if constexpr (W::QT == 2) {
+          // half by half: while the softmax has one, the values of the other and, in their probabilities' place, its next scores are made
 #pragma unroll
-        for (unsigned t = 0; t < W::QT; t++) {
-          if (!ok || t >= qts) continue;
-          if (W::QT == 1 && i + 1u < tiles) {  // the next scores in front of these values
+          for (unsigned h = 0; h < 2u; h++) {
+            ok = ok && wait(B_V_FULL + h, i) && wait(B_P_FULL + 2u * t + h, i);
+            if (!ok) continue;
+            tc_fence_after();
+#pragma unroll
+            for (unsigned ks = 0; ks < COLS_S / 16u; ks++)
+              issue_ts(leader, t * W::t_tile + W::t_o, t * W::t_tile + W::t_p + h * COLS_S + 8u * ks, d_v + h * (W::kv_bytes / 32u) + 2u * ks * HD, idesc_o, ks | h ? 1u : i);
+            commit_if(leader, base + 8u * (B_PV_DONE + 2u * t + h));
+            commit_if(leader, base + 8u * (B_V_FREE + h));
+            if (i + 1u < tiles) {
+              ok = (h || wait(B_K_FULL + (i + 1u) % W::NK, (i + 1u) / W::NK)) && wait(B_PV_DONE + 2u * t + h, i);
+              if (!ok) continue;
+              tc_fence_after();
+              scores(i + 1u, h);
+            }
+          }
+        } else {
+          if (i + 1u < tiles) {  // the next scores in front of these values
             ok = wait(B_K_FULL + (i + 1u) % W::NK, (i + 1u) / W::NK) && wait(B_S_FREE, i);
             if (!ok) continue;
             tc_fence_after();
-            scores(i + 1u, t);
+            scores(i + 1u, 0);
           }
-          ok = (t || wait(B_V_FULL + i % W::NV, i / W::NV)) && wait(B_P_FULL + t, i);
+          ok = wait(B_V_FULL + i % W::NV, i / W::NV) && wait(B_P_FULL, i);
           if (!ok) continue;
           tc_fence_after();
-          const uint32_t v = d_v + i % W::NV * (W::kv_bytes / 16u), to = t * W::t_tile + W::t_o, p = t * W::t_tile + W::t_p;
+          const uint32_t v = d_v + i % W::NV * (W::kv_bytes / 16u);
           if constexpr (W::TERMS == 2) {
 #pragma unroll
-            for (unsigned ks = 0; ks < W::TILE / 16u; ks++) issue_ts(leader, to, p + W::TILE / 2 + 8u * ks, v + 2u * ks * HD, idesc_o, ks ? 1u : 0u);
+            for (unsigned ks = 0; ks < W::TILE / 16u; ks++) issue_ts(leader, W::t_o, W::t_p + W::TILE / 2 + 8u * ks, v + 2u * ks * HD, idesc_o, ks ? 1u : 0u);
 #pragma unroll
-            for (unsigned ks = 0; ks < W::TILE / 16u; ks++) issue_ts(leader, to, p + 8u * ks, v + 2u * ks * HD, idesc_o, 1u);
+            for (unsigned ks = 0; ks < W::TILE / 16u; ks++) issue_ts(leader, W::t_o, W::t_p + 8u * ks, v + 2u * ks * HD, idesc_o, 1u);
           } else {
 #pragma unroll
-            for (unsigned ks = 0; ks < W::TILE / 16u; ks++) issue_ts(leader, to, p + 8u * ks, v + 2u * ks * HD, idesc_o, ks ? 1u : i);
+            for (unsigned ks = 0; ks < W::TILE / 16u; ks++) issue_ts(leader, W::t_o, W::t_p + 8u * ks, v + 2u * ks * HD, idesc_o, ks ? 1u : i);
           }
-          commit_if(leader, base + 8u * (B_PV_DONE + t));
-          if (t + 1u == qts) commit_if(leader, base + 8u * (B_V_FREE + i % W::NV));
-          if (W::QT == 2 && i + 1u < tiles) {  // behind them: they take the probabilities' place.  Meanwhile the other row tile's softmax runs
-            ok = (t || wait(B_K_FULL + (i + 1u) % W::NK, (i + 1u) / W::NK)) && wait(B_PV_DONE + t, i);
-            if (!ok) continue;
-            tc_fence_after();
-            scores(i + 1u, t);
-          }
+          commit_if(leader, base + 8u * B_PV_DONE);
+          commit_if(leader, base + 8u * (B_V_FREE + i % W::NV));
         }
       }
       if (leader) {  // every product issued must finish before shared and tensor memory go away (bounded)
         if (!ok) *fail = 1;
-        tc_commit(bar(B_DONE));
+        tc_commit(bar(B_DONE + t));
       }
       __syncwarp();
-      mb_wait(bar(B_DONE), 0u, kWait);
-    } else if (warp <= MMA_WARP + 2) {
+      mb_wait(bar(B_DONE + t), 0u, kWait);
+    } else if (warp == MMA_WARP + 1u || warp == MMA_WARP + 2u) {
       // ---- codes, K and the scales by one warp, V by another: the runs of a tile that lie in one page, a lane each
       const bool keys = warp == MMA_WARP + 1;
       const unsigned kv4 = keys ? 0u : 4u;
