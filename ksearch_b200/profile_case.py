@@ -7,6 +7,8 @@ profiler captures are taken on.
     python -m ksearch_b200.profile_case decode --layers 4 --tokens 4
     python -m ksearch_b200.profile_case attn --kv 1 --ctx 16384 --slots 4 --copies 8 --iters 2
     python -m ksearch_b200.profile_case chunk --rows 2047 --ctx 0 --kv 1 --splits 2 --iters 4
+    python -m ksearch_b200.profile_case paged --slots 8 --ctx 8192 --rows 1 --kv 8 --group 4 --copies 2 --iters 1
+    python -m ksearch_b200.profile_case paged --slots 1 --ctx 4096 --rows 2048 --kv 4 --group 4 --copies 2 --iters 1
 
 `--copies` distinct weight copies are cycled so that a launch never finds its weights in L2
 (copies * matrix bytes should exceed the 126 MB L2).  Prints the CUDA-event time per launch.
@@ -17,13 +19,13 @@ import argparse
 
 import numpy as np
 
-from . import Q4K, Q6K, CudaContext, Eng, synth
+from . import E4M3, F16, Q4K, Q6K, CudaContext, Eng, PageTables, Q8Cache, synth
 from . import model as ksm
 
 
 def main():
     ap = argparse.ArgumentParser()
-    ap.add_argument("op", choices=["matvec", "gate_up", "decode", "attn", "chunk"])
+    ap.add_argument("op", choices=["matvec", "gate_up", "decode", "attn", "chunk", "paged"])
     ap.add_argument("--dtype", default="q4k", choices=["q4k", "q6k"])
     ap.add_argument("--rows", type=int, default=4096)
     ap.add_argument("--cols", type=int, default=4096)
@@ -32,10 +34,11 @@ def main():
     ap.add_argument("--layers", type=int, default=4)
     ap.add_argument("--tokens", type=int, default=4)
     ap.add_argument("--pdl", type=int, default=0)
-    ap.add_argument("--kv", type=int, default=1, help="attn, chunk: KV heads (8 query heads)")
-    ap.add_argument("--ctx", type=int, default=16384, help="attn: positions per slot; chunk: positions in front of its rows")
+    ap.add_argument("--kv", type=int, default=1, help="attn, chunk: KV heads (8 query heads); paged: KV heads")
+    ap.add_argument("--ctx", type=int, default=16384, help="attn: positions per slot; chunk: positions in front of its rows; paged: positions of a sequence, its rows the last")
     ap.add_argument("--splits", type=int, default=1, help="chunk: context splits")
-    ap.add_argument("--slots", type=int, default=4, help="attn: slots")
+    ap.add_argument("--slots", type=int, default=4, help="attn: slots; paged: sequences")
+    ap.add_argument("--group", type=int, default=4, help="paged: query heads of a KV head (f16, heads of 128, e4m3 in pages of 64)")
     ap.add_argument("--batch", type=int, default=1, help="token rows per matvec call (more than 8: the tensor-core GEMM)")
     args = ap.parse_args()
     ctx = CudaContext(0, flags=args.pdl)
@@ -75,6 +78,36 @@ def main():
             chunk()
         us = ctx.timer_end_ms() / args.iters * 1e3
         print(f"chunk: {args.rows} rows behind {args.ctx} positions, {args.kv} KV heads, {args.splits} splits: {us:.1f} us/launch")
+        return
+    if args.op == "paged":
+        eng, hd, page, n = Eng(F16), 128, 64, args.slots
+        blocks = -(-args.ctx // page)
+        t = PageTables(ctx, n, blocks, n * blocks, page, n * args.rows)
+        caches = [Q8Cache(ctx, t.n_pages, page, args.kv, hd, E4M3) for _ in range(args.copies)]
+        rng = np.random.default_rng(1)
+        some = rng.integers(0, 120, caches[0].k.nbytes, np.uint8)    # positive codes up to 288
+        for c in caches:
+            for codes, scale in ((c.k, c.k_scale), (c.v, c.v_scale)):
+                ctx.write_buffer(codes, rng.permutation(some))
+                ctx.write_buffer(scale, np.full(scale.nbytes // 4, 2.0 ** -9, np.float32))
+        ctx.write_buffer(t.tables, rng.permutation(t.n_pages).astype(np.int32))
+        ctx.write_buffer(t.lens, np.full(n, args.ctx, np.int32))
+        ctx.write_buffer(t.plan, (np.arange(n + 1) * args.rows).astype(np.int32), 4 * t.plan_part(t.ROW_START))
+        q = ctx.buffer_bytes(synth.normals(1, "q", t.max_rows * args.kv * args.group * hd).astype(np.float16))
+        out = ctx.buffer_empty_bytes(q.nbytes)
+        tmp = ctx.buffer_empty_bytes(4 * eng.sdpa_paged_tmp_floats(ctx, caches[0], t, args.kv * args.group, args.rows))
+
+        def paged(c):
+            eng.sdpa_paged_q8(ctx, c, t, args.kv * args.group, args.rows, args.ctx, q, tmp, out, hd ** -0.5)
+        for c in caches:   # first touch
+            paged(c)
+        ctx.synchronize()
+        ctx.timer_begin()
+        for _ in range(args.iters):
+            for c in caches:
+                paged(c)
+        us = ctx.timer_end_ms() / (args.iters * args.copies) * 1e3
+        print(f"paged: {n} sequences of {args.ctx} positions, {args.rows} rows each, {args.kv} KV heads: {us:.1f} us/call")
         return
     if args.op == "attn":
         from .eng import write_meta
