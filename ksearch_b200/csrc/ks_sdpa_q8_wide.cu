@@ -22,7 +22,7 @@
 // 1100 beside them.  Making the warps take turns at the unit: 245 us (their own chain of latencies is as long); every fourth exponential by a polynomial 231,
 // every third 244, left out.  Sixteen softmax warps instead of eight were 7 % slower.  Single steps on the way there: products issued
 // behind a branch 381 (90 to 130 clocks each, now 32 and up), rings for K and V together 286, 64 positions a tile 284, whole tiles handed on 251.  2047 rows (f32,
-// 8 heads on 1 of 256, two splits): 75 us, a tile of 128 x 64 2.6 us, 1.1 of them products.
+// 8 heads on 1 of 256, two splits): 71 us (75 before V's one buffer was handed on by halves), a tile of 128 x 64 2.5 us, 1.1 of them products.
 #include "ks_sdpa_q8.cuh"
 #include "ks_gemm_common.cuh"
 
@@ -42,6 +42,7 @@ struct Wide {
   static constexpr int QT = TERMS == 1 && HD <= 128 ? 2 : 1, ROWS = QT * kRows;  // tiles of query rows a block takes
   static constexpr int TILE = HD == 256 ? 64 : 128, GROUPS = TILE / 16, COLS = TILE / 2;  // (a softmax thread has COLS positions in registers at a time)
   static constexpr int NK = 2, NV = HD == 256 || QT == 2 ? 1 : 2;                            // buffers of converted K and V
+  static constexpr unsigned PIECES = NV == 1 ? 2 : 1;  // a lone buffer of V is handed on, and back, by halves: one is converted while the other is multiplied
   static constexpr int RING = HD == 64 ? 4 : 2;     // tiles of codes
   // The loader of K is RING tiles ahead of its converters at most, those NK ahead of the products and the softmax warps one behind those: a tile's scales are
   // read before their place comes again
@@ -473,96 +474,96 @@ __global__ void __launch_bounds__(Wide<HD, T>::THREADS, 1) sdpa_q8_wide_kernel(c
         }
       }
     } else {
-    for (unsigned i = 0; i < my_tiles; i++) {
-      ok = __all_sync(0xffffffffu, mb_wait(bar(B_SCALE + i % W::SCALES), i / W::SCALES & 1u, kWait)) && __all_sync(0xffffffffu, mb_wait(bar(B_S_FULL), i & 1u, kWait));
-      uint32_t r[COLS / 16][16];
-      float top = kNone;
-      const float4* scale = reinterpret_cast<const float4*>(smem + W::scale) + i % W::SCALES * W::GROUPS + half * (W::GROUPS / 2);
-      const int p0 = t_begin + (int)i * W::TILE + (int)half * COLS;
-      if (ok) {
-        tc_fence_after();
-        fetch(r, tlane + W::t_s + half * COLS, p0);
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) arrive1(bar(B_S_FREE));
-        top = largest(r, scale);
-      }
-      float turn = 1.0f;
-      bool turned = false;
-      if (meet_any(1u + quad, 64u, !ok || top > ref + kSlack)) {  // the two warps that share 32 rows
-        best[half * kRows + row] = top;
-        if (!meet_all(1u + quad, 64u, ok)) {
-          ok = false;
-          break;
-        }
-        top = fmaxf(fmaxf(top, best[(half ^ 1u) * kRows + row]), ref);
-        turn = exp2_fast(ref - top);
-        ref = top;
-        l *= turn;
-        turned = true;
-      }
-      uint32_t pl[W::TERMS == 2 ? COLS / 2 : 1];
-#pragma unroll
-      for (int c = 0; c < COLS / 16; c++) {
-        const float4 sc = scale[c];
-        const float f = factor(sc.x), d = sc.y - ref;
-        const uint64_t ff = pair(f, f), dd = pair(d, d);
-        uint64_t sum = 0;
-#pragma unroll
-        for (int e = 0; e < 16; e += 2) {
-          const float2 y = apart(fma2(pair(__uint_as_float(r[c][e]), __uint_as_float(r[c][e + 1])), ff, dd));
-          const float y0 = exp2_fast(y.x), y1 = exp2_fast(y.y);
-          const uint64_t yy = pair(y0, y1);
-          sum = add2(sum, yy);
-          if constexpr (W::TERMS == 1) {
-            r[c][e / 2] = q8_u32(__floats2half2_rn(y0, y1));  // (V's scale is in the exponent)
-          } else {
-            const float2 z = apart(mul2(yy, pair(sc.z, sc.z)));
-            const __half2 h = __floats2half2_rn(z.x, z.y);
-            const float2 b = __half22float2(h);
-            r[c][e / 2] = q8_u32(h);
-            pl[c * 8 + e / 2] = q8_u32(__floats2half2_rn(z.x - b.x, z.y - b.y));
-          }
-        }
-        const float2 t = apart(sum);
-        l = fmaf(t.x + t.y, sc.w, l);
-      }
-      // the tile before's values are done: P's place is free, O may be touched
-      if (i > 0) ok = __all_sync(0xffffffffu, mb_wait(bar(B_PV_DONE), (i - 1u) & 1u, kWait));
-      if (ok && i > 0) {
-        if constexpr (W::TERMS == 2) {
-          fold();
-          if (turned)
-#pragma unroll
-            for (int c = 0; c < HALF; c++) acc[c] *= turn;
-        } else if (turned) {
+      for (unsigned i = 0; i < my_tiles; i++) {
+        ok = __all_sync(0xffffffffu, mb_wait(bar(B_SCALE + i % W::SCALES), i / W::SCALES & 1u, kWait)) && __all_sync(0xffffffffu, mb_wait(bar(B_S_FULL), i & 1u, kWait));
+        uint32_t r[COLS / 16][16];
+        float top = kNone;
+        const float4* scale = reinterpret_cast<const float4*>(smem + W::scale) + i % W::SCALES * W::GROUPS + half * (W::GROUPS / 2);
+        const int p0 = t_begin + (int)i * W::TILE + (int)half * COLS;
+        if (ok) {
           tc_fence_after();
-#pragma unroll 1
-          for (unsigned c = 0; c < HALF; c += 8u) {
-            uint32_t o[8];
-            tc_ld8(tlane + W::t_o + half * HALF + c, o);
-#pragma unroll
-            for (int e = 0; e < 8; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * turn);
-            tc_st8(tlane + W::t_o + half * HALF + c, o);
-          }
+          fetch(r, tlane + W::t_s + half * COLS, p0);
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) arrive1(bar(B_S_FREE));
+          top = largest(r, scale);
         }
-      }
-      if (ok) {
+        float turn = 1.0f;
+        bool turned = false;
+        if (meet_any(1u + quad, 64u, !ok || top > ref + kSlack)) {  // the two warps that share 32 rows
+          best[half * kRows + row] = top;
+          if (!meet_all(1u + quad, 64u, ok)) {
+            ok = false;
+            break;
+          }
+          top = fmaxf(fmaxf(top, best[(half ^ 1u) * kRows + row]), ref);
+          turn = exp2_fast(ref - top);
+          ref = top;
+          l *= turn;
+          turned = true;
+        }
+        uint32_t pl[W::TERMS == 2 ? COLS / 2 : 1];
 #pragma unroll
         for (int c = 0; c < COLS / 16; c++) {
-          const uint32_t w[8] = {r[c][0], r[c][1], r[c][2], r[c][3], r[c][4], r[c][5], r[c][6], r[c][7]};
-          tc_st8(tlane + W::t_p + half * (COLS / 2) + 8 * c, w);
+          const float4 sc = scale[c];
+          const float f = factor(sc.x), d = sc.y - ref;
+          const uint64_t ff = pair(f, f), dd = pair(d, d);
+          uint64_t sum = 0;
+#pragma unroll
+          for (int e = 0; e < 16; e += 2) {
+            const float2 y = apart(fma2(pair(__uint_as_float(r[c][e]), __uint_as_float(r[c][e + 1])), ff, dd));
+            const float y0 = exp2_fast(y.x), y1 = exp2_fast(y.y);
+            const uint64_t yy = pair(y0, y1);
+            sum = add2(sum, yy);
+            if constexpr (W::TERMS == 1) {
+              r[c][e / 2] = q8_u32(__floats2half2_rn(y0, y1));  // (V's scale is in the exponent)
+            } else {
+              const float2 z = apart(mul2(yy, pair(sc.z, sc.z)));
+              const __half2 h = __floats2half2_rn(z.x, z.y);
+              const float2 b = __half22float2(h);
+              r[c][e / 2] = q8_u32(h);
+              pl[c * 8 + e / 2] = q8_u32(__floats2half2_rn(z.x - b.x, z.y - b.y));
+            }
+          }
+          const float2 t = apart(sum);
+          l = fmaf(t.x + t.y, sc.w, l);
+        }
+        // the tile before's values are done: P's place is free, O may be touched
+        if (i > 0) ok = __all_sync(0xffffffffu, mb_wait(bar(B_PV_DONE), (i - 1u) & 1u, kWait));
+        if (ok && i > 0) {
           if constexpr (W::TERMS == 2) {
-            const uint32_t z[8] = {pl[8 * c], pl[8 * c + 1], pl[8 * c + 2], pl[8 * c + 3], pl[8 * c + 4], pl[8 * c + 5], pl[8 * c + 6], pl[8 * c + 7]};
-            tc_st8(tlane + W::t_p + W::TILE / 2 + half * (COLS / 2) + 8 * c, z);
+            fold();
+            if (turned)
+#pragma unroll
+              for (int c = 0; c < HALF; c++) acc[c] *= turn;
+          } else if (turned) {
+            tc_fence_after();
+#pragma unroll 1
+            for (unsigned c = 0; c < HALF; c += 8u) {
+              uint32_t o[8];
+              tc_ld8(tlane + W::t_o + half * HALF + c, o);
+#pragma unroll
+              for (int e = 0; e < 8; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * turn);
+              tc_st8(tlane + W::t_o + half * HALF + c, o);
+            }
           }
         }
-        tc_wait_st();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) arrive1(bar(B_P_FULL));
+        if (ok) {
+#pragma unroll
+          for (int c = 0; c < COLS / 16; c++) {
+            const uint32_t w[8] = {r[c][0], r[c][1], r[c][2], r[c][3], r[c][4], r[c][5], r[c][6], r[c][7]};
+            tc_st8(tlane + W::t_p + half * (COLS / 2) + 8 * c, w);
+            if constexpr (W::TERMS == 2) {
+              const uint32_t z[8] = {pl[8 * c], pl[8 * c + 1], pl[8 * c + 2], pl[8 * c + 3], pl[8 * c + 4], pl[8 * c + 5], pl[8 * c + 6], pl[8 * c + 7]};
+              tc_st8(tlane + W::t_p + W::TILE / 2 + half * (COLS / 2) + 8 * c, z);
+            }
+          }
+          tc_wait_st();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) arrive1(bar(B_P_FULL));
+        }
       }
-    }
     }
     if (my_tiles) ok = ok && __all_sync(0xffffffffu, mb_wait(bar(B_PV_DONE + (W::QT == 2 ? 2u * qt + 1u : 0u)), (n_tiles - 1u) & 1u, kWait));
     if (!ok && lane == 0) *fail = 1;
@@ -645,14 +646,14 @@ __global__ void __launch_bounds__(Wide<HD, T>::THREADS, 1) sdpa_q8_wide_kernel(c
         }
       } else {
         raw += W::TILE * HD;
-        // eight positions and four dims a lane; dim 4 w + j becomes column j HD / 4 + w of O, so that neighbouring lanes write neighbouring chunks.  With
-        // two row tiles the halves of a tile are handed on one by one
-        constexpr unsigned PIECES = W::QT, WORDS = HD / 4, PARTS = WORDS >= 32 ? WORDS / 32 : 1, PG = WORDS >= 32 ? 1 : 2, STEPS = W::TILE / PIECES / 8 * WORDS / 32, PER = STEPS / W::CONV_V;
+        // eight positions and four dims a lane; dim 4 w + j becomes column j HD / 4 + w of O, so that neighbouring lanes write neighbouring chunks.  A lone
+        // buffer's halves are handed on one by one
+        constexpr unsigned PIECES = W::PIECES, WORDS = HD / 4, PARTS = WORDS >= 32 ? WORDS / 32 : 1, PG = WORDS >= 32 ? 1 : 2, STEPS = W::TILE / PIECES / 8 * WORDS / 32, PER = STEPS / W::CONV_V;
         static_assert(STEPS % W::CONV_V == 0, "steps of a warp");
         bool there = true;
 #pragma unroll
         for (unsigned h = 0; h < PIECES; h++) {
-          const unsigned b = W::QT == 2 ? h : i % W::NV, turn = W::QT == 2 ? i : i / W::NV;  // the buffer, and which time it is used
+          const unsigned b = PIECES == 2 ? h : i % W::NV, turn = PIECES == 2 ? i : i / W::NV;  // the buffer, and which time it is used
           if (turn > 0u && !__all_sync(0xffffffffu, mb_wait(bar(B_V_FREE + b), (turn - 1u) & 1u, kWait))) {
             there = false;
             break;
@@ -738,21 +739,25 @@ __global__ void __launch_bounds__(Wide<HD, T>::THREADS, 1) sdpa_q8_wide_kernel(c
             tc_fence_after();
             scores(i + 1u, 0);
           }
-          ok = wait(B_V_FULL + i % W::NV, i / W::NV) && wait(B_P_FULL, i);
+          ok = wait(B_P_FULL, i);
           if (!ok) continue;
-          tc_fence_after();
-          const uint32_t v = d_v + i % W::NV * (W::kv_bytes / 16u);
-          if constexpr (W::TERMS == 2) {
 #pragma unroll
-            for (unsigned ks = 0; ks < W::TILE / 16u; ks++) issue_ts(leader, W::t_o, W::t_p + W::TILE / 2 + 8u * ks, v + 2u * ks * HD, idesc_o, ks ? 1u : 0u);
+          for (unsigned h = 0; h < W::PIECES; h++) {
+            const unsigned b = W::PIECES == 2 ? h : i % W::NV;
+            ok = ok && wait(B_V_FULL + b, W::PIECES == 2 ? i : i / W::NV);
+            if (!ok) continue;
+            tc_fence_after();
+            const uint32_t v = d_v + b * (W::kv_bytes / W::PIECES / 16u);
+            constexpr unsigned STEPS = W::TILE / 16 / W::PIECES;
+            if constexpr (W::TERMS == 2)
 #pragma unroll
-            for (unsigned ks = 0; ks < W::TILE / 16u; ks++) issue_ts(leader, W::t_o, W::t_p + 8u * ks, v + 2u * ks * HD, idesc_o, 1u);
-          } else {
+              for (unsigned ks = 0; ks < STEPS; ks++) issue_ts(leader, W::t_o, W::t_p + W::TILE / 2 + 8u * (h * STEPS + ks), v + 2u * ks * HD, idesc_o, h | ks ? 1u : 0u);
 #pragma unroll
-            for (unsigned ks = 0; ks < W::TILE / 16u; ks++) issue_ts(leader, W::t_o, W::t_p + 8u * ks, v + 2u * ks * HD, idesc_o, ks ? 1u : i);
+            for (unsigned ks = 0; ks < STEPS; ks++) issue_ts(leader, W::t_o, W::t_p + 8u * (h * STEPS + ks), v + 2u * ks * HD, idesc_o, W::TERMS == 2 || h | ks ? 1u : i);
+            commit_if(leader, base + 8u * (B_V_FREE + b));
           }
+          if (!ok) continue;
           commit_if(leader, base + 8u * B_PV_DONE);
-          commit_if(leader, base + 8u * (B_V_FREE + i % W::NV));
         }
       }
       if (leader) {  // every product issued must finish before shared and tensor memory go away (bounded)
