@@ -29,8 +29,8 @@ namespace {
 // each, as much again as rounding the result: 2.9e-4 against 2.1e-4 of a plain f32 form, both off 64 bits), values accumulate in the MMAs.
 // The maximum that probabilities refer to moves only when a score exceeds it by 2^4.
 //
-// Bound by: many long contexts by memory (48 sequences of about 6800 positions, f16, 32 heads on 8 of 128: 664 MB in 109 us, 93 % of the measured copy
-// rate; with 16 x 64 score tiles on the untransposed products and three block barriers a tile it was 314).  Turning codes into f16 is
+// Bound by: many long contexts by memory (48 sequences of about 6800 positions, f16, 32 heads on 8 of 128: 664 MB in 110 us, 93 % of the measured copy
+// rate, and in 124 over seconds at the power limit, 1.66 GHz; with 16 x 64 score tiles on the untransposed products and three block barriers a tile it was 314).  Turning codes into f16 is
 // most of what is issued: 5 instructions per 4 codes of K, 7 of V, half the issue slots.  A lone short context by its chain: 700 positions
 // (f32, 8 heads on 1 of 256) 10 us with the merge: lengths and counts 1.0, page, q and first codes 1.4, 16 positions 1.3, the warps' results 1.3,
 // merge and launches the rest.  Four slots of 1024 to 16384 positions (f32, 2 KV heads): 38.8 MB in 19.1 us, four steps of 1.4 us in the middle.
