@@ -381,13 +381,6 @@ def _plain(s):
 # ---- the framework's operators -------------------------------------------------------------------------
 
 _CTX = []
-_TMP = []                   # one attention workspace, kept and grown: every call here is on the context's one stream
-
-
-def _workspace(ctx, floats):
-    if not _TMP or _TMP[0].nbytes < 4 * floats:
-        _TMP[:] = [ctx.buffer_empty_f32(floats)]
-    return _TMP[0]
 
 
 def _handles(s):
@@ -411,8 +404,7 @@ def _handles(s):
     if s.kind != "tables":
         h.cache = Q8Cache(ctx, s.n_pages, s.page, s.n_kv, s.hd, I8 if s.fmt == "i8" else E4M3, k=buf(s.K), v=buf(s.V), k_scale=buf(s.ks), v_scale=buf(s.vs))
     if s.kind == "attention":
-        h.tmp_floats = h.eng.sdpa_paged_tmp_floats(ctx, h.cache, h.tables, s.n_q, s.rows_most)
-        _workspace(ctx, h.tmp_floats)
+        h.tmp = ctx.buffer_empty_f32(h.eng.sdpa_paged_tmp_floats(ctx, h.cache, h.tables, s.n_q, s.rows_most))
     return h
 
 
@@ -429,7 +421,7 @@ def _framework(s):
     elif s.kind == "norm_append":
         eng.rmsnorm_per_head_qkv_q8(ctx, h.cache, h.tables, s.n_q, EPS, h.q, h.qw, h.rope, h.k, h.kw, h.v, h.q_out)
     elif s.kind == "attention":
-        eng.sdpa_paged_q8(ctx, h.cache, h.tables, s.n_q, s.rows_most, s.ctx_most, h.q, _workspace(ctx, h.tmp_floats), h.out, s.scale, s.window)
+        eng.sdpa_paged_q8(ctx, h.cache, h.tables, s.n_q, s.rows_most, s.ctx_most, h.q, h.tmp, h.out, s.scale, s.window)
     if s.kind in ("append", "norm_append", "read"):
         (h.f16 if s.kind == "norm_append" else eng).kv_read_q8(ctx, h.cache, s.rows, h.tables.plan, h.tables.row_slot, h.k_back, h.v_back)
 
