@@ -7,7 +7,8 @@
 //   converters  codes -> f16 (exact) core matrices: K as positions x dims, V transposed as dims x positions, by warps of their own;
 //   products    S = q K^T into tensor memory and O (+)= P V with P out of tensor memory;
 //   softmax     eight warps: S -> mask, maximum, probabilities -> P.
-// The maximum that probabilities refer to moves only when a score exceeds it by 2^4.
+// The maximum that probabilities refer to moves only when a score exceeds it by 2^4; it is one of scores and V's scales alone, the probabilities' 2^10 comes
+// behind it (in the exponent, f16, or as a factor, f32).
 //   f16   q as it is, P rounded to f16, O stays in tensor memory and is rescaled there when the maximum moves.  Two row tiles share the converted
 //         codes (a conversion is worth half the softmax); a thread has a row.  They fill tensor memory: P lies in the place of its scores, half a tile
 //         (64 positions) at a time.  While the softmax has one half, the other's values and the next scores in its place are made, for each row tile by a
@@ -430,7 +431,7 @@ __global__ void __launch_bounds__(Wide<HD, T>::THREADS, 1) sdpa_q8_wide_kernel(c
           }
           // 16 columns' exponentials run while the 16 before are summed, packed and stored (in the scores' place)
           auto powers = [&](int c) {
-            const float d = sc[c].y - ref;
+            const float d = sc[c].y + (kProbsLog2 - ref);
             const uint64_t ff = pair(sc[c].x, sc[c].x), dd = pair(d, d);
 #pragma unroll
             for (int e = 0; e < 16; e += 2) {
@@ -506,7 +507,7 @@ __global__ void __launch_bounds__(Wide<HD, T>::THREADS, 1) sdpa_q8_wide_kernel(c
 #pragma unroll
         for (int c = 0; c < COLS / 16; c++) {
           const float4 sc = scale[c];
-          const float f = factor(sc.x), d = sc.y - ref;
+          const float f = factor(sc.x), d = sc.y + (W::TERMS == 1 ? kProbsLog2 - ref : -ref);
           const uint64_t ff = pair(f, f), dd = pair(d, d);
           uint64_t sum = 0;
 #pragma unroll
@@ -808,7 +809,7 @@ __global__ void __launch_bounds__(Wide<HD, T>::THREADS, 1) sdpa_q8_wide_kernel(c
           float4 w;
           if constexpr (W::TERMS == 1) {
             const float x = q8_scale(sc.y);
-            w = make_float4(f, __log2f(x) + kProbsLog2, 0.0f, 1.0f / (x * kProbs));
+            w = make_float4(f, __log2f(x), 0.0f, 1.0f / (x * kProbs));
           } else {
             float e, mant, down;
             split_scale(q8_scale(sc.y), e, mant, down);
