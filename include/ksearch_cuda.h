@@ -267,7 +267,9 @@ int ks_pages_trim(ks_ctx* ctx, const ks_page_tables* t, const ks_buf* keep);
 int ks_kv_append_q8(ks_ctx* ctx, const ks_q8_cache* c, const ks_page_tables* t, ks_dtype act, const ks_buf* k, size_t k_off,
                     const ks_buf* v, size_t v_off, size_t kv_ld);
 /* ks_rmsnorm_per_head_qkv_q40 over such a cache: q per-head RMS * qw and RoPE -> q_out [max_rows, n_q, hd], k RMS * kw and RoPE, v RMS,
- * both appended as ks_kv_append_q8 does.  Row r turns by row row_pos[r] of rope, f32 [*, hd] = cos[hd / 2] || sin[hd / 2]. */
+ * both appended as ks_kv_append_q8 does, with the scales and codes that 64 bits give (where they are within 2^-40 of the middle between two codes
+ * either is right).  What passes f32's range on the way, a product or a row's sum of squares, counts as infinite; a K or V row with NaN, an infinity or such a
+ * sum becomes zeros.  Row r turns by row row_pos[r] of rope, f32 [*, hd] = cos[hd / 2] || sin[hd / 2]. */
 int ks_rmsnorm_per_head_qkv_q8(ks_ctx* ctx, const ks_q8_cache* c, const ks_page_tables* t, size_t n_q, float eps, ks_dtype act, const ks_buf* q,
                                const ks_buf* qw, const ks_buf* rope, const ks_buf* k, const ks_buf* kw, const ks_buf* v, ks_buf* q_out);
 /* Cached rows as numbers: k, v [n_rows, n_kv, hd] in `act` (f16: rounded to nearest) of slots int32 [n_rows] from element slot_off on,

@@ -137,8 +137,10 @@ __device__ __forceinline__ Two plus(Two a, Two b) {
   const float s = __fadd_rn(a.hi, b.hi), t = __fsub_rn(s, a.hi);
   return {s, __fadd_rn(__fadd_rn(__fsub_rn(a.hi, __fsub_rn(s, t)), __fsub_rn(b.hi, t)), __fadd_rn(a.lo, b.lo))};
 }
-// Rounded to one float toward the odd neighbour, so that rounding it again to 8 bits, and comparing it with a limit, give what the sum gives.
+// Rounded to one float toward the odd neighbour, so that rounding it again to 8 bits, and comparing it with a limit, give what the sum gives.  A first term
+// that has passed f32's range (or is NaN) is the result as one float has it; the second one is no error of it any more.
 __device__ __forceinline__ float to_odd(Two x) {
+  if (!(fabsf(x.hi) < INFINITY)) return x.hi;
   const float f = __fadd_rn(x.hi, x.lo), rest = __fsub_rn(x.lo, __fsub_rn(f, x.hi));
   const uint32_t b = __float_as_uint(f);
   if (rest == 0.0f || (b & 1u) || !(fabsf(f) < INFINITY) || f == 0.0f) return f;
