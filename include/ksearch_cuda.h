@@ -257,7 +257,9 @@ int ks_pages_reset(ks_ctx* ctx, const ks_page_tables* t);
 enum { KS_PLAN_OK = 0, KS_PLAN_NO_PAGES = 1, KS_PLAN_TABLE_FULL = 2, KS_PLAN_TOO_MANY_ROWS = 3, KS_PLAN_BAD_LENGTH = 4 };
 int ks_pages_step(ks_ctx* ctx, const ks_page_tables* t, const ks_buf* n_new);
 /* keep int32 [n_seqs]: sequence i ends at keep[i] positions if it holds more (0: it is released; below 0: left as it is); the
- * pages behind go back on the stack, the last page first, so that the step that took them can be taken back exactly. */
+ * pages behind go back on the stack, the last page first, so that the step that took them can be taken back exactly.  An entry that is no
+ * page of the pool leaves its table, is named by the next ks_synchronize and goes back nowhere.  A page belongs to one sequence: the same id
+ * twice in tables that a host wrote is not noticed, and goes back twice. */
 int ks_pages_trim(ks_ctx* ctx, const ks_page_tables* t, const ks_buf* keep);
 /* Rows k, v [max_rows, n_kv, hd] in `act`, kv_ld elements apart (a multiple of 8, at least n_kv * hd; offsets multiples of 8), into
  * the slots of the plan; rows behind the plan's last are not read.  A page's scale is the least power of two that makes its largest

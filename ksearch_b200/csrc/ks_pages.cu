@@ -146,7 +146,7 @@ __global__ void __launch_bounds__(1024) pages_step_kernel(const TablesArgs a, co
   }
 }
 
-// One block: the sum over the sequences, then one page per thread and step.
+// One block: the sum over the sequences, then one page per thread and step.  Ids that no page has stay out of the stack.
 __global__ void __launch_bounds__(1024) pages_trim_kernel(const TablesArgs a, const int* keep) {
   __shared__ unsigned red[32][3];
   __shared__ unsigned first[KS_PAGES_MAX_SEQS], from[KS_PAGES_MAX_SEQS];
@@ -173,6 +173,7 @@ __global__ void __launch_bounds__(1024) pages_trim_kernel(const TablesArgs a, co
     return;
   }
   if (cut) a.lens[tid] = to;
+  bool bad = false;
   for (unsigned k = tid; k < tot[0]; k += blockDim.x) {
     unsigned lo = 0, hi = a.n_seqs;
     while (hi - lo > 1u) {
@@ -182,11 +183,25 @@ __global__ void __launch_bounds__(1024) pages_trim_kernel(const TablesArgs a, co
     }
     int* entry = a.tables + (size_t)lo * a.max_blocks + from[lo] + (k - first[lo]);
     const int id = *entry;
-    if (id < 0 || (unsigned)id >= a.n_pages) atomicOr(a.bad, KS_BAD_PAGE);
+    bad |= (unsigned)id >= a.n_pages;
     a.free_pages[(unsigned)count + tot[0] - k] = id;
     *entry = -1;
   }
-  if (tid == 0) a.free_pages[0] = count + (int)tot[0];
+  unsigned back = tot[0];
+  if (__syncthreads_or(bad)) {  // ids that no page has leave the stack again: the others move down, in their order
+    if (tid == 0) atomicOr(a.bad, KS_BAD_PAGE);
+    back = 0;
+    for (unsigned k0 = 0; k0 < tot[0]; k0 += blockDim.x) {
+      const int id = k0 + tid < tot[0] ? a.free_pages[(unsigned)count + 1u + k0 + tid] : -1;
+      const bool good = (unsigned)id < a.n_pages;
+      unsigned w[3] = {good, 0u, 0u}, n[3];
+      scan3(w, n, red);  // (a barrier inside: this round's ids have been read, and no later one lies where they go)
+      if (good) a.free_pages[(unsigned)count + 1u + back + w[0]] = id;
+      back += n[0];
+      __syncthreads();
+    }
+  }
+  if (tid == 0) a.free_pages[0] = count + (int)back;
 }
 
 __global__ void __launch_bounds__(256) pages_reset_kernel(const TablesArgs a, size_t n_plan) {
