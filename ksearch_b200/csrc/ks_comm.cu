@@ -245,7 +245,8 @@ int ks_comm_p2p_handle(ks_comm* c, void* handle_out) {
   if (!c->box_local) {
     const size_t bytes = 256 + 2 * (size_t)c->n_ranks * sizeof(unsigned long long);
     KS_CUDA(ctx, cudaMalloc((void**)&c->box_local, bytes));
-    KS_CUDA(ctx, cudaMemset(c->box_local, 0, bytes));
+    KS_CUDA(ctx, cudaMemsetAsync(c->box_local, 0, bytes, ctx->stream));
+    KS_CUDA(ctx, cudaStreamSynchronize(ctx->stream));  // the other ranks may write to it as soon as they have the handle
     c->step = reinterpret_cast<unsigned*>(c->box_local + 2 * (size_t)c->n_ranks);
   }
   cudaIpcMemHandle_t h;
@@ -284,8 +285,8 @@ int ks_comm_set(ks_comm* c, int what, unsigned value) {
   else if (what == 1) c->poll_limit = value ? value : 1u;
   else if (what == 2 && c->box_local) {
     cudaSetDevice(c->ctx->device);
-    cudaStreamSynchronize(c->ctx->stream);
-    cudaMemset(c->box_local, 0, 256 + 2 * (size_t)c->n_ranks * sizeof(unsigned long long));
+    KS_CUDA(c->ctx, cudaMemsetAsync(c->box_local, 0, 256 + 2 * (size_t)c->n_ranks * sizeof(unsigned long long), c->ctx->stream));
+    KS_CUDA(c->ctx, cudaStreamSynchronize(c->ctx->stream));
   } else if (what != 2) return KS_ERR_INVALID;
   return KS_OK;
 }

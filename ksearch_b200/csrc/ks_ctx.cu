@@ -67,7 +67,7 @@ ks_ctx* ks_ctx_create(int device, uint64_t flags) {
     delete c;
     return nullptr;
   }
-  if (cudaMalloc(&c->ws, KS_WS_BYTES) != cudaSuccess || cudaMemset(c->ws, 0, KS_WS_BYTES) != cudaSuccess || cudaMalloc(&c->gemm_ws, KS_FEW_WS) != cudaSuccess) {
+  if (cudaMalloc(&c->ws, KS_WS_BYTES) != cudaSuccess || cudaMemsetAsync(c->ws, 0, KS_WS_BYTES, c->stream) != cudaSuccess || cudaMalloc(&c->gemm_ws, KS_FEW_WS) != cudaSuccess) {
     g_create_err = "workspace allocation failed";
     cudaFree(c->ws);
     cudaStreamDestroy(c->stream);
@@ -235,11 +235,13 @@ int ks_synchronize(ks_ctx* c) {
   unsigned words[KS_WS_INDEX_WORD - KS_WS_ERR_WORD + 1] = {0};
   KS_CUDA(c, cudaMemcpy(words, (unsigned*)c->ws + KS_WS_ERR_WORD, sizeof words, cudaMemcpyDeviceToHost));
   const unsigned flag = words[0], index = words[KS_WS_INDEX_WORD - KS_WS_ERR_WORD];
-  if (index) cudaMemset((unsigned*)c->ws + KS_WS_INDEX_WORD, 0, sizeof index);
-  if (flag) {
-    cudaMemset((unsigned*)c->ws + KS_WS_ERR_WORD, 0, sizeof flag);
-    return ks_fail(c, KS_ERR_TIMEOUT, "a device-side wait gave up (status word 0x%x)", flag);
+  // (cleared on the context's stream, in front of all that is enqueued from now on: the default stream is in no order with it)
+  if (index || flag) {
+    ks_on_device on(c);
+    if (index) KS_CUDA(c, cudaMemsetAsync((unsigned*)c->ws + KS_WS_INDEX_WORD, 0, sizeof index, c->stream));
+    if (flag) KS_CUDA(c, cudaMemsetAsync((unsigned*)c->ws + KS_WS_ERR_WORD, 0, sizeof flag, c->stream));
   }
+  if (flag) return ks_fail(c, KS_ERR_TIMEOUT, "a device-side wait gave up (status word 0x%x)", flag);
   if (index)
     return ks_fail(c, KS_ERR_INVALID, "paged cache: an index on the device is out of range:%s%s%s%s%s", index & KS_BAD_PAGE ? " page id" : "", index & KS_BAD_SLOT ? " slot" : "",
                    index & KS_BAD_POSITION ? " position behind the RoPE table" : "", index & KS_BAD_ROWS ? " rows of a sequence" : "", index & KS_BAD_STACK ? " free stack" : "");
