@@ -244,7 +244,10 @@ typedef struct {
  * then, each part from a multiple of 4 words on: row_start [n_seqs + 1] (rows of sequence i: row_start[i] .. row_start[i + 1] - 1),
  * row_seq, row_pos, row_slot [max_rows] (sequence, position and cache slot page_id * page + position % page of a row; -1 behind
  * the last), jobs [max_rows / page + 2 n_seqs][4] (for each touched page: its first row, how many rows of the step lie in it, the first
- * row's slot and position; -1 behind the last).  The plan starts on 16 bytes. */
+ * row's slot and position; -1 behind the last).  The plan starts on 16 bytes.  Words of zeros are a plan without rows.
+ * Lengths, tables and the stack may have several plans of different max_rows (ks_page_tables that share those three buffers; a step fills the one it is
+ * given): what the appends and attention cost grows with max_rows and n_seqs, whatever the step has, so a server keeps a small one for steps that
+ * decode beside that for prompts. */
 enum { KS_PLAN_ROW_START = 0, KS_PLAN_ROW_SEQ = 1, KS_PLAN_ROW_POS = 2, KS_PLAN_ROW_SLOT = 3, KS_PLAN_JOBS = 4, KS_PLAN_END = 5 };
 size_t ks_pages_plan_offset(size_t n_seqs, size_t max_rows, size_t page, int part);  /* first word of a part; 0 for arguments out of range */
 size_t ks_pages_plan_ints(size_t n_seqs, size_t max_rows, size_t page);              /* words of a plan (= offset of KS_PLAN_END) */

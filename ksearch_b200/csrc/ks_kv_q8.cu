@@ -218,7 +218,7 @@ __global__ void __launch_bounds__(1024) append_q8_kernel(const AppendArgs a) {
   const unsigned j = blockIdx.x / per_job, head = blockIdx.x % per_job >> 1;
   const bool vals = blockIdx.x & 1u;
   const int4 job = reinterpret_cast<const int4*>(a.plan + a.at.jobs)[j];
-  if (job.x < 0) return;
+  if (job.x < 0 || job.y == 0) return;  // (no rows: words of zeros, a plan that no step has filled yet)
   const unsigned row0 = (unsigned)job.x, rows = (unsigned)job.y, slot = (unsigned)job.z, off = slot & (page - 1u);
   if (job.z < 0 || slot >= a.n_slots || rows > page - off || row0 >= a.max_rows || rows > a.max_rows - row0) {
     if (threadIdx.x == 0) atomicOr(a.bad, KS_BAD_SLOT);

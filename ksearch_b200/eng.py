@@ -194,8 +194,9 @@ class CudaContext:
 class PageTables:
     """Lengths, page tables, the stack of free pages and the plan of up to ``n_seqs`` sequences (``ks_page_tables``).
 
-    Buffers that are not given are allocated, and everything is emptied then.  ``plan_part`` says where a part of the
-    plan starts; ``row_slot`` is the one that a read-back takes."""
+    Buffers that are not given are allocated; if all are, everything is emptied.  With another's ``lens``, ``tables`` and ``free``
+    it is one more plan over the same sequences (without rows until its first step).  ``plan_part`` says where a part of
+    the plan starts; ``row_slot`` is the one that a read-back takes."""
 
     ROW_START, ROW_SEQ, ROW_POS, ROW_SLOT, JOBS, END = range(6)
     STATUS = ("ok", "not enough free pages", "a sequence would outgrow its table", "more rows than max_rows", "a bad count or length")
