@@ -286,7 +286,12 @@ int ks_kv_read_q8(ks_ctx* ctx, const ks_q8_cache* c, size_t n_rows, const ks_buf
  * scale * (q . k).  Only row_start, the lengths and the tables are read: a host may write its own.  rows_most: no sequence has
  * more rows (0: nothing is done); ctx_most: the longest context to expect (a hint for how the work is split).  Rows behind the last
  * sequence are left as they are.  tmp: ks_sdpa_paged_tmp_floats() f32, not shared with work that may overlap.  n_seqs, max_blocks and
- * n_kv together have a limit (KS_ERR_UNSUPPORTED): n_seqs * n_kv * max_blocks * page below 2^36. */
+ * n_kv together have a limit (KS_ERR_UNSUPPORTED): n_seqs * n_kv * max_blocks * page below 2^36.
+ * Precision.  f32: q and the probabilities are two f16 terms each, sums are f32.  f16: the probabilities are rounded to f16 once (2^-11 of each), and
+ * the products with V are summed up in the tensor cores' f32 accumulators, which round toward zero: sums of one sign over one block's positions came out smaller by 2^-16 at
+ * 8192 of them and by 2^-11.5, about as much as rounding the result to f16, at 65536 (many rows behind 131072 positions; few rows: 2^-17.5 there).  Either
+ * way a probability below 2^-24 of the largest is kept to 2^-35 of that one, where "largest" counts V's scale with it (2^-60 at least), and the sum of
+ * probabilities loses what is below 2^-126 in that measure: V scales that one row sees may differ by 2^100. */
 size_t ks_sdpa_paged_tmp_floats(const ks_ctx* ctx, const ks_q8_cache* c, const ks_page_tables* t, size_t n_q, size_t rows_most);
 int ks_sdpa_paged_q8(ks_ctx* ctx, const ks_q8_cache* c, const ks_page_tables* t, size_t n_q, size_t rows_most, size_t ctx_most, size_t window,
                      float scale, ks_dtype act, const ks_buf* q, ks_buf* tmp, ks_buf* out);

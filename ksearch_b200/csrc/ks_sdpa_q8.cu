@@ -5,7 +5,7 @@
 // With v_j = vs_j c_j, vs_j = 2^e f (1 <= f < 2) the scale of its page, everything runs on t_j = s_j log2(e) + e and the codes c_j:
 //   w_j = 2^(t_j - M) f,   out = sum w_j c_j / sum 2^(t_j - M) 2^-e,   M = max_j t_j:
 // weights are below 2^5 whatever the scales (they are rounded to f16 with 2^10 in front), and a sequence whose pages differ by powers of ten
-// keeps what carries the sum.
+// keeps what carries the sum.  e is -60 at least (f takes the rest): the sum's terms would be lost below 2^-126 of the largest t.
 //
 // This file: sequences of up to few_of() rows times query heads of a group, and the merge; ks_sdpa_q8_wide.cu: the others.
 #include "ks_sdpa_q8.cuh"

@@ -91,14 +91,14 @@ __device__ __forceinline__ void put_dims(__half* to, const float* v, int n) {
   if (n == 4) *reinterpret_cast<uint2*>(to) = make_uint2(x, q8_u32(__floats2half2_rn(v[2], v[3])));
   else *reinterpret_cast<uint32_t*>(to) = x;
 }
-// A positive scale (inside q8_scale's range) as 2^e and a factor of 1 to 2.
+// A positive scale (inside q8_scale's range) as 2^e and a factor of 1 to 2, or below 1 where e is kLeastV: the least one, so that a page of zeros (2^-100)
+// beside values of 2^50 still leaves its probabilities in the sum, which carries 2^(t - M) 2^-e with t - M down to -126.
+constexpr int kLeastV = -60;
 __device__ __forceinline__ void split_scale(float s, float& e, float& factor, float& down) {
-  const uint32_t b = __float_as_uint(s);
-  const int x = (int)(b >> 23) - 127;
+  const int x = max((int)(__float_as_uint(s) >> 23) - 127, kLeastV);
   e = (float)x;
-  factor = __uint_as_float((b & 0x7FFFFFu) | 0x3F800000u);
   down = __uint_as_float((uint32_t)(127 - x) << 23);
+  factor = s * down;
 }
-
 
 }  // namespace

@@ -9,7 +9,8 @@
 //   softmax     eight warps: S -> mask, maximum, probabilities -> P.
 // The maximum that probabilities refer to moves only when a score exceeds it by 2^4; it is one of scores and V's scales alone, the probabilities' 2^10 comes
 // behind it (in the exponent, f16, or as a factor, f32).
-//   f16   q as it is, P rounded to f16, O stays in tensor memory and is rescaled there when the maximum moves.  Two row tiles share the converted
+//   f16   q as it is, P rounded to f16 (2^-11 of each, as much as the result's rounding), O stays in tensor memory and is rescaled there when the maximum moves.
+//         Its accumulator rounds toward zero, which takes 2^-23.5 of the sum a product of 16 positions: 2^-16 after 8192 positions of one sign, 2^-11.5 after 65536.  Two row tiles share the converted
 //         codes (a conversion is worth half the softmax); a thread has a row.  They fill tensor memory: P lies in the place of its scores, half a tile
 //         (64 positions) at a time.  While the softmax has one half, the other's values and the next scores in its place are made, for each row tile by a
 //         warp of its own.
@@ -808,7 +809,7 @@ __global__ void __launch_bounds__(Wide<HD, T>::THREADS, 1) sdpa_q8_wide_kernel(c
           const float f = fmaxf(q8_scale(sc.x) * fabsf(a.scale) * 1.44269504088896340736f, 1.0e-37f);
           float4 w;
           if constexpr (W::TERMS == 1) {
-            const float x = q8_scale(sc.y);
+            const float x = fmaxf(q8_scale(sc.y), 0x1p-60f);  // (as kLeastV: below f16's range whatever the code)
             w = make_float4(f, __log2f(x), 0.0f, 1.0f / (x * kProbs));
           } else {
             float e, mant, down;

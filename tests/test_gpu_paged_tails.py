@@ -41,7 +41,8 @@ def attend(ctx, p, c, n_q, act, q, most, announced, scale):
 
 def least_that_counts(c, table, length, rows, q, scale):
     """Probabilities are stored as f16 with 2^10 in front, relative to the largest exp2(score + log2 of V's scale): one below 2^-14 of the
-    format is off by 2^-25 at most, which is 2^-35 of that largest.  Over all codes, and over the sum of exponentials."""
+    format is off by 2^-25 at most, which is 2^-35 of that largest.  Over all codes, and over the sum of exponentials.  V's scales count as 2^-60
+    at least in the exponent."""
     n_q, hd = q.shape[1:]
     G = n_q // c.n_kv
     off = np.zeros(q.shape)
@@ -49,7 +50,7 @@ def least_that_counts(c, table, length, rows, q, scale):
     for h in range(c.n_kv):
         K = c.values(0, pages, h)[:length]
         codes = np.abs(ref.decode(c.codes[1][pages, h], c.fmt).reshape(-1, hd)[:length])
-        vs = np.log2(np.repeat(c.scales[1][pages, h], c.page)[:length])
+        vs = np.log2(np.maximum(np.repeat(c.scales[1][pages, h], c.page)[:length], 2.0 ** -60))
         for r in range(rows):
             seen = length - rows + r + 1
             for g in range(G):
@@ -59,11 +60,11 @@ def least_that_counts(c, table, length, rows, q, scale):
     return off
 
 
-def check(c, table, length, rows, q, scale, got, act):
+def check(c, table, length, rows, q, scale, got, act, tiny=1e-30):
     """run_attention's tolerance (tests/test_gpu_paged_cache.py), and what the smallest probabilities add."""
     want, spread, weight = ref.attention(c, table, length, rows, q, scale, 0)
     d = 2.0 ** -19 * spread[..., None]
-    tol = weight * (2 * d + (2.0 ** -18 if act == F32 else 2.0 ** -11 + 2.0 ** -15)) + (1e-30 if act == F32 else np.abs(want) * 2.0 ** -11 + 2.0 ** -25)
+    tol = weight * (2 * d + (2.0 ** -18 if act == F32 else 2.0 ** -11 + 2.0 ** -15)) + (tiny if act == F32 else np.abs(want) * 2.0 ** -11 + 2.0 ** -25)
     tol = tol + least_that_counts(c, table, length, rows, q, scale)
     err = np.abs(got - want)
     assert (err <= tol).all(), (float((err / tol).max()), np.argwhere(err > tol)[:3].tolist())
@@ -147,3 +148,56 @@ def test_flat_sums_over_131072_positions(ctx, n_q, hd, rows):
         want = w @ V[:seen] / w.sum()
         d = 2.0 ** -19 * (np.abs(K[:seen]) @ np.abs(x)).max() * scale
         assert (np.abs(got[r, g] - want) <= want * (2 * d + 2.0 ** -11 + 2.0 ** -15 + 2.0 ** -11)).all(), (r, g, float((np.abs(got[r, g] - want) / want).max()), float(((got[r, g] - want) / want).mean()))
+
+
+@pytest.mark.parametrize("act", [F32, F16])
+@pytest.mark.parametrize("fmt", [I8, E4M3])
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("rows", [FEW, MANY])
+def test_pages_of_zeros_beside_large_values(ctx, act, fmt, hd, rows):
+    """One page of large V among pages whose V is all zero, which an append gives the least scale, 2^-100: the zeros' probabilities count in full.
+    f32: values of some 2^35; f16: up to the format's end.  The large page leads by 0 to 18 bits, so that its 16 positions have from 1/128
+    to 99 % of the sum."""
+    rng = np.random.default_rng(hd + 3 * rows)
+    page, n_q, length = 16, 2, 2048 + rows
+    n_pages = -(-length // page)
+    p, tables = tables_of(ctx, rng, [length], [rows], page, n_pages)
+    c = CachePair(ctx, n_pages, page, 1, hd, fmt)
+    large = tables[0, 3]
+    c.cpu.codes[0][:] = 0
+    c.cpu.codes[0][large, 0, :, 0] = ref.encode(np.array(64.0), fmt)
+    c.cpu.scales[0][:] = 2.0 ** -6
+    c.cpu.codes[1][:] = 0
+    c.cpu.scales[1][:] = 2.0 ** -100
+    c.cpu.codes[1][large, 0] = ref.encode(np.abs(rng.normal(0, 16, (page, hd))).clip(1, 60), fmt)
+    c.cpu.scales[1][large, 0] = 2.0 ** 30 if act == F32 else 2.0 ** 10
+    upload(ctx, c)
+    q = rng.normal(0, 1, (rows, n_q, hd))
+    q[..., 0] = 1
+    q = q.astype(NP[act])
+    for lead in (0, 10, 18):
+        scale = float(np.float32(lead * np.log(2)))
+        got = attend(ctx, p, c, n_q, act, q, rows, 1 << 20, scale)
+        check(c.cpu, tables[0], length, rows, q.astype(np.float64), scale, got, act)
+
+
+@pytest.mark.parametrize("fmt", [I8, E4M3])
+@pytest.mark.parametrize("hd", [64, 256])
+@pytest.mark.parametrize("rows", [FEW, MANY])
+def test_small_values_everywhere_in_f32(ctx, fmt, hd, rows):
+    """V of 2^-65 throughout, and beside scales of 2^-60."""
+    rng = np.random.default_rng(hd)
+    page, n_q, length = 32, 2, 700
+    n_pages = -(-length // page)
+    p, tables = tables_of(ctx, rng, [length], [rows], page, n_pages)
+    c = CachePair(ctx, n_pages, page, 1, hd, fmt)
+    unit = 32.0 if fmt == I8 else 110.0
+    for w in range(2):
+        c.cpu.codes[w][:] = ref.encode(rng.normal(0, unit, c.cpu.codes[w].shape), fmt)
+    c.cpu.scales[0][:] = 2.0 ** -6
+    q = rng.normal(0, 1, (rows, n_q, hd)).astype(np.float32)
+    for least, most in ((-70, -70), (-72, -56)):
+        c.cpu.scales[1][:] = 2.0 ** rng.integers(least, most + 1, c.cpu.scales[1].shape)
+        upload(ctx, c)
+        got = attend(ctx, p, c, n_q, F32, q, rows, 1 << 20, hd ** -0.5)
+        check(c.cpu, tables[0], length, rows, q.astype(np.float64), hd ** -0.5, got, F32, 0.0)
