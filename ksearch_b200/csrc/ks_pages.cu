@@ -280,6 +280,8 @@ int ks_pages_step(ks_ctx* ctx, const ks_page_tables* t, const ks_buf* n_new) {
   KS_REQUIRE(ctx, ks_fits(n_new, 0, t->n_seqs * 4) && ks_aligned(n_new, 4), "pages_step: n_new buffer too small or not on 4 bytes");
   KS_REQUIRE_DEVICE(ctx, "pages_step");
   ks_on_device on(ctx);
+  // A thread per sequence, and small blocks only where one of them holds all rows.  128 / 256 threads, with a trim in front: 8 rows of 8 sequences 4.37 / 4.45 us,
+  // 512 of 8 4.73 / 4.83, 513 of 8 (two blocks of 128) 5.46 / 4.83, 128 or 512 of 128 4.87 / 4.87 and 4.59 / 4.59, 16000 of 128 8.61 / 8.52.
   const unsigned threads = round32(t->n_seqs) < 256u ? (t->max_rows <= 512 && t->n_seqs <= 128 ? 128 : 256) : round32(t->n_seqs);
   const size_t blocks = (t->max_rows + 4 * threads - 1) / (4 * threads), most = 64;
   KS_LAUNCH(ctx, pages_step_kernel, (unsigned)(blocks < most ? blocks : most), threads, 0, args_of(ctx, t), (const int*)n_new->dptr);

@@ -675,7 +675,10 @@ int launch_split(ks_ctx* ctx, const ks_sdpa_q8_args& a, unsigned blocks) {
 }
 template <int HD, typename T>
 int launch_split_merge(ks_ctx* ctx, const ks_sdpa_q8_args& a, unsigned blocks) {
-  // many pieces lie in two or three blocks each: small blocks, so that all are there at once
+  // Many pieces lie in two or three blocks each: small blocks, so that all are there at once; few pieces may lie in up to 64 blocks each.  Calls of single rows
+  // with 256 / 1024 threads: 32 sequences of 2000 positions (f16, 8 KV heads of 128) 29.3 / 34.7 us, 48 of about 6800 108 to 110 / 115, one of 16384 (f16, one KV
+  // head of 128: one piece in 64 blocks) 13.2 / 12.0, four of up to 16384 (f32, two of 256) 19.0 / 19.2.  Where few pieces lie in few blocks each the line
+  // stands too high: one of 700 (f32, one of 256) 9.1 / 10.6, 16 of 600 (f16, four of 128) 10.7 / 13.3, 16 of 4000 20.0 / 22.4.
   const size_t pieces = (size_t)a.n_seqs * a.n_kv * ((a.few + 7u) / 8u);
   KS_LAUNCH(ctx, (sdpa_q8_merge_kernel<HD, T>), dim3(blocks, HD / 64), pieces >= blocks / 4 ? 256 : 1024, 0, a);
   return ks_after_launch(ctx, "sdpa_paged_q8 merge");

@@ -9,11 +9,11 @@
 //   softmax     eight warps: S -> mask, maximum, probabilities -> P.
 // The maximum that probabilities refer to moves only when a score exceeds it by 2^4; it is one of scores and V's scales alone, the probabilities' 2^10 comes
 // behind it (in the exponent, f16, or as a factor, f32).
-//   f16   q as it is, P rounded to f16 (2^-11 of each, as much as the result's rounding), O stays in tensor memory and is rescaled there when the maximum moves.
-//         Its accumulator rounds toward zero, which takes 2^-23.5 of the sum a product of 16 positions: 2^-16 after 8192 positions of one sign, 2^-11.5 after 65536.  Two row tiles share the converted
-//         codes (a conversion is worth half the softmax); a thread has a row.  They fill tensor memory: P lies in the place of its scores, half a tile
-//         (64 positions) at a time.  While the softmax has one half, the other's values and the next scores in its place are made, for each row tile by a
-//         warp of its own.
+//   f16   q as it is, P rounded to f16 (2^-11 of each, as much as the result's rounding), O stays in tensor memory and is rescaled there when the
+//         maximum moves.  Its accumulator rounds toward zero: sums of one sign came out smaller by 2^-17 to 2^-16 after 8192 positions, by 2^-11.5 after 65536.
+//         Two row tiles share the converted codes (a conversion is worth half the softmax); a thread has a row.  They fill tensor memory: P lies in
+//         the place of its scores, half a tile (64 positions) at a time.  While the softmax has one half, the other's values and the next scores in its
+//         place are made, for each row tile by a warp of its own.
 //   f32   q (first term in tensor memory, second in shared memory) and P are two f16 terms each, small terms first, and O leaves tensor memory
 //         after every tile for f32 registers, because its accumulator drops the low bits of what is added.  Two threads share a row and agree by
 //         one vote a tile.  (f16 heads of 256 run this way too, with one term and O left where it is.)
