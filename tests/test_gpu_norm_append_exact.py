@@ -231,3 +231,43 @@ def test_products_that_pass_the_range_of_f32(ctx, fmt, hd, n_kv, page):
     held = ref.decode(got[0][0], fmt)
     for (_, pos, slot) in p.cpu.rows:
         assert (np.abs(held[slot // page, :, slot % page][:, [m, m + hd // 2]]) == ref.QMAX[fmt]).all()
+
+
+@gpu
+@pytest.mark.parametrize("act", [F32, F16])
+@pytest.mark.parametrize("fmt", [I8, E4M3])
+@pytest.mark.parametrize("hd,n_kv,page", HEADS)
+def test_pages_that_are_continued(ctx, act, fmt, hd, n_kv, page):
+    """Steps that go on in a page, flat rows first and rows with a large value behind them: the scale grows, and the earlier codes are rounded again as
+    the definition says."""
+    rng = np.random.default_rng(hd * 3 + page)
+    p, c = Pair(ctx, 3, 4, 12, page, 2 * page), CachePair(ctx, 12, page, n_kv, hd, fmt)
+    eng, T = Eng(act), 2 * page
+    ang = rng.uniform(0, 6, (4 * page, hd // 2))
+    rope = np.concatenate([np.cos(ang), np.sin(ang)], 1).astype(np.float32)
+    kw = rng.uniform(0.8, 1.2, hd).astype(NP[act])
+    fixed = [ctx.buffer_bytes(x) for x in (np.ones((T, 1, hd), NP[act]), np.ones(hd, NP[act]), rope)]
+    grown = 0
+    for i, new in enumerate(([page // 2, 3, 0], [1, page // 4, 2], [2, 1, page // 2], [page // 2, 1, 1], [1, 0, page])):
+        p.step(new)
+        n = len(p.cpu.rows)
+        k, v = (rng.uniform(-1, 1, (T, n_kv, hd)) for _ in range(2))
+        if i:
+            for x in (k, v):
+                x[:n, :, rng.integers(0, hd)] *= 3.0 ** i
+        k, v = k.astype(NP[act]), v.astype(NP[act])
+        eng.rmsnorm_per_head_qkv_q8(ctx, c.gpu, p.gpu, 1, EPS, *fixed, ctx.buffer_bytes(k), ctx.buffer_bytes(kw), ctx.buffer_bytes(v), ctx.buffer_empty_bytes(4 * T * hd))
+        cs = rope[[r[1] for r in p.cpu.rows]].astype(np.float64)
+        rows = [ref.norm_rope(k[:n], kw, cs, EPS), ref.norm_rope(v[:n], None, None, EPS)]
+        held = [s.copy() for s in c.cpu.scales]
+        c.cpu.append(p.cpu, *rows)
+        got = c.read()
+        same(p, c, rows, got, page, fmt)
+        for w in range(2):
+            for _, _, slot, _ in p.cpu.jobs:
+                pg, off = divmod(int(slot), page)
+                assert np.array_equal(ref.decode(got[0][w][pg, :, :off], fmt), ref.decode(c.cpu.codes[w][pg, :, :off], fmt))
+                grown += int(off > 0 and (c.cpu.scales[w][pg] > held[w][pg]).any())
+            c.cpu.codes[w][:] = got[0][w]
+    assert grown >= 4
+    ctx.synchronize()
